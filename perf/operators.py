@@ -323,7 +323,7 @@ def _own(s):
         r = ops.token_logprobs(s["logits"], s["tokens"], **how)
         out = {"logprobs": r.logprobs, "entropy": r.entropy}
         if c["backward"]:
-            out["grad"] = ops.token_logprobs_grad(s["logits"], s["tokens"], r.stats, s["d_logprobs"], s["d_entropy"], **how)
+            out["grad"] = ops.token_logprobs_grad(s["logits"], s["tokens"], r, s["d_logprobs"], s["d_entropy"], **how)
         return out
     if c["op"] == "top":
         r = ops.top_logits(s["logits"], c["k"], **how)
