@@ -239,6 +239,92 @@ bs_status bs_sample_static(const bs_config *cfg, uint64_t *d_rng, const float *d
                            uint32_t rows, uint32_t vocab, const uint32_t *d_prev, uint32_t n_prev,
                            uint32_t *d_out, void *stream);
 
+/* Operators on rows of logits beside the sampler.  No counterpart in the
+ * reference, whose logits only ever become tokens.  All take the logits as a
+ * descriptor, see each row through the sampler's logit prologue and
+ * temperature,
+ *     z_j = c(v_j) / (logit_scale T),  c(v) = cap tanh(v / cap) or v,
+ *     p_j = exp(z_j - lse),            lse = log sum_j exp(z_j),
+ * and are stream-ordered: the pointers' device must be the current one, and
+ * a call returns once the work is enqueued.  They hold no state, so any
+ * number of calls may run at once.  The sums are f32, in an order fixed by
+ * the sizes and the alignment: the same call gives the same bits.
+ *
+ * Logits of -inf are masked tokens (p = 0, gradient 0 without a soft-cap); a
+ * NaN or +inf logit makes its row NaN; a row all of -inf has no distribution
+ * and is NaN too.  Gradients are of the logits' type, rounded once from f32;
+ * d_grad may be the logits themselves (same pointer, ld_grad = ld) and must
+ * not overlap them in any other way. */
+typedef enum bs_dtype { BS_F32 = 0, BS_BF16 = 1, BS_F16 = 2 } bs_dtype;
+typedef struct bs_logits {
+    const void *data;                /* row i at element i * ld               */
+    size_t ld;                       /* >= vocab, in elements                 */
+    uint32_t rows;                   /* 0: nothing is done (a loss is 0)      */
+    uint32_t vocab;                  /* 1 .. BS_MAX_VOCAB                     */
+    uint32_t dtype;                  /* bs_dtype                              */
+    float temperature;               /* finite, > 0                           */
+    float final_logit_softcapping;   /* <= 0: off                             */
+    float logit_scale;               /* >= 0; 1 or 0: off                     */
+} bs_logits;
+#define BS_MAX_VOCAB 1048576
+#define BS_MAX_TOP 1024
+
+/* Log-probability z_t - lse of each row's token and the row's entropy
+ * -sum p log p.  d_entropy and d_stats may be NULL; d_stats (rows x 2, 8-byte
+ * aligned) gets the row's maximum of c(v) and log sum exp(z - max z), what
+ * bs_token_logprobs_grad starts from.  A row whose token is outside the
+ * vocabulary (-1, or the sampler's 0xFFFFFFFF) is left out: zeros. */
+bs_status bs_token_logprobs(const bs_logits *x, const int32_t *d_tokens, float *d_logprobs, float *d_entropy,
+                            float *d_stats, void *stream);
+
+/* The logits' gradient from the gradients of log-probability and entropy
+ * (either may be NULL, not both), with d_stats and d_entropy of the forward
+ * call on the same logits, tokens and factors.  Rows left out get zeros. */
+bs_status bs_token_logprobs_grad(const bs_logits *x, const int32_t *d_tokens, const float *d_stats,
+                                 const float *d_entropy, const float *d_grad_logprobs, const float *d_grad_entropy,
+                                 void *d_grad, size_t ld_grad, void *stream);
+
+/* The k largest logits of each row in falling order, the lowest id first
+ * among equals (NaN below everything), as c(v) / logit_scale, with their ids;
+ * and the row's lse at the temperature.  k <= BS_MAX_TOP and <= vocab. */
+bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t *d_ids, float *d_lse, void *stream);
+
+/* Distillation from a teacher's top logits: L = sum_k q_k (log q_k - log p_k)
+ * over the row's teacher ids, loss = sum_i w_i L_i, and the loss's gradient.
+ *   d_teacher_ids, d_teacher_logits : rows x n_ids (n_ids <= BS_MAX_TOP);
+ *       an id outside the vocabulary is an empty slot; an id that comes
+ *       twice has the sum of its shares
+ *   d_teacher_lse : NULL, and q is the softmax of teacher_logits / T over the
+ *       row's slots; or rows values, and q_k = exp(t_k / T - lse) with the
+ *       rest of the vocabulary as one more outcome (its share 1 - sum q_k,
+ *       where positive; left out where the student gives the rest no mass)
+ *   d_weights : rows, or NULL for 1 / rows each
+ *   d_row_loss: the L_i;  d_grad: NULL, or d loss / d logits
+ * A row of weight 0 or without a teacher id (or, where q is a softmax, all of
+ * whose teacher logits are -inf) is left out: zeros. */
+bs_status bs_distill_loss(const bs_logits *x, const int32_t *d_teacher_ids, const float *d_teacher_logits,
+                          const float *d_teacher_lse, uint32_t n_ids, const float *d_weights, float *d_loss,
+                          float *d_row_loss, void *d_grad, size_t ld_grad, void *stream);
+
+/* Clipped policy loss of the rows' tokens, with lp their log-probability,
+ * r = exp(lp - old), d = ref - lp:
+ *   L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (exp(d) - d - 1) - entropy_coef H,   loss = sum_i w_i L_i
+ *   d_ref_logprobs : NULL if kl_coef is 0 (then d_kl gets zeros)
+ *   d_weights      : rows, or NULL for 1 / rows each
+ *   d_logprobs, d_entropy, d_kl, d_grad may be NULL
+ * The gradient of the clipped term is zero where the clip binds (r beyond the
+ * bound on the side that A favours).  A row of weight 0 or with a token
+ * outside the vocabulary is left out: zeros. */
+typedef struct bs_policy_config {
+    float clip_low, clip_high;       /* >= 0; +inf: no bound on that side     */
+    float kl_coef, entropy_coef;     /* finite                                */
+} bs_policy_config;
+bs_status bs_policy_loss(const bs_logits *x, const int32_t *d_tokens, const float *d_old_logprobs,
+                         const float *d_advantages, const float *d_ref_logprobs, const float *d_weights,
+                         const bs_policy_config *cfg, float *d_loss, float *d_row_loss, float *d_logprobs,
+                         float *d_entropy, float *d_kl, void *d_grad, size_t ld_grad, void *stream);
+
 void bs_destroy(bs_sampler *s);
 
 const char *bs_status_string(bs_status st);

@@ -3,8 +3,9 @@
 The product is ``libb200_sampler.so`` (CUDA kernels for sm_100a behind the C
 ABI in include/b200_sampler.h).  This package holds its sources (csrc/), the
 build step (build.py), the Python mirror of the reference interface
-(sampler.py), the batch sharding across ranks (sharding.py) and the benchmark
-workloads (workloads.py).
+(sampler.py), the operators on the same rows of logits (logit_ops.py: token
+log-probabilities, top logits, training losses), the batch sharding across
+ranks (sharding.py) and the benchmark workloads (workloads.py).
 
 The directory name contains a dot, so it is loaded by path, e.g.::
 
@@ -16,6 +17,10 @@ The directory name contains a dot, so it is loaded by path, e.g.::
     spec.loader.exec_module(pkg)
 """
 from . import build, sharding, workloads  # noqa: F401
+from .logit_ops import (  # noqa: F401
+    DistillLoss, PolicyLoss, TokenLogprobs, TopLogits, distill_loss, policy_loss, token_logprobs, token_logprobs_grad,
+    top_logits,
+)
 from .sampler import (  # noqa: F401
     EXPORTS, Sampler, SamplerConfig, SamplerError, lib, sample_argmax, status_string,
 )

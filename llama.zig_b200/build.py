@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200_sampler.so")
-SOURCES = ["sampler.cu"]
+SOURCES = ["sampler.cu", "logit_ops.cu"]
 HEADERS = ["bs_math.cuh", "sampler_kernels.cuh"]
 
 NVCC_FLAGS = [

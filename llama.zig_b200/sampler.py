@@ -35,6 +35,7 @@ EXPORTS = [
     "bs_get_rng_state", "bs_set_rng_state", "bs_last_device_status", "bs_destroy",
     "bs_status_string", "bs_profile_enable", "bs_profile_read", "bs_argmax_ex", "bs_set_logit_prologue",
     "bs_sample_static", "bs_seed_state",
+    "bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_distill_loss", "bs_policy_loss",
 ]
 
 
@@ -142,6 +143,15 @@ def lib() -> ctypes.CDLL:
         L.bs_debug_row_traces.argtypes = [vp, vp, ctypes.c_size_t]
         L.bs_profile_enable.argtypes = [vp, u32]
         L.bs_profile_read.argtypes = [vp, vp, u32, ctypes.POINTER(u32)]
+        f32p, sz = vp, ctypes.c_size_t
+        L.bs_token_logprobs.argtypes = [vp, vp, f32p, f32p, f32p, vp]
+        L.bs_token_logprobs_grad.argtypes = [vp, vp, f32p, f32p, f32p, f32p, vp, sz, vp]
+        L.bs_top_logits.argtypes = [vp, u32, f32p, vp, f32p, vp]
+        L.bs_distill_loss.argtypes = [vp, vp, f32p, f32p, u32, f32p, f32p, f32p, vp, sz, vp]
+        L.bs_policy_loss.argtypes = [vp, vp, f32p, f32p, f32p, f32p, vp, f32p, f32p, f32p, f32p, f32p, vp, sz, vp]
+        for name in ("bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_distill_loss",
+                     "bs_policy_loss"):
+            getattr(L, name).restype = ctypes.c_int
         for name in ("bs_create", "bs_sample", "bs_sample_host", "bs_argmax", "bs_argmax_ex",
                      "bs_set_logit_prologue", "bs_get_rng_state",
                      "bs_set_rng_state", "bs_last_device_status", "bs_debug_row_traces",
@@ -330,6 +340,17 @@ class Sampler:
         self._prologue = (float(final_logit_softcapping), float(logit_scale))
         if self._h:
             _check(lib().bs_set_logit_prologue(self._h, *self._prologue), "bs_set_logit_prologue")
+
+    def token_logprobs(self, logits, tokens, stream=None):
+        """Log-probability of each row's token, and the row's entropy, under
+        this sampler's temperature and logit prologue (before the repetition
+        penalty and the filters; a greedy sampler's rows at temperature 1):
+        :func:`token_logprobs` with this sampler's factors."""
+        from .logit_ops import token_logprobs
+        cap, scale = getattr(self, "_prologue", None) or (0.0, 1.0)
+        t = self.cfg.temperature if self.cfg.temperature > 0.0 else 1.0
+        return token_logprobs(logits, tokens, temperature=t, final_logit_softcapping=cap, logit_scale=scale,
+                              stream=stream)
 
     def last_status(self) -> int:
         return lib().bs_last_device_status(self._h)
