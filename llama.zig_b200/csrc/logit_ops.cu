@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -24,9 +25,9 @@
 namespace bs {
 namespace ops {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int MAX_K = 1024;          // most teacher ids of a row, most top logits
+constexpr int MAX_CLUSTER = 8;       // CTAs of a row
 constexpr float LN2 = 0.6931471805599453f;
 constexpr double LN2_D = 0.6931471805599453;
 // 2^d is zero in f32 below this; products with d stop here, so that a logit
@@ -46,6 +47,7 @@ struct RowArgs {
     const void *x;
     size_t ld;
     uint32_t vocab;
+    uint32_t keep;              // 16-byte chunks of a CTA's slice that stay in shared memory
     Scale sc;
     const int32_t *tokens;
     // outputs (null where not asked for)
@@ -92,37 +94,49 @@ template <bool CAP> __device__ __forceinline__ float slope(float c, const Scale 
     return fmaf(-t, t, 1.0f);
 }
 
-// A row as 16-byte chunks of its memory.  The row may start anywhere, so
-// chunk 0 begins up to 15 bytes before it and the last one may end behind it;
-// `head` is the number of elements before the row in chunk 0.
+// A streaming read: the line is the first to leave L2 (and L1) again.
+__device__ __forceinline__ uint4 ld_stream(const void *p) {
+    uint4 q;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p) : "memory");
+    return q;
+}
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &q, float (&v)[16 / sizeof(T)]) {
+    const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); i++) v[i] = to_f(e[i]);
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
+    uint4 q;
+    T *e = reinterpret_cast<T *>(&q);
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); i++) e[i] = from_f<T>(v[i]);
+    return q;
+}
+
+// A row as its body, the 16-byte aligned chunks that lie wholly inside it,
+// and at most E - 1 single elements before and behind the body.
 template <typename T> struct Row {
     static constexpr int E = 16 / sizeof(T);
-    const T *x;          // element 0
-    uint32_t head, vocab, chunks;
-    __device__ Row(const void *base, size_t ld, uint32_t row, uint32_t v) {
-        x = (const T *)base + (size_t)row * ld;
-        head = (uint32_t)(((uintptr_t)x & 15u) / sizeof(T));
-        vocab = v;
-        chunks = (uint32_t)(((uint64_t)head + v + E - 1) / E);
+    const T *x;              // element 0
+    uint32_t vocab;
+    uint32_t lead;           // elements before the body
+    uint32_t chunks;         // of the body
+    uint32_t trail;          // elements behind it
+    __device__ Row(const void *base, size_t ld, uint32_t row, uint32_t v) : x((const T *)base + (size_t)row * ld), vocab(v) {
+        uint32_t head = (uint32_t)(((uintptr_t)x & 15u) / sizeof(T));
+        lead = head ? min(E - head, v) : 0u;
+        chunks = (v - lead) / E;
+        trail = v - lead - chunks * E;
     }
-    __device__ int64_t first(uint32_t c) const { return (int64_t)c * E - head; }
-    __device__ bool whole(uint32_t c) const { return first(c) >= 0 && first(c) + E <= (int64_t)vocab; }
-    // the chunk's logits after the soft-cap; -inf outside the row
-    template <bool CAP> __device__ void load(uint32_t c, const Scale &sc, float (&v)[E]) const {
-        int64_t j0 = first(c);
-        if (whole(c)) {
-            uint4 q = *reinterpret_cast<const uint4 *>(x + j0);
-            const T *e = reinterpret_cast<const T *>(&q);
-#pragma unroll
-            for (int i = 0; i < E; i++) v[i] = capped<CAP>(to_f(e[i]), sc);
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                int64_t j = j0 + i;
-                v[i] = j >= 0 && j < (int64_t)vocab ? capped<CAP>(to_f(x[j]), sc) : -INFINITY;
-            }
-        }
+    // the single element of thread tid (tid < 32): leading ones in lanes
+    // 0.., trailing ones in lanes 8..; -1 where there is none
+    __device__ int32_t edge(uint32_t tid) const {
+        if (tid < lead) return (int32_t)tid;
+        if (tid >= 8 && tid - 8 < trail) return (int32_t)(vocab - trail + tid - 8);
+        return -1;
     }
+    __device__ const T *at(uint32_t chunk) const { return x + lead + (size_t)chunk * E; }
 };
 
 // Running (M, S, U) of a set of logits.
@@ -151,6 +165,64 @@ __device__ __forceinline__ Stat merge(Stat a, const Stat &b, float k) {
     return a;
 }
 
+// What a thread gathers of the logits it reads.  With TAIL, s is the sum over
+// the tokens that are not the teacher's and `top` that over those that are;
+// u is then not kept.
+template <bool ENT, bool TAIL> struct Gather {
+    Stat a{-INFINITY, 0.0f, 0.0f};
+    float top = 0.0f;
+    __device__ __forceinline__ void raise(float m, float k) {
+        if (m > a.m) {
+            if (TAIL) top *= ex2(fmaxf((a.m - m) * k, D_MIN));
+            rebase(a, m, k);
+        }
+    }
+    __device__ __forceinline__ void add(float v, float base, float k, bool marked = false) {
+        const float d = (v - base) * k;
+        const float e = ex2(d);
+        if (TAIL && marked) {
+            top += e;
+        } else {
+            a.s += e;
+            if (ENT) a.u = fmaf(e, max_nan(d, D_MIN), a.u);
+        }
+    }
+    template <int N> __device__ __forceinline__ void chunk(const float (&v)[N], float k, uint32_t marks = 0) {
+        const float base = anchor(a.m);
+#pragma unroll
+        for (int i = 0; i < N; i++) add(v[i], base, k, TAIL && (marks >> i & 1u));
+    }
+};
+template <int N> __device__ __forceinline__ float max_of(const float (&v)[N]) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) m = fmaxf(m, v[i]);
+    return m;
+}
+
+// The CTAs of a row form a cluster.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The address, in CTA `rank` of the cluster, of a shared variable of this one.
+__device__ __forceinline__ uint32_t remote(const void *p, uint32_t rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void st_remote(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
 // log2 S as exponent + log2 of the mantissa: exact to 2^-24 for any S.
 __device__ __forceinline__ double log2_d(float s) {
     if (!(s > 0.0f) || isinf(s)) return (double)log2f(s);
@@ -169,40 +241,105 @@ template <typename V> __device__ __forceinline__ V block_sum(V v, V *scratch) {
     return r;
 }
 
-// One CTA per row: the row's statistics in one pass over its logits, the
-// row's results, then (if asked for) the gradient in a second pass, which
-// finds the row in L2.
+// The sums of all threads of the row's CTAs, in a fixed order, on one scale
+// (with TAIL: s over the rest, u over the teacher's tokens).
+struct RowShared {
+    Stat warp[WARPS];
+    float cta[MAX_CLUSTER][4];
+};
+// RUNS: the caller has made sure that all CTAs of the row run.
+template <bool ENT, bool TAIL, bool RUNS = false>
+__device__ __forceinline__ Stat row_sum(Gather<ENT, TAIL> g, float k, RowShared &sh) {
+    const uint32_t tid = threadIdx.x, ranks = cluster_size();
+    auto fold = [&](Stat a, float top, Stat b, float btop) {
+        // (with TAIL the second sum rides in u; its scale is the same)
+        float m = fmaxf(a.m, b.m);
+        if (TAIL) {
+            float fa = ex2(fmaxf((a.m - m) * k, D_MIN)), fb = ex2(fmaxf((b.m - m) * k, D_MIN));
+            return Stat{m, a.s * fa + b.s * fb, top * fa + btop * fb};
+        }
+        return merge(a, b, k);
+    };
+    Stat a = g.a;
+    if (TAIL) a.u = g.top;
+    for (int o = 16; o; o >>= 1) {
+        Stat b{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.u, o)};
+        // both lanes of a pair fold in the same order: the same bits
+        a = (tid & o) ? fold(b, b.u, a, a.u) : fold(a, a.u, b, b.u);
+    }
+    if ((tid & 31) == 0) sh.warp[tid >> 5] = a;
+    __syncthreads();
+    a = sh.warp[0];
+    for (int i = 1; i < WARPS; i++) a = fold(a, a.u, sh.warp[i], sh.warp[i].u);
+    if (ranks > 1) {
+        if (!RUNS) cluster_wait();   // (the arrival is at the kernel's start: every CTA of the row runs)
+        const uint32_t me = cluster_rank();
+        if (tid < ranks) {
+            st_remote(remote(&sh.cta[me][0], tid), a.m);
+            st_remote(remote(&sh.cta[me][1], tid), a.s);
+            st_remote(remote(&sh.cta[me][2], tid), a.u);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        a = Stat{sh.cta[0][0], sh.cta[0][1], sh.cta[0][2]};
+        for (uint32_t i = 1; i < ranks; i++) a = fold(a, a.u, Stat{sh.cta[i][0], sh.cta[i][1], sh.cta[i][2]}, sh.cta[i][2]);
+    }
+    return a;
+}
+
+// Chunks of a thread in one batch: 8 16-byte loads are under way before the
+// first is used.
+constexpr int BATCH = 8;
+
+// One cluster of CTAs per row, each with a slice of the row's chunks.  First
+// pass: the slice is read once from memory for the row's statistics, and as
+// much of it as fits stays in shared memory (each thread keeps the chunks it
+// read itself, so nothing waits for other threads).  The CTAs exchange their
+// sums through the cluster's shared memory.  Second pass: the gradient, from
+// the kept chunks (what did not fit is read again, mostly from L2).
 template <typename T, int OP, bool CAP>
 __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
     constexpr bool DIST = OP == OP_DISTILL || OP == OP_DISTILL_TAIL;
     constexpr bool TAIL = OP == OP_DISTILL_TAIL;
     constexpr bool POLICY = OP == OP_POLICY || OP == OP_POLICY_ENT;
     constexpr int E = Row<T>::E;
-    extern __shared__ uint32_t dyn[];
-    __shared__ Stat sh_stat[WARPS];
+    extern __shared__ uint4 dyn[];
+    __shared__ RowShared sh;
     __shared__ float sh_f[WARPS];
     __shared__ double sh_d[WARPS];
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, V = A.vocab;
+    const uint32_t ranks = cluster_size(), rank = cluster_rank();
+    const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, V = A.vocab;
+    if (ranks > 1) cluster_arrive();
     const float k = A.sc.k;
     Row<T> R(A.x, A.ld, row, V);
     T *gout = A.grad ? (T *)A.grad + (size_t)row * A.ld_grad : nullptr;
+    // this CTA's chunks of the body; rank 0 also has the single elements
+    const uint32_t per = (R.chunks + ranks - 1) / ranks;
+    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
+    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
 
     const float w = DIST || POLICY ? (A.weights ? A.weights[row] : A.w_all) : 1.0f;
     bool live = w != 0.0f;
     const int32_t tok = DIST ? -1 : A.tokens[row];
     if (!DIST) live = live && (uint32_t)tok < V;
+    const float adv = POLICY ? A.adv[row] : 0.0f, old_lp = POLICY ? A.old_lp[row] : 0.0f;
+    const float ref_lp = POLICY && A.ref_lp ? A.ref_lp[row] : 0.0f;
 
-    // the teacher's slots
-    int32_t *s_id = (int32_t *)dyn;              // n_ids; -1: empty
+    // the teacher's slots; every CTA of the row has them
+    uint4 *kept = dyn;                           // [keep]
+    int32_t *s_id = (int32_t *)(dyn + A.keep);   // n_ids; -1: empty
     float *s_q = (float *)(s_id + A.n_ids);      // share q of the slot
     float *s_c = s_q + A.n_ids;                  // the student's c(v) there
-    uint32_t *s_bits = (uint32_t *)(s_c + A.n_ids);  // tail: one bit per element of the row's chunks
+    uint32_t *s_bits = (uint32_t *)(s_c + A.n_ids);  // tail: one bit per element of the slice
+    const uint32_t e0 = R.lead + c0 * E;         // first element of the slice
+    bool edge_marked = false;
     if (DIST && live) {
         const size_t at = (size_t)row * A.n_ids;
         float umax = -INFINITY;
         bool any = false;
         if (TAIL)
-            for (uint32_t i = tid; i < (R.chunks * E + 31) / 32; i += THREADS) s_bits[i] = 0;
+            for (uint32_t i = tid; i < ((c1 - c0) * E + 31) / 32; i += THREADS) s_bits[i] = 0;
         for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
             int32_t id = A.t_ids[at + i];
             if ((uint32_t)id >= V) id = -1;
@@ -230,7 +367,8 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
                 float q = 0.0f;
                 if (s_id[i] >= 0) {
                     q = expf((float)((double)A.t_logits[at + i] * A.sc.inv_t - ref));
-                    if (TAIL) atomicOr(&s_bits[(R.head + s_id[i]) >> 5], 1u << ((R.head + s_id[i]) & 31));
+                    const uint32_t j = (uint32_t)s_id[i] - e0;
+                    if (TAIL && j < (c1 - c0) * E) atomicOr(&s_bits[j >> 5], 1u << (j & 31));
                 }
                 s_q[i] = q;
                 q_sum += q;
@@ -240,74 +378,95 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
                 for (uint32_t i = tid; i < A.n_ids; i += THREADS) s_q[i] /= total;
             }
             __syncthreads();
+            if (TAIL && edge >= 0)
+                for (uint32_t i = 0; i < A.n_ids; i++) edge_marked |= s_id[i] == edge;
         }
     }
 
+    // 16-byte stores where the gradient's rows are aligned like the logits'
+    const bool wide = gout && (((uintptr_t)(gout + R.lead)) & 15u) == 0;
+    auto store = [&](uint32_t c, const float (&v)[E]) {
+        T *g = gout + R.lead + (size_t)c * E;
+        if (wide) {
+            *reinterpret_cast<uint4 *>(g) = pack<T>(v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; i++) g[i] = from_f<T>(v[i]);
+        }
+    };
+
     if (!live) {  // the row is left out: zeros, and its logits are not read
-        if (tid == 0) {
+        if (rank == 0 && tid == 0) {
             if (A.logprobs) A.logprobs[row] = 0.0f;
             if (A.entropy) A.entropy[row] = 0.0f;
             if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
             if (A.kl) A.kl[row] = 0.0f;
             if (A.row_loss) A.row_loss[row] = 0.0f;
         }
-        if (gout)
-            for (uint32_t j = tid; j < V; j += THREADS) gout[j] = from_f<T>(0.0f);
+        if (gout) {
+            float zero[E] = {};
+            for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, zero);
+            if (edge >= 0) gout[edge] = from_f<T>(0.0f);
+        }
+        if (ranks > 1) cluster_wait();
         return;
     }
 
     const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(R.x[tok]), A.sc);
+    const float c_edge = edge >= 0 ? capped<CAP>(to_f(R.x[edge]), A.sc) : -INFINITY;
 
-    // statistics; with a tail, s is the rest's sum and `top` that of the teacher's ids
-    Stat a{-INFINITY, 0.0f, 0.0f};
-    float top = 0.0f;
-    for (uint32_t c = tid; c < R.chunks; c += THREADS) {
-        float v[E];
-        R.template load<CAP>(c, A.sc, v);
-        float m = v[0];
+    // statistics
+    Gather<!DIST, TAIL> G;
+    const T *body = R.at(0);
+    auto marks = [&](uint32_t c) -> uint32_t {
+        if (!TAIL) return 0u;
+        const uint32_t b = (c - c0) * E;
+        return s_bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
+    };
+    const uint32_t keep_end = gout ? c0 + A.keep : c0;   // the first `keep` chunks stay
+    uint32_t c = c0 + tid;
+    for (; c + (BATCH - 1) * THREADS < c1; c += BATCH * THREADS) {
+        uint4 q[BATCH];
 #pragma unroll
-        for (int i = 1; i < E; i++) m = fmaxf(m, v[i]);
-        if (m > a.m) {
-            if (TAIL) top *= ex2(fmaxf((a.m - m) * k, D_MIN));
-            rebase(a, m, k);
+        for (int u = 0; u < BATCH; u++) q[u] = ld_stream(body + (size_t)(c + u * THREADS) * E);
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            const uint32_t cu = c + u * THREADS;
+            if (cu < keep_end) kept[cu - c0] = q[u];
+            float v[E];
+            unpack<T>(q[u], v);
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = capped<CAP>(v[i], A.sc);
+            G.raise(max_of(v), k);
+            G.chunk(v, k, marks(cu));
         }
-        const float base = anchor(a.m);
-        uint32_t marked = 0;
-        if (TAIL) marked = s_bits[(c * E) >> 5] >> ((c * E) & 31) & ((1u << E) - 1u);
+    }
+    if (c < c1) {   // the slice's end: fewer than BATCH chunks
+        uint4 q[BATCH];
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            float d = (v[i] - base) * k;
-            float e = ex2(d);
-            if (TAIL && (marked >> i & 1u)) {
-                top += e;
-            } else {
-                a.s += e;
-                if (!DIST) a.u = fmaf(e, max_nan(d, D_MIN), a.u);
+        for (int u = 0; u < BATCH; u++)
+            if (c + u * THREADS < c1) q[u] = ld_stream(body + (size_t)(c + u * THREADS) * E);
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            const uint32_t cu = c + u * THREADS;
+            if (cu < c1) {
+                if (cu < keep_end) kept[cu - c0] = q[u];
+                float v[E];
+                unpack<T>(q[u], v);
+#pragma unroll
+                for (int i = 0; i < E; i++) v[i] = capped<CAP>(v[i], A.sc);
+                G.raise(max_of(v), k);
+                G.chunk(v, k, marks(cu));
             }
         }
     }
-    // block: the maximum first, then the sums on one scale
-    float m = a.m;
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    if ((tid & 31) == 0) sh_f[tid >> 5] = m;
-    __syncthreads();
-    for (int i = 0; i < WARPS; i++) m = fmaxf(m, sh_f[i]);
-    if (TAIL) top *= ex2(fmaxf((a.m - m) * k, D_MIN));
-    rebase(a, m, k);
-    if (TAIL) a.u = top;
-    for (int o = 16; o; o >>= 1) {
-        a.s += __shfl_xor_sync(~0u, a.s, o);
-        a.u += __shfl_xor_sync(~0u, a.u, o);
+    if (edge >= 0) {
+        G.raise(c_edge, k);
+        G.add(c_edge, anchor(G.a.m), k, edge_marked);
     }
-    if ((tid & 31) == 0) sh_stat[tid >> 5] = a;
-    __syncthreads();
-    float s = 0.0f, u = 0.0f;
-    for (int i = 0; i < WARPS; i++) {
-        s += sh_stat[i].s;
-        u += sh_stat[i].u;
-    }
-    const float rest = s;
-    if (TAIL) s += u;
+    const Stat st = row_sum(G, k, sh);
+    const float m = st.m, rest = st.s, u = st.u;
+    const float s = TAIL ? st.s + st.u : st.s;
     const double l2s = log2_d(s);
 
     // the row's results and the gradient's coefficients:
@@ -316,16 +475,15 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
     if (!DIST) {
         const double lp = LN2_D * (((double)c_tok - (double)m) * (double)k - l2s);
         const float H = (float)(LN2_D * (l2s - (double)u / (double)s));
-        float g = 0.0f, kl = 0.0f;
+        float g = 0.0f, kl = 0.0f, loss = 0.0f;
         if (POLICY) {
-            const float adv = A.adv[row];
-            const float r = expf((float)(lp - (double)A.old_lp[row]));
+            const float r = expf((float)(lp - (double)old_lp));
             // min(r A, clip(r) A) is the clipped one only beyond the bound that A favours
             const bool over = adv > 0.0f && r > A.clip_hi, under = adv < 0.0f && r < A.clip_lo;
-            float loss = -adv * (over ? A.clip_hi : under ? A.clip_lo : r);
+            loss = -adv * (over ? A.clip_hi : under ? A.clip_lo : r);
             g = over || under ? 0.0f : -r * adv;
             if (A.ref_lp) {
-                const float dr = (float)((double)A.ref_lp[row] - lp);
+                const float dr = (float)((double)ref_lp - lp);
                 const float x1 = expm1f(dr);
                 kl = x1 - dr;
                 if (A.kl_coef != 0.0f) {
@@ -334,13 +492,13 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
                 }
             }
             if (OP == OP_POLICY_ENT) loss -= A.ent_coef * H;
-            if (tid == 0) A.row_loss[row] = loss;
             const float wm = w * A.sc.m;
             ct = wm * g;
             ca = wm * (OP == OP_POLICY_ENT ? A.ent_coef * H - g : -g);
             cb = OP == OP_POLICY_ENT ? wm * A.ent_coef * LN2 : 0.0f;
         }
-        if (tid == 0) {
+        if (rank == 0 && tid == 0) {
+            if (POLICY) A.row_loss[row] = loss;
             if (A.logprobs) A.logprobs[row] = (float)lp;
             if (A.entropy) A.entropy[row] = H;
             if (A.kl) A.kl[row] = kl;
@@ -369,44 +527,63 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
                 share = (float)((double)qr * (double)s / (double)rest);
             }
         }
-        if (tid == 0) A.row_loss[row] = (float)(LN2_D * loss);
+        if (rank == 0 && tid == 0) A.row_loss[row] = (float)(LN2_D * loss);
         q_all = w * A.sc.m * (float)mass;
         ca = w * A.sc.m * ((float)mass - share);
     }
     if (!gout) return;
 
     const float l2f = (float)l2s;
-    for (uint32_t c = tid; c < R.chunks; c += THREADS) {
-        float v[E];
-        R.template load<CAP>(c, A.sc, v);
-        const int64_t j0 = R.first(c);
+    auto grad_of = [&](float cv) {
+        const float lp2 = (cv - m) * k - l2f;
+        const float p = ex2(lp2);
+        return OP == OP_POLICY_ENT ? p * fmaf(cb, max_nan(lp2, D_MIN), ca) : p * ca;
+    };
+    // the token's chunk of the body (none where the token is a single element)
+    const uint32_t t_at = (uint32_t)tok - R.lead;
+    const uint32_t t_chunk = !DIST && (uint32_t)tok >= R.lead && t_at / E < R.chunks ? t_at / E : ~0u;
+    auto gradient = [&](uint32_t cu, const uint4 &q) {
+        float v[E], o[E];
+        unpack<T>(q, v);
 #pragma unroll
         for (int i = 0; i < E; i++) {
-            const float lp2 = (v[i] - m) * k - l2f;
-            const float p = ex2(lp2);
-            float g = OP == OP_POLICY_ENT ? p * fmaf(cb, max_nan(lp2, D_MIN), ca) : p * ca;
-            if (!DIST && j0 + i == (int64_t)tok) g += ct;
-            v[i] = g * slope<CAP>(v[i], A.sc);
+            v[i] = capped<CAP>(v[i], A.sc);
+            o[i] = grad_of(v[i]);
         }
-        if (R.whole(c) && (((uintptr_t)(gout + j0)) & 15u) == 0) {
-            uint4 q;
-            T *e = reinterpret_cast<T *>(&q);
-#pragma unroll
-            for (int i = 0; i < E; i++) e[i] = from_f<T>(v[i]);
-            *reinterpret_cast<uint4 *>(gout + j0) = q;
-        } else {
+        if (!DIST && cu == t_chunk) {
 #pragma unroll
             for (int i = 0; i < E; i++)
-                if (j0 + i >= 0 && j0 + i < (int64_t)V) gout[j0 + i] = from_f<T>(v[i]);
+                if (t_at % E == (uint32_t)i) o[i] += ct;
         }
+#pragma unroll
+        for (int i = 0; i < E; i++) o[i] *= slope<CAP>(v[i], A.sc);
+        store(cu, o);
+    };
+    const uint32_t k1 = min(keep_end, c1);
+    for (c = c0 + tid; c < k1; c += THREADS) gradient(c, kept[c - c0]);
+    for (; c < c1; c += BATCH * THREADS) {
+        uint4 q[BATCH];
+#pragma unroll
+        for (int u2 = 0; u2 < BATCH; u2++)
+            if (c + u2 * THREADS < c1) q[u2] = ld_stream(body + (size_t)(c + u2 * THREADS) * E);
+#pragma unroll
+        for (int u2 = 0; u2 < BATCH; u2++)
+            if (c + u2 * THREADS < c1) gradient(c + u2 * THREADS, q[u2]);
+    }
+    if (edge >= 0) {
+        float o = grad_of(c_edge);
+        if (!DIST && edge == tok) o += ct;
+        gout[edge] = from_f<T>(o * slope<CAP>(c_edge, A.sc));
     }
     if (DIST) {
-        // the teacher's ids: p Q - q, where q is the sum over the slots that
-        // hold the id (the first of them writes)
+        // the teacher's ids of this slice: p Q - q, where q is the sum over
+        // the slots that hold the id (the first of them writes)
         __syncthreads();
         for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
             const int32_t id = s_id[i];
             if (id < 0) continue;
+            const bool single = (uint32_t)id < R.lead || (uint32_t)id >= V - R.trail;
+            if (single ? rank != 0 : (uint32_t)id - e0 >= (c1 - c0) * E) continue;
             float q = 0.0f;
             bool first = true;
             for (uint32_t j = 0; j < A.n_ids; j++)
@@ -424,46 +601,86 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
 // The logits' gradient from those of log-probability and entropy, with the
 // forward pass's statistics:
 //   dv_j = m c'(v_j) [g (d_jt - p_j) - h p_j (log p_j + H)]
+// Grid: rows x slices of GRAD_SLICE chunks.
+constexpr int GRAD_BATCH = 4;
+constexpr uint32_t GRAD_SLICE = THREADS * GRAD_BATCH * 2;   // chunks of a CTA
 template <typename T, bool CAP, bool ENT>
-__global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, const float2 *stats, const float *d_lp,
-                                                          const float *d_ent, const float *entropy) {
+__global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t slices, const float2 *stats,
+                                                          const float *d_lp, const float *d_ent, const float *entropy) {
     constexpr int E = Row<T>::E;
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, V = A.vocab;
+    const uint32_t row = blockIdx.x / slices, slice = blockIdx.x % slices, tid = threadIdx.x, V = A.vocab;
     Row<T> R(A.x, A.ld, row, V);
     T *gout = (T *)A.grad + (size_t)row * A.ld_grad;
+    const bool wide = (((uintptr_t)(gout + R.lead)) & 15u) == 0;
+    const uint32_t c0 = slice * GRAD_SLICE, c1 = min(c0 + GRAD_SLICE, R.chunks);
+    const int32_t edge = slice == 0 && tid < 32 ? R.edge(tid) : -1;
     const int32_t tok = A.tokens[row];
-    if ((uint32_t)tok >= V) {
-        for (uint32_t j = tid; j < V; j += THREADS) gout[j] = from_f<T>(0.0f);
-        return;
+    const bool live = (uint32_t)tok < V;
+    float m = 0.0f, l2s = 0.0f, g = 0.0f, ca = 0.0f, cb = 0.0f;
+    const float k = A.sc.k;
+    if (live) {
+        const float2 st = stats[row];
+        m = st.x;
+        l2s = st.y * (float)(1.0 / LN2_D);
+        g = d_lp ? d_lp[row] * A.sc.m : 0.0f;
+        const float h = ENT ? d_ent[row] * A.sc.m : 0.0f;
+        ca = ENT ? -g - h * entropy[row] : -g;
+        cb = ENT ? -h * LN2 : 0.0f;
     }
-    const float2 st = stats[row];
-    const float m = st.x, k = A.sc.k, l2s = st.y * (float)(1.0 / LN2_D);
-    const float g = d_lp ? d_lp[row] * A.sc.m : 0.0f;
-    const float h = ENT ? d_ent[row] * A.sc.m : 0.0f;
-    const float ca = ENT ? -g - h * entropy[row] : -g, cb = ENT ? -h * LN2 : 0.0f;
-    for (uint32_t c = tid; c < R.chunks; c += THREADS) {
-        float v[E];
-        R.template load<CAP>(c, A.sc, v);
-        const int64_t j0 = R.first(c);
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const float lp2 = (v[i] - m) * k - l2s;
-            const float p = ex2(lp2);
-            float o = ENT ? p * fmaf(cb, max_nan(lp2, D_MIN), ca) : p * ca;
-            if (j0 + i == (int64_t)tok) o += g;
-            v[i] = o * slope<CAP>(v[i], A.sc);
-        }
-        if (R.whole(c) && (((uintptr_t)(gout + j0)) & 15u) == 0) {
-            uint4 q;
-            T *e = reinterpret_cast<T *>(&q);
-#pragma unroll
-            for (int i = 0; i < E; i++) e[i] = from_f<T>(v[i]);
-            *reinterpret_cast<uint4 *>(gout + j0) = q;
+    auto grad_of = [&](float cv) {
+        const float lp2 = (cv - m) * k - l2s;
+        const float p = ex2(lp2);
+        return ENT ? p * fmaf(cb, max_nan(lp2, D_MIN), ca) : p * ca;
+    };
+    auto store = [&](uint32_t c, const float (&v)[E]) {
+        T *o = gout + R.lead + (size_t)c * E;
+        if (wide) {
+            *reinterpret_cast<uint4 *>(o) = pack<T>(v);
         } else {
 #pragma unroll
-            for (int i = 0; i < E; i++)
-                if (j0 + i >= 0 && j0 + i < (int64_t)V) gout[j0 + i] = from_f<T>(v[i]);
+            for (int i = 0; i < E; i++) o[i] = from_f<T>(v[i]);
         }
+    };
+    if (!live) {
+        float zero[E] = {};
+        for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, zero);
+        if (edge >= 0) gout[edge] = from_f<T>(0.0f);
+        return;
+    }
+    const T *body = R.at(0);
+    const uint32_t t_at = (uint32_t)tok - R.lead;
+    const uint32_t t_chunk = (uint32_t)tok >= R.lead && t_at / E < R.chunks ? t_at / E : ~0u;
+    for (uint32_t c = c0 + tid; c < c1; c += GRAD_BATCH * THREADS) {
+        uint4 q[GRAD_BATCH];
+#pragma unroll
+        for (int u = 0; u < GRAD_BATCH; u++)
+            if (c + u * THREADS < c1) q[u] = ld_stream(body + (size_t)(c + u * THREADS) * E);
+#pragma unroll
+        for (int u = 0; u < GRAD_BATCH; u++) {
+            const uint32_t cu = c + u * THREADS;
+            if (cu >= c1) break;
+            float v[E], o[E];
+            unpack<T>(q[u], v);
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                v[i] = capped<CAP>(v[i], A.sc);
+                o[i] = grad_of(v[i]);
+            }
+            if (cu == t_chunk) {
+#pragma unroll
+                for (int i = 0; i < E; i++)
+                    if (t_at % E == (uint32_t)i) o[i] += g;
+            }
+#pragma unroll
+            for (int i = 0; i < E; i++) o[i] *= slope<CAP>(v[i], A.sc);
+            store(cu, o);
+        }
+    }
+    if (edge >= 0) {
+        const float cv = capped<CAP>(to_f(R.x[edge]), A.sc);
+        float o = grad_of(cv);
+        if (edge == tok) o += g;
+        gout[edge] = from_f<T>(o * slope<CAP>(cv, A.sc));
     }
 }
 
@@ -510,112 +727,246 @@ __device__ __forceinline__ uint32_t pick_bin(const uint32_t *hist, uint32_t &nee
     return 0u;
 }
 
-// One CTA per row: statistics, then a radix selection over the whole row
-// (four passes over the key's digits; ties are cut by the same selection over
-// the ids), then a sort of the k winners by (key, lower id).
-template <typename T, bool CAP>
-__global__ void __launch_bounds__(THREADS) k_top_row(const void *x, size_t ld, uint32_t vocab, Scale sc, float out_scale,
-                                                     uint32_t top, float *values, int32_t *ids, float *lse) {
-    constexpr int E = Row<T>::E;
-    __shared__ Stat sh_stat[WARPS];
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t sh_bin, sh_need, sh_n;
-    __shared__ unsigned long long best[MAX_K];
-    const uint32_t row = blockIdx.x, tid = threadIdx.x;
-    Row<T> R(x, ld, row, vocab);
+constexpr int TOP_CAND = 2048;       // candidates of a row
+constexpr int TOP_BINS = 2048;
+constexpr int TOP_TILE = 8;          // chunks of a tile: 128 bytes
+struct TopShared {
+    unsigned long long cand[TOP_CAND];   // key << 32 | ~id
+    uint32_t hist[TOP_BINS];
+    uint32_t tiles[TOP_CAND];
+    uint32_t warp[WARPS];
+    uint32_t bin, need, n, n_tiles;
+};
 
-    Stat a{-INFINITY, 0.0f, 0.0f};
-    for (uint32_t c = tid; c < R.chunks; c += THREADS) {
-        float v[E];
-        R.template load<CAP>(c, sc, v);
-        float m = v[0];
-#pragma unroll
-        for (int i = 1; i < E; i++) m = fmaxf(m, v[i]);
-        if (m > a.m) rebase(a, m, sc.k);
-        const float base = anchor(a.m);
-#pragma unroll
-        for (int i = 0; i < E; i++) a.s += ex2((v[i] - base) * sc.k);
-    }
-    for (int o = 16; o; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor_sync(~0u, a.m, o);
-        b.s = __shfl_xor_sync(~0u, a.s, o);
-        b.u = 0.0f;
-        a = merge(a, b, sc.k);
-    }
-    if ((tid & 31) == 0) sh_stat[tid >> 5] = a;
-    __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < WARPS; i++) a = merge(a, sh_stat[i], sc.k);
-        lse[row] = (float)((double)a.m * (double)sc.m + LN2_D * log2_d(a.s));
-        sh_n = 0;
-    }
-
-    // the k-th largest key
-    uint32_t need = top, prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (uint32_t i = tid; i < 256; i += THREADS) hist[i] = 0;
-        __syncthreads();
-        for (uint32_t j = tid; j < vocab; j += THREADS) {
-            uint32_t key = order_key(to_f(R.x[j]));
-            if ((key & mask) == prefix) atomicAdd(&hist[key >> shift & 255u], 1u);
+// Selection over the whole row by its keys' digits (four passes over the row
+// in L2; ties are cut by the same selection over the ids): for rows whose
+// candidates do not fit, as those of a few distinct values.
+template <typename T> __device__ __noinline__ void select_whole_row(const T *x, uint32_t vocab, uint32_t top, TopShared &sh) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t need = top, kth = 0, mask = 0, id_floor = 0, id_mask = 0;
+    for (int part = 0; part < 2; part++) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            for (uint32_t i = tid; i < 256; i += THREADS) sh.hist[i] = 0;
+            __syncthreads();
+            for (uint32_t j = tid; j < vocab; j += THREADS) {
+                const uint32_t key = order_key(to_f(x[j]));
+                if (part == 0 ? (key & mask) == kth : key == kth && (~j & id_mask) == id_floor)
+                    atomicAdd(&sh.hist[(part == 0 ? key : ~j) >> shift & 255u], 1u);
+            }
+            __syncthreads();
+            if (tid == 0) {
+                sh.bin = pick_bin(sh.hist, need);
+                sh.need = need;
+            }
+            __syncthreads();
+            need = sh.need;
+            (part == 0 ? kth : id_floor) |= sh.bin << shift;
+            (part == 0 ? mask : id_mask) |= 255u << shift;
         }
-        __syncthreads();
-        if (tid == 0) {
-            sh_bin = pick_bin(hist, need);
-            sh_need = need;
-        }
-        __syncthreads();
-        need = sh_need;
-        prefix |= sh_bin << shift;
-        mask |= 255u << shift;
     }
-    const uint32_t kth = prefix;
-    // of the elements that equal it, the `need` with the lowest ids: the
-    // need-th largest ~id
-    uint32_t id_floor = 0, id_mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (uint32_t i = tid; i < 256; i += THREADS) hist[i] = 0;
-        __syncthreads();
-        for (uint32_t j = tid; j < vocab; j += THREADS)
-            if (order_key(to_f(R.x[j])) == kth && (~j & id_mask) == id_floor) atomicAdd(&hist[~j >> shift & 255u], 1u);
-        __syncthreads();
-        if (tid == 0) {
-            sh_bin = pick_bin(hist, need);
-            sh_need = need;
-        }
-        __syncthreads();
-        need = sh_need;
-        id_floor |= sh_bin << shift;
-        id_mask |= 255u << shift;
-    }
-    for (uint32_t i = tid; i < MAX_K; i += THREADS) best[i] = 0ull;
+    if (tid == 0) sh.n = 0;
     __syncthreads();
     for (uint32_t j = tid; j < vocab; j += THREADS) {
-        uint32_t key = order_key(to_f(R.x[j]));
+        const uint32_t key = order_key(to_f(x[j]));
         if (key > kth || (key == kth && ~j >= id_floor)) {
-            uint32_t at = atomicAdd(&sh_n, 1u);
-            if (at < MAX_K) best[at] = (unsigned long long)key << 32 | (uint32_t)~j;
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < TOP_CAND) sh.cand[at] = (unsigned long long)key << 32 | (uint32_t)~j;
         }
     }
-    uint32_t n = 1;
-    while (n < top) n <<= 1;
-    for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t stride = size >> 1; stride; stride >>= 1) {
+    __syncthreads();
+}
+
+// One cluster of CTAs per row.  Each CTA streams its slice once: the row's
+// statistics, and the largest logit of each 128-byte tile, written into CTA
+// 0's shared memory.  CTA 0 then selects: a tile maximum that at least k tiles
+// reach is a floor that all of the k largest logits reach; the few tiles
+// above it are read again (from L2), their logits above the floor sorted.
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(THREADS) k_top(const void *x, size_t ld, uint32_t vocab, Scale sc, float out_scale,
+                                                 uint32_t top, float *values, int32_t *ids, float *lse) {
+    constexpr int E = Row<T>::E;
+    extern __shared__ float tile_max[];          // CTA 0's: the row's tiles, then the single elements as one more
+    __shared__ RowShared sh;
+    __shared__ TopShared ts;
+    const uint32_t ranks = cluster_size(), rank = cluster_rank();
+    const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31;
+    if (ranks > 1) {
+        cluster_arrive();
+        cluster_wait();                          // every CTA of the row runs: its shared memory can be written
+    }
+    Row<T> R(x, ld, row, vocab);
+    const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE;
+    const uint32_t per = (tiles + ranks - 1) / ranks * TOP_TILE;
+    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
+    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
+    const T *body = R.at(0);
+    const uint32_t dst = remote(tile_max, 0);
+    const float k = sc.k;
+    const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
+    Gather<false, false> G;
+
+    // whole batches of the CTA, so that a warp's lanes stay together
+    for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
+        uint4 q[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            const uint32_t cu = b + u * THREADS + tid;
+            if (cu < c1) q[u] = ld_stream(body + (size_t)cu * E);
+        }
+        float mx[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            mx[u] = -INFINITY;
+            if (b + u * THREADS + tid < c1) {
+                float v[E];
+                unpack<T>(q[u], v);
+                mx[u] = max_of(v);
+#pragma unroll
+                for (int i = 0; i < E; i++) v[i] = capped<CAP>(v[i], sc);
+                G.raise(CAP ? max_of(v) : mx[u], k);
+                G.chunk(v, k);
+            }
+        }
+        // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
+        // the maximum of batch step l & 7 over the group, one tile
+        static_assert(BATCH == 8 && TOP_TILE == 8, "one tile per lane and batch");
+#pragma unroll
+        for (int o = 4; o; o >>= 1) {
+#pragma unroll
+            for (int u = 0; u < o; u++) {
+                const bool up = lane & o;
+                const float keep = up ? mx[u + o] : mx[u], give = up ? mx[u] : mx[u + o];
+                mx[u] = fmaxf(keep, __shfl_xor_sync(~0u, give, o));
+            }
+        }
+        const uint32_t first = b + (lane & 7) * THREADS + (tid & ~7u);   // the tile's first chunk
+        if (first < c1) st_remote(dst + first / TOP_TILE * 4, mx[0]);
+    }
+    float e_max = v_edge;
+    if (tid < 32)
+        for (int o = 16; o; o >>= 1) e_max = fmaxf(e_max, __shfl_xor_sync(~0u, e_max, o));
+    if (rank == 0 && tid == 0) tile_max[tiles] = e_max;
+    if (edge >= 0) {
+        const float c = capped<CAP>(v_edge, sc);
+        G.raise(c, k);
+        G.add(c, anchor(G.a.m), k);
+    }
+    // (its barriers also make the tile maxima visible to CTA 0)
+    const Stat st = row_sum<false, false, true>(G, k, sh);
+    if (rank != 0) return;
+    if (tid == 0) lse[row] = (float)((double)st.m * (double)sc.m + LN2_D * log2_d(st.s));
+
+    // a floor that at least `top` tile maxima reach, by a histogram of their
+    // keys below the largest: 2^-10 of an octave a bin, coarser while the
+    // floor is not among the bins
+    const uint32_t n_max = tiles + 1;
+    uint32_t floor_key = 0;
+    if (tid == 0) ts.n = ts.n_tiles = 0;
+    float hi = -INFINITY;
+    for (uint32_t i = tid; i < n_max; i += THREADS) hi = fmaxf(hi, tile_max[i]);
+    for (int o = 16; o; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+    __syncthreads();
+    if (lane == 0) ts.warp[tid >> 5] = order_key(hi);
+    __syncthreads();
+    uint32_t hi_key = ts.warp[0];
+    for (int i = 1; i < WARPS; i++) hi_key = max(hi_key, ts.warp[i]);
+    if (n_max > top) {
+        constexpr int PER = TOP_BINS / THREADS;
+        for (int shift = 13; shift <= 21; shift += 4) {
             __syncthreads();
-            for (uint32_t i = tid; i < n / 2; i += THREADS) {
-                uint32_t lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
-                bool down = (lo & size) == 0;
-                unsigned long long p = best[lo], q = best[hi];
-                if ((p < q) == down) {
-                    best[lo] = q;
-                    best[hi] = p;
+            for (uint32_t i = tid; i < TOP_BINS; i += THREADS) ts.hist[i] = 0;
+            if (tid == 0) ts.bin = TOP_BINS - 1;
+            __syncthreads();
+            for (uint32_t i = tid; i < n_max; i += THREADS)
+                atomicAdd(&ts.hist[min((hi_key - order_key(tile_max[i])) >> shift, TOP_BINS - 1u)], 1u);
+            __syncthreads();
+            uint32_t h[PER], sum = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) sum += h[i] = ts.hist[tid * PER + i];
+            uint32_t before = sum;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t t = __shfl_up_sync(~0u, before, o);
+                if (lane >= (uint32_t)o) before += t;
+            }
+            if (lane == 31) ts.warp[tid >> 5] = before;
+            __syncthreads();
+            before -= sum;
+            for (uint32_t i = 0; i < tid >> 5; i++) before += ts.warp[i];
+            if (before < top && before + sum >= top) {
+                for (int i = 0; i < PER; i++) {
+                    before += h[i];
+                    if (before >= top) {
+                        ts.bin = tid * PER + i;
+                        break;
+                    }
                 }
             }
+            __syncthreads();
+            const uint32_t bin = ts.bin;
+            if (bin < TOP_BINS - 1) {
+                const uint32_t depth = ((bin + 1) << shift) - 1;
+                floor_key = hi_key > depth ? hi_key - depth : 0u;
+                break;
+            }
+        }
+    }
+    // the tiles that reach it, then their logits that do
+    for (uint32_t i = tid; i < n_max; i += THREADS)
+        if (order_key(tile_max[i]) >= floor_key) {
+            const uint32_t at = atomicAdd(&ts.n_tiles, 1u);
+            if (at < TOP_CAND) ts.tiles[at] = i;
+        }
+    __syncthreads();
+    const uint32_t n_tiles = ts.n_tiles;
+    if (n_tiles <= TOP_CAND) {
+        auto offer = [&](float v, uint32_t id) {
+            const uint32_t key = order_key(v);
+            if (key >= floor_key) {
+                const uint32_t at = atomicAdd(&ts.n, 1u);
+                if (at < TOP_CAND) ts.cand[at] = (unsigned long long)key << 32 | (uint32_t)~id;
+            }
+        };
+        for (uint32_t i = tid >> 3; i < n_tiles; i += THREADS / 8) {
+            const uint32_t t = ts.tiles[i], c = t * TOP_TILE + (tid & 7);
+            if (t < tiles && c < R.chunks) {
+                const uint4 q = ld_stream(body + (size_t)c * E);
+                float v[E];
+                unpack<T>(q, v);
+#pragma unroll
+                for (int j = 0; j < E; j++) offer(v[j], R.lead + c * E + j);
+            }
+        }
+        if (edge >= 0) offer(v_edge, (uint32_t)edge);
+    }
+    __syncthreads();
+    if (n_tiles > TOP_CAND || ts.n > TOP_CAND || ts.n < top) select_whole_row(R.x, vocab, top, ts);
+
+    // sort by (key, lower id): a bitonic network; strides below 64 stay
+    // within a warp's 64 elements
+    const uint32_t n = ts.n;
+    uint32_t size = 64;
+    while (size < n) size <<= 1;
+    for (uint32_t i = n + tid; i < size; i += THREADS) ts.cand[i] = 0ull;
+    __syncthreads();
+    for (uint32_t run = 2; run <= size; run <<= 1)
+        for (uint32_t stride = run >> 1; stride; stride >>= 1) {
+            for (uint32_t i = tid; i < size / 2; i += THREADS) {
+                const uint32_t lo = 2 * i - (i & (stride - 1)), up = lo + stride;
+                const unsigned long long p = ts.cand[lo], r = ts.cand[up];
+                if ((p < r) == ((lo & run) == 0)) {
+                    ts.cand[lo] = r;
+                    ts.cand[up] = p;
+                }
+            }
+            // the next stage's stride: this run's, or the next run's first
+            const uint32_t next = stride > 1 ? stride >> 1 : run;
+            if (stride > 32 || next > 32) __syncthreads();
+            else __syncwarp();
         }
     __syncthreads();
     for (uint32_t i = tid; i < top; i += THREADS) {
-        unsigned long long b = best[i];
+        const unsigned long long b = ts.cand[i];
         values[(size_t)row * top + i] = capped<CAP>(key_value((uint32_t)(b >> 32)), sc) * out_scale;
         ids[(size_t)row * top + i] = (int32_t)~(uint32_t)b;
     }
@@ -660,26 +1011,78 @@ static bs_status check_grad(const bs_logits *x, const void *grad, size_t ld_grad
     return BS_OK;
 }
 
-template <typename T, int OP>
-static bs_status launch_row(const RowArgs &A, uint32_t rows, bool cap, size_t smem, cudaStream_t st) {
-    auto kern = cap ? k_row<T, OP, true> : k_row<T, OP, false>;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) {
-            fprintf(stderr, "b200_sampler: logit_ops: shared memory of %zu bytes: %s\n", smem, cudaGetErrorString(e));
-            return BS_ECUDA;
-        }
+constexpr int MAX_DEVICES = 64;
+constexpr int SMEM_MAX = 227 * 1024;
+
+// Launches kernel K as clusters of `ranks` CTAs, one cluster per row.  The
+// first launch on a device lets the kernel use all of an SM's shared memory
+// (per device, as kernel attributes are; twice does no harm).
+template <auto K, typename... Q>
+static bs_status launch_rows(const char *what, uint32_t rows, uint32_t ranks, size_t smem, cudaStream_t st, Q... args) {
+    static std::atomic<bool> ready[MAX_DEVICES];
+    if ((uint64_t)rows * ranks > 0x7FFFFFFFull) return BS_EINVAL;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= MAX_DEVICES)) e = cudaErrorInvalidDevice;
+    if (e == cudaSuccess && !ready[dev].load(std::memory_order_acquire)) {
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, K);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - (int)fa.sharedSizeBytes);
+        if (e == cudaSuccess) ready[dev].store(true, std::memory_order_release);
     }
-    kern<<<rows, THREADS, smem, st>>>(A);
-    return launched("logit_ops");
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(rows * ranks);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, K, args...);
+    }
+    if (e == cudaSuccess) return BS_OK;
+    cudaGetLastError();
+    fprintf(stderr, "b200_sampler: %s: launch failed: %s\n", what, cudaGetErrorString(e));
+    return BS_ECUDA;
+}
+
+constexpr uint32_t KEEP_MAX = 72 * 64;     // chunks kept by a CTA: 72 KB, three CTAs to an SM
+constexpr uint32_t SLICE_MIN = 2 * THREADS;   // no CTA with less than two chunks a thread
+constexpr uint32_t GRID_FULL = 148 * 4;
+
+// CTAs per row: enough that a slice fits in shared memory (where one is kept)
+// and that few rows still fill the GPU.
+static uint32_t row_ranks(uint32_t rows, uint32_t chunks, bool keep) {
+    uint32_t r = 1;
+    while (r < MAX_CLUSTER && ((keep && (chunks + r - 1) / r > KEEP_MAX) ||
+                               ((uint64_t)rows * r < GRID_FULL && chunks / (2 * r) >= SLICE_MIN)))
+        r *= 2;
+    return r;
+}
+
+template <typename T, int OP>
+static bs_status launch_row(RowArgs A, uint32_t rows, bool cap, cudaStream_t st) {
+    constexpr uint32_t E = 16 / sizeof(T);
+    const uint32_t chunks = A.vocab / E, ranks = row_ranks(rows, chunks, A.grad != nullptr);
+    const uint32_t slice = (chunks + ranks - 1) / ranks;
+    A.keep = A.grad ? (slice < KEEP_MAX ? slice : KEEP_MAX) : 0;
+    size_t smem = (size_t)A.keep * 16 + (size_t)A.n_ids * 12;
+    if (OP == OP_DISTILL_TAIL) smem += ((size_t)slice * E + 31) / 32 * 4;
+    return cap ? launch_rows<k_row<T, OP, true>>("logit_ops", rows, ranks, smem, st, A)
+               : launch_rows<k_row<T, OP, false>>("logit_ops", rows, ranks, smem, st, A);
 }
 
 template <int OP>
-static bs_status launch_row_typed(const bs_logits *x, const RowArgs &A, bool cap, size_t smem, cudaStream_t st) {
+static bs_status launch_row_typed(const bs_logits *x, const RowArgs &A, bool cap, cudaStream_t st) {
     switch (x->dtype) {
-        case BS_F32: return launch_row<float, OP>(A, x->rows, cap, smem, st);
-        case BS_BF16: return launch_row<__nv_bfloat16, OP>(A, x->rows, cap, smem, st);
-        default: return launch_row<__half, OP>(A, x->rows, cap, smem, st);
+        case BS_F32: return launch_row<float, OP>(A, x->rows, cap, st);
+        case BS_BF16: return launch_row<__nv_bfloat16, OP>(A, x->rows, cap, st);
+        default: return launch_row<__half, OP>(A, x->rows, cap, st);
     }
 }
 
@@ -725,7 +1128,7 @@ extern "C" bs_status bs_token_logprobs(const bs_logits *x, const int32_t *d_toke
     A.logprobs = d_logprobs;
     A.entropy = d_entropy;
     A.stats = (float2 *)d_stats;
-    return launch_row_typed<OP_LOGPROB>(x, A, cap, 0, (cudaStream_t)stream);
+    return launch_row_typed<OP_LOGPROB>(x, A, cap, (cudaStream_t)stream);
 }
 
 template <typename T>
@@ -733,7 +1136,10 @@ static bs_status launch_logprob_grad(const RowArgs &A, uint32_t rows, bool cap, 
                                      const float *d_ent, const float *entropy, cudaStream_t st) {
     auto kern = cap ? (d_ent ? k_logprob_grad<T, true, true> : k_logprob_grad<T, true, false>)
                     : (d_ent ? k_logprob_grad<T, false, true> : k_logprob_grad<T, false, false>);
-    kern<<<rows, THREADS, 0, st>>>(A, stats, d_lp, d_ent, entropy);
+    const uint32_t chunks = A.vocab / (16 / sizeof(T));
+    const uint32_t slices = chunks ? (chunks + GRAD_SLICE - 1) / GRAD_SLICE : 1;
+    if ((uint64_t)rows * slices > 0x7FFFFFFFull) return BS_EINVAL;
+    kern<<<rows * slices, THREADS, 0, st>>>(A, slices, stats, d_lp, d_ent, entropy);
     return launched("bs_token_logprobs_grad");
 }
 
@@ -802,8 +1208,8 @@ extern "C" bs_status bs_policy_loss(const bs_logits *x, const int32_t *d_tokens,
     A.grad = d_grad;
     A.ld_grad = ld_grad;
     cudaStream_t s = (cudaStream_t)stream;
-    st = cfg->entropy_coef != 0.0f ? launch_row_typed<OP_POLICY_ENT>(x, A, cap, 0, s)
-                                   : launch_row_typed<OP_POLICY>(x, A, cap, 0, s);
+    st = cfg->entropy_coef != 0.0f ? launch_row_typed<OP_POLICY_ENT>(x, A, cap, s)
+                                   : launch_row_typed<OP_POLICY>(x, A, cap, s);
     return st != BS_OK ? st : total_loss(A, x->rows, d_loss, s);
 }
 
@@ -830,20 +1236,22 @@ extern "C" bs_status bs_distill_loss(const bs_logits *x, const int32_t *d_teache
     A.row_loss = d_row_loss;
     A.grad = d_grad;
     A.ld_grad = ld_grad;
-    size_t smem = (size_t)n_ids * 12;
-    if (d_teacher_lse) smem += ((size_t)x->vocab + 16 + 31) / 32 * 4 + 16;
     cudaStream_t s = (cudaStream_t)stream;
-    st = d_teacher_lse ? launch_row_typed<OP_DISTILL_TAIL>(x, A, cap, smem, s)
-                       : launch_row_typed<OP_DISTILL>(x, A, cap, smem, s);
+    st = d_teacher_lse ? launch_row_typed<OP_DISTILL_TAIL>(x, A, cap, s)
+                       : launch_row_typed<OP_DISTILL>(x, A, cap, s);
     return st != BS_OK ? st : total_loss(A, x->rows, d_loss, s);
 }
 
 template <typename T>
 static bs_status launch_top(const bs_logits *x, const Scale &sc, float os, bool cap, uint32_t k, float *values,
                             int32_t *ids, float *lse, cudaStream_t st) {
-    auto kern = cap ? k_top_row<T, true> : k_top_row<T, false>;
-    kern<<<x->rows, THREADS, 0, st>>>(x->data, x->ld, x->vocab, sc, os, k, values, ids, lse);
-    return launched("bs_top_logits");
+    const uint32_t chunks = x->vocab / (16 / sizeof(T));
+    const size_t smem = ((size_t)chunks / TOP_TILE + 2) * 4;
+    const uint32_t ranks = row_ranks(x->rows, chunks, false);
+    return cap ? launch_rows<k_top<T, true>>("bs_top_logits", x->rows, ranks, smem, st, x->data, x->ld, x->vocab, sc, os,
+                                             k, values, ids, lse)
+               : launch_rows<k_top<T, false>>("bs_top_logits", x->rows, ranks, smem, st, x->data, x->ld, x->vocab, sc,
+                                              os, k, values, ids, lse);
 }
 
 extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t *d_ids, float *d_lse,
