@@ -41,6 +41,7 @@ struct Scale {
     float m;         // 1 / (logit_scale T)
     float cap, icap; // soft-cap and its reciprocal
     double inv_t;    // 1 / T
+    double dk;       // what rounding left off k, relative
 };
 
 struct RowArgs {
@@ -84,9 +85,85 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// c(v) and its slope 1 - (c / cap)^2.
+// Two f32 in one 64-bit register: Blackwell's FMA pipe does both halves in
+// one issue slot, and issue slots are what the 16-bit types run short of.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ f2 both(float a) { return pair(a, a); }
+__device__ __forceinline__ void halves(f2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 ex2_2(f2 v) {
+    float a, b;
+    halves(v, a, b);
+    return pair(ex2(a), ex2(b));
+}
+__device__ __forceinline__ f2 floor2(f2 v) {   // at least D_MIN; a NaN stays
+    float a, b;
+    halves(v, a, b);
+    return pair(max_nan(a, D_MIN), max_nan(b, D_MIN));
+}
+
+// The soft-cap c(v) = cap tanh(v / cap).  tanh(x) is x P(x^2) / Q(x^2) for
+// |x| <= 9, where 1 - tanh is below half a step: a least-squares fit of the
+// relative error over [0, 9], reweighted towards its maximum, 2.1e-8.  All
+// coefficients are positive, so the two sums lose nothing; at most 12 half
+// steps off with the products and the approximate reciprocal.  Two FMA-pipe
+// slots a term for two logits and one reciprocal each, where the form with an
+// exponential needs two of the scarce special functions.
+__constant__ const float TANH_P[5] = {0.9999999794944238f, 0.13381039141757592f, 0.0034956033997520213f,
+                                      2.0609303648709823e-05f, 1.3354913460618338e-08f};
+__constant__ const float TANH_Q[4] = {0.46714354763692456f, 0.025877042277977037f, 0.0003285658489434587f,
+                                      7.776672917322147e-07f};
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float within(float x) {   // [-9, 9]; a NaN stays
+    float y;
+    asm("min.NaN.f32 %0, %1, 0f41100000;" : "=f"(y) : "f"(max_nan(x, -9.0f)));
+    return y;
+}
+template <bool CAP> __device__ __forceinline__ f2 capped2(f2 v, const Scale &sc) {
+    if (!CAP) return v;
+    float a, b;
+    halves(mul2(v, both(sc.icap)), a, b);
+    const f2 x = pair(within(a), within(b)), y = mul2(x, x);
+    f2 p = both(TANH_P[4]), q = both(TANH_Q[3]);
+#pragma unroll
+    for (int i = 3; i >= 0; i--) p = fma2(p, y, both(TANH_P[i]));
+#pragma unroll
+    for (int i = 2; i >= 0; i--) q = fma2(q, y, both(TANH_Q[i]));
+    halves(fma2(q, y, both(1.0f)), a, b);
+    return mul2(mul2(mul2(x, p), pair(rcp(a), rcp(b))), both(sc.cap));
+}
 template <bool CAP> __device__ __forceinline__ float capped(float v, const Scale &sc) {
-    return CAP ? sc.cap * tanhf(v * sc.icap) : v;
+    float a, b;
+    halves(capped2<CAP>(both(v), sc), a, b);
+    return a;
+}
+// The soft-cap's slope 1 - (c / cap)^2.
+template <bool CAP> __device__ __forceinline__ f2 slope2(f2 c, const Scale &sc) {
+    const f2 t = mul2(c, both(sc.icap));
+    return fma2(mul2(t, both(-1.0f)), t, both(1.0f));
 }
 template <bool CAP> __device__ __forceinline__ float slope(float c, const Scale &sc) {
     if (!CAP) return 1.0f;
@@ -101,17 +178,74 @@ __device__ __forceinline__ uint4 ld_stream(const void *p) {
                  : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p) : "memory");
     return q;
 }
-template <typename T> __device__ __forceinline__ void unpack(const uint4 &q, float (&v)[16 / sizeof(T)]) {
+__device__ __forceinline__ f2 widen(uint32_t w, __nv_bfloat16) {
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ f2 widen(uint32_t w, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return pair(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t narrow(f2 v, __nv_bfloat16) {
+    float a, b;
+    halves(v, a, b);
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t narrow(f2 v, __half) {
+    float a, b;
+    halves(v, a, b);
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b, __half) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// A 16-byte chunk of E logits as pairs, and back.
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &q, f2 (&v)[8 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 4) {
+        v[0] = pair(__uint_as_float(q.x), __uint_as_float(q.y));
+        v[1] = pair(__uint_as_float(q.z), __uint_as_float(q.w));
+    } else {
+        v[0] = widen(q.x, T());
+        v[1] = widen(q.y, T());
+        v[2] = widen(q.z, T());
+        v[3] = widen(q.w, T());
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const f2 (&v)[8 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 4) {
+        float a, b, c, d;
+        halves(v[0], a, b);
+        halves(v[1], c, d);
+        return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+    } else {
+        return make_uint4(narrow(v[0], T()), narrow(v[1], T()), narrow(v[2], T()), narrow(v[3], T()));
+    }
+}
+// The largest logit of a chunk (a NaN is passed over).
+template <typename T> __device__ __forceinline__ float max_of(const uint4 &q) {
+    if constexpr (sizeof(T) == 4) {
+        return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    } else {
+        float a, b;
+        halves(widen(max_pair(max_pair(q.x, q.y, T()), max_pair(q.z, q.w, T()), T()), T()), a, b);
+        return fmaxf(a, b);
+    }
+}
+// What a thread writes of a chunk where 16-byte stores do not fit.
+template <typename T> __device__ __forceinline__ void store_each(T *g, const uint4 &q) {
     const T *e = reinterpret_cast<const T *>(&q);
 #pragma unroll
-    for (int i = 0; i < (int)(16 / sizeof(T)); i++) v[i] = to_f(e[i]);
-}
-template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
-    uint4 q;
-    T *e = reinterpret_cast<T *>(&q);
-#pragma unroll
-    for (int i = 0; i < (int)(16 / sizeof(T)); i++) e[i] = from_f<T>(v[i]);
-    return q;
+    for (int i = 0; i < (int)(16 / sizeof(T)); i++) g[i] = e[i];
 }
 
 // A row as its body, the 16-byte aligned chunks that lie wholly inside it,
@@ -165,40 +299,65 @@ __device__ __forceinline__ Stat merge(Stat a, const Stat &b, float k) {
     return a;
 }
 
-// What a thread gathers of the logits it reads.  With TAIL, s is the sum over
-// the tokens that are not the teacher's and `top` that over those that are;
-// u is then not kept.
-template <bool ENT, bool TAIL> struct Gather {
-    Stat a{-INFINITY, 0.0f, 0.0f};
-    float top = 0.0f;
-    __device__ __forceinline__ void raise(float m, float k) {
-        if (m > a.m) {
-            if (TAIL) top *= ex2(fmaxf((a.m - m) * k, D_MIN));
-            rebase(a, m, k);
+// What a thread gathers of the logits it reads, on the scale of its running
+// maximum m: s = sum 2^d and u = sum 2^d d in pairs (even and odd logits).
+// With TAIL, s is the sum over the tokens that are not the teacher's and
+// `top` that over those that are; u is then not kept.
+template <typename T, bool CAP, bool ENT, bool TAIL> struct Gather {
+    static constexpr int E = 16 / sizeof(T);
+    float m = -INFINITY, top = 0.0f;
+    f2 s = 0, u = 0;
+    __device__ __forceinline__ void raise(float to, float k) {
+        if (to > m) {
+            const float d = fmaxf((m - to) * k, D_MIN), f = ex2(d);
+            if (TAIL) top *= f;
+            if (ENT) u = mul2(both(f), fma2(both(d), s, u));
+            s = mul2(s, both(f));
+            m = to;
         }
     }
-    __device__ __forceinline__ void add(float v, float base, float k, bool marked = false) {
-        const float d = (v - base) * k;
-        const float e = ex2(d);
+    // logits after the soft-cap, none above m (but for the soft-cap's rounding)
+    __device__ __forceinline__ void chunk(const f2 (&v)[E / 2], float k, uint32_t marks = 0) {
+        const f2 base = both(-anchor(m)), kk = both(k);
+#pragma unroll
+        for (int i = 0; i < E / 2; i++) {
+            const f2 d = mul2(add2(v[i], base), kk);
+            f2 e = ex2_2(d);
+            if (TAIL && marks) {
+                float a, b;
+                halves(e, a, b);
+                if (marks >> (2 * i) & 1u) top += a, a = 0.0f;
+                if (marks >> (2 * i) & 2u) top += b, b = 0.0f;
+                e = pair(a, b);
+            }
+            s = add2(s, e);
+            if (ENT) u = fma2(e, floor2(d), u);
+        }
+    }
+    __device__ __forceinline__ void chunk(const uint4 &q, const Scale &sc, uint32_t marks = 0) {
+        f2 v[E / 2];
+        unpack<T>(q, v);
+#pragma unroll
+        for (int i = 0; i < E / 2; i++) v[i] = capped2<CAP>(v[i], sc);
+        chunk(v, sc.k, marks);
+    }
+    __device__ __forceinline__ void one(float c, float k, bool marked) {   // a single logit
+        raise(c, k);
+        const float d = (c - anchor(m)) * k, e = ex2(d);
         if (TAIL && marked) {
             top += e;
         } else {
-            a.s += e;
-            if (ENT) a.u = fmaf(e, max_nan(d, D_MIN), a.u);
+            s = add2(s, pair(e, 0.0f));
+            if (ENT) u = fma2(pair(e, 0.0f), both(max_nan(d, D_MIN)), u);
         }
     }
-    template <int N> __device__ __forceinline__ void chunk(const float (&v)[N], float k, uint32_t marks = 0) {
-        const float base = anchor(a.m);
-#pragma unroll
-        for (int i = 0; i < N; i++) add(v[i], base, k, TAIL && (marks >> i & 1u));
+    __device__ __forceinline__ Stat stat() const {
+        float a, b, c, d;
+        halves(s, a, b);
+        halves(u, c, d);
+        return Stat{m, a + b, TAIL ? top : c + d};
     }
 };
-template <int N> __device__ __forceinline__ float max_of(const float (&v)[N]) {
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) m = fmaxf(m, v[i]);
-    return m;
-}
 
 // The CTAs of a row form a cluster.
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -248,29 +407,24 @@ struct RowShared {
     float cta[MAX_CLUSTER][4];
 };
 // RUNS: the caller has made sure that all CTAs of the row run.
-template <bool ENT, bool TAIL, bool RUNS = false>
-__device__ __forceinline__ Stat row_sum(Gather<ENT, TAIL> g, float k, RowShared &sh) {
+template <bool TAIL, bool RUNS = false>
+__device__ __forceinline__ Stat row_sum(Stat a, float k, RowShared &sh) {
     const uint32_t tid = threadIdx.x, ranks = cluster_size();
-    auto fold = [&](Stat a, float top, Stat b, float btop) {
-        // (with TAIL the second sum rides in u; its scale is the same)
-        float m = fmaxf(a.m, b.m);
-        if (TAIL) {
-            float fa = ex2(fmaxf((a.m - m) * k, D_MIN)), fb = ex2(fmaxf((b.m - m) * k, D_MIN));
-            return Stat{m, a.s * fa + b.s * fb, top * fa + btop * fb};
-        }
-        return merge(a, b, k);
+    auto fold = [&](const Stat &a, const Stat &b) {
+        if (!TAIL) return merge(a, b, k);
+        const float m = fmaxf(a.m, b.m);   // (u is another sum)
+        const float fa = ex2(fmaxf((a.m - m) * k, D_MIN)), fb = ex2(fmaxf((b.m - m) * k, D_MIN));
+        return Stat{m, a.s * fa + b.s * fb, a.u * fa + b.u * fb};
     };
-    Stat a = g.a;
-    if (TAIL) a.u = g.top;
     for (int o = 16; o; o >>= 1) {
         Stat b{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.u, o)};
         // both lanes of a pair fold in the same order: the same bits
-        a = (tid & o) ? fold(b, b.u, a, a.u) : fold(a, a.u, b, b.u);
+        a = (tid & o) ? fold(b, a) : fold(a, b);
     }
     if ((tid & 31) == 0) sh.warp[tid >> 5] = a;
     __syncthreads();
     a = sh.warp[0];
-    for (int i = 1; i < WARPS; i++) a = fold(a, a.u, sh.warp[i], sh.warp[i].u);
+    for (int i = 1; i < WARPS; i++) a = fold(a, sh.warp[i]);
     if (ranks > 1) {
         if (!RUNS) cluster_wait();   // (the arrival is at the kernel's start: every CTA of the row runs)
         const uint32_t me = cluster_rank();
@@ -283,10 +437,42 @@ __device__ __forceinline__ Stat row_sum(Gather<ENT, TAIL> g, float k, RowShared 
         cluster_arrive();
         cluster_wait();
         a = Stat{sh.cta[0][0], sh.cta[0][1], sh.cta[0][2]};
-        for (uint32_t i = 1; i < ranks; i++) a = fold(a, a.u, Stat{sh.cta[i][0], sh.cta[i][1], sh.cta[i][2]}, sh.cta[i][2]);
+        for (uint32_t i = 1; i < ranks; i++) a = fold(a, Stat{sh.cta[i][0], sh.cta[i][1], sh.cta[i][2]});
     }
     return a;
 }
+
+// The gradient of one row: c'(v_j) p_j (ca + cb log2 p_j), log2 p_j = d_j - log2 S.
+template <bool ENT> struct GradRow {
+    float m, k, l2s, ca, cb;
+    __device__ __forceinline__ float one(float c) const {
+        const float l = fmaf(c - m, k, -l2s), p = ex2(l);
+        return ENT ? p * fmaf(cb, max_nan(l, D_MIN), ca) : p * ca;
+    }
+    // a chunk of it; ct is added at element t (none: ~0u)
+    template <typename T, bool CAP>
+    __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc, uint32_t t, float ct) const {
+        constexpr int N = 8 / sizeof(T);
+        f2 v[N], o[N];
+        unpack<T>(q, v);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = capped2<CAP>(v[i], sc);
+            const f2 l = fma2(add2(v[i], both(-m)), both(k), both(-l2s));
+            o[i] = mul2(ex2_2(l), ENT ? fma2(both(cb), floor2(l), both(ca)) : both(ca));
+        }
+        if (t != ~0u) {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                o[i] = add2(o[i], pair(t == 2u * i ? ct : 0.0f, t == 2u * i + 1 ? ct : 0.0f));
+        }
+        if (CAP) {
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = mul2(o[i], slope2<CAP>(v[i], sc));
+        }
+        return pack<T>(o);
+    }
+};
 
 // Chunks of a thread in one batch: 8 16-byte loads are under way before the
 // first is used.
@@ -385,14 +571,10 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
 
     // 16-byte stores where the gradient's rows are aligned like the logits'
     const bool wide = gout && (((uintptr_t)(gout + R.lead)) & 15u) == 0;
-    auto store = [&](uint32_t c, const float (&v)[E]) {
+    auto store = [&](uint32_t c, const uint4 &q) {
         T *g = gout + R.lead + (size_t)c * E;
-        if (wide) {
-            *reinterpret_cast<uint4 *>(g) = pack<T>(v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; i++) g[i] = from_f<T>(v[i]);
-        }
+        if (wide) *reinterpret_cast<uint4 *>(g) = q;
+        else store_each<T>(g, q);
     };
 
     if (!live) {  // the row is left out: zeros, and its logits are not read
@@ -404,8 +586,7 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
             if (A.row_loss) A.row_loss[row] = 0.0f;
         }
         if (gout) {
-            float zero[E] = {};
-            for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, zero);
+            for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, make_uint4(0, 0, 0, 0));
             if (edge >= 0) gout[edge] = from_f<T>(0.0f);
         }
         if (ranks > 1) cluster_wait();
@@ -416,7 +597,7 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
     const float c_edge = edge >= 0 ? capped<CAP>(to_f(R.x[edge]), A.sc) : -INFINITY;
 
     // statistics
-    Gather<!DIST, TAIL> G;
+    Gather<T, CAP, !DIST, TAIL> G;
     const T *body = R.at(0);
     auto marks = [&](uint32_t c) -> uint32_t {
         if (!TAIL) return 0u;
@@ -424,21 +605,22 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
         return s_bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
     };
     const uint32_t keep_end = gout ? c0 + A.keep : c0;   // the first `keep` chunks stay
+    auto keep = [&](uint32_t c, const uint4 &q) {
+        if (c < keep_end) kept[c - c0] = q;
+    };
     uint32_t c = c0 + tid;
     for (; c + (BATCH - 1) * THREADS < c1; c += BATCH * THREADS) {
         uint4 q[BATCH];
 #pragma unroll
         for (int u = 0; u < BATCH; u++) q[u] = ld_stream(body + (size_t)(c + u * THREADS) * E);
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
+        for (int u = 0; u < BATCH; u += 2) {
             const uint32_t cu = c + u * THREADS;
-            if (cu < keep_end) kept[cu - c0] = q[u];
-            float v[E];
-            unpack<T>(q[u], v);
-#pragma unroll
-            for (int i = 0; i < E; i++) v[i] = capped<CAP>(v[i], A.sc);
-            G.raise(max_of(v), k);
-            G.chunk(v, k, marks(cu));
+            keep(cu, q[u]);
+            keep(cu + THREADS, q[u + 1]);
+            G.raise(capped<CAP>(fmaxf(max_of<T>(q[u]), max_of<T>(q[u + 1])), A.sc), k);
+            G.chunk(q[u], A.sc, marks(cu));
+            G.chunk(q[u + 1], A.sc, marks(cu + THREADS));
         }
     }
     if (c < c1) {   // the slice's end: fewer than BATCH chunks
@@ -450,31 +632,27 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
         for (int u = 0; u < BATCH; u++) {
             const uint32_t cu = c + u * THREADS;
             if (cu < c1) {
-                if (cu < keep_end) kept[cu - c0] = q[u];
-                float v[E];
-                unpack<T>(q[u], v);
-#pragma unroll
-                for (int i = 0; i < E; i++) v[i] = capped<CAP>(v[i], A.sc);
-                G.raise(max_of(v), k);
-                G.chunk(v, k, marks(cu));
+                keep(cu, q[u]);
+                G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
+                G.chunk(q[u], A.sc, marks(cu));
             }
         }
     }
-    if (edge >= 0) {
-        G.raise(c_edge, k);
-        G.add(c_edge, anchor(G.a.m), k, edge_marked);
-    }
-    const Stat st = row_sum(G, k, sh);
+    if (edge >= 0) G.one(c_edge, k, edge_marked);
+    const Stat st = row_sum<TAIL>(G.stat(), k, sh);
     const float m = st.m, rest = st.s, u = st.u;
     const float s = TAIL ? st.s + st.u : st.s;
-    const double l2s = log2_d(s);
+    double l2s = log2_d(s);
+    // k is m log2 e in f32: to first order, what its rounding did to the sum
+    if (!DIST) l2s += A.sc.dk * (double)u / (double)s;
+    const double k_all = (double)k * (1.0 + A.sc.dk);
 
     // the row's results and the gradient's coefficients:
     //   dv_j = c'(v_j) p_j (ca + cb log2 p_j), + c'(v_t) ct at the token
     float ca = 0.0f, cb = 0.0f, ct = 0.0f, q_all = 0.0f;
     if (!DIST) {
-        const double lp = LN2_D * (((double)c_tok - (double)m) * (double)k - l2s);
-        const float H = (float)(LN2_D * (l2s - (double)u / (double)s));
+        const double lp = LN2_D * (((double)c_tok - (double)m) * k_all - l2s);
+        const float H = (float)(LN2_D * (l2s - (1.0 + A.sc.dk) * (double)u / (double)s));
         float g = 0.0f, kl = 0.0f, loss = 0.0f;
         if (POLICY) {
             const float r = expf((float)(lp - (double)old_lp));
@@ -510,7 +688,7 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
         for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
             const float q = s_q[i];
             if (s_id[i] >= 0 && !(q <= 0.0f)) {
-                const double l2p = ((double)s_c[i] - (double)m) * (double)k - l2s;
+                const double l2p = ((double)s_c[i] - (double)m) * k_all - l2s;
                 loss += (double)q * (log2_d(q) - l2p);
                 mass += (double)q;
             }
@@ -534,30 +712,12 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
     if (!gout) return;
 
     const float l2f = (float)l2s;
-    auto grad_of = [&](float cv) {
-        const float lp2 = (cv - m) * k - l2f;
-        const float p = ex2(lp2);
-        return OP == OP_POLICY_ENT ? p * fmaf(cb, max_nan(lp2, D_MIN), ca) : p * ca;
-    };
+    const GradRow<OP == OP_POLICY_ENT> gr{m, k, l2f, ca, cb};
     // the token's chunk of the body (none where the token is a single element)
     const uint32_t t_at = (uint32_t)tok - R.lead;
     const uint32_t t_chunk = !DIST && (uint32_t)tok >= R.lead && t_at / E < R.chunks ? t_at / E : ~0u;
     auto gradient = [&](uint32_t cu, const uint4 &q) {
-        float v[E], o[E];
-        unpack<T>(q, v);
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            v[i] = capped<CAP>(v[i], A.sc);
-            o[i] = grad_of(v[i]);
-        }
-        if (!DIST && cu == t_chunk) {
-#pragma unroll
-            for (int i = 0; i < E; i++)
-                if (t_at % E == (uint32_t)i) o[i] += ct;
-        }
-#pragma unroll
-        for (int i = 0; i < E; i++) o[i] *= slope<CAP>(v[i], A.sc);
-        store(cu, o);
+        store(cu, gr.template chunk<T, CAP>(q, A.sc, cu == t_chunk ? t_at % E : ~0u, ct));
     };
     const uint32_t k1 = min(keep_end, c1);
     for (c = c0 + tid; c < k1; c += THREADS) gradient(c, kept[c - c0]);
@@ -571,8 +731,7 @@ __global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
             if (c + u2 * THREADS < c1) gradient(c + u2 * THREADS, q[u2]);
     }
     if (edge >= 0) {
-        float o = grad_of(c_edge);
-        if (!DIST && edge == tok) o += ct;
+        const float o = gr.one(c_edge) + (!DIST && edge == tok ? ct : 0.0f);
         gout[edge] = from_f<T>(o * slope<CAP>(c_edge, A.sc));
     }
     if (DIST) {
@@ -627,23 +786,14 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
         ca = ENT ? -g - h * entropy[row] : -g;
         cb = ENT ? -h * LN2 : 0.0f;
     }
-    auto grad_of = [&](float cv) {
-        const float lp2 = (cv - m) * k - l2s;
-        const float p = ex2(lp2);
-        return ENT ? p * fmaf(cb, max_nan(lp2, D_MIN), ca) : p * ca;
-    };
-    auto store = [&](uint32_t c, const float (&v)[E]) {
+    const GradRow<ENT> gr{m, k, l2s, ca, cb};
+    auto store = [&](uint32_t c, const uint4 &q) {
         T *o = gout + R.lead + (size_t)c * E;
-        if (wide) {
-            *reinterpret_cast<uint4 *>(o) = pack<T>(v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; i++) o[i] = from_f<T>(v[i]);
-        }
+        if (wide) *reinterpret_cast<uint4 *>(o) = q;
+        else store_each<T>(o, q);
     };
     if (!live) {
-        float zero[E] = {};
-        for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, zero);
+        for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, make_uint4(0, 0, 0, 0));
         if (edge >= 0) gout[edge] = from_f<T>(0.0f);
         return;
     }
@@ -658,28 +808,12 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
 #pragma unroll
         for (int u = 0; u < GRAD_BATCH; u++) {
             const uint32_t cu = c + u * THREADS;
-            if (cu >= c1) break;
-            float v[E], o[E];
-            unpack<T>(q[u], v);
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                v[i] = capped<CAP>(v[i], A.sc);
-                o[i] = grad_of(v[i]);
-            }
-            if (cu == t_chunk) {
-#pragma unroll
-                for (int i = 0; i < E; i++)
-                    if (t_at % E == (uint32_t)i) o[i] += g;
-            }
-#pragma unroll
-            for (int i = 0; i < E; i++) o[i] *= slope<CAP>(v[i], A.sc);
-            store(cu, o);
+            if (cu < c1) store(cu, gr.template chunk<T, CAP>(q[u], A.sc, cu == t_chunk ? t_at % E : ~0u, g));
         }
     }
     if (edge >= 0) {
         const float cv = capped<CAP>(to_f(R.x[edge]), A.sc);
-        float o = grad_of(cv);
-        if (edge == tok) o += g;
+        const float o = gr.one(cv) + (edge == tok ? g : 0.0f);
         gout[edge] = from_f<T>(o * slope<CAP>(cv, A.sc));
     }
 }
@@ -804,7 +938,7 @@ __global__ void __launch_bounds__(THREADS) k_top(const void *x, size_t ld, uint3
     const uint32_t dst = remote(tile_max, 0);
     const float k = sc.k;
     const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
-    Gather<false, false> G;
+    Gather<T, CAP, false, false> G;
 
     // whole batches of the CTA, so that a warp's lanes stay together
     for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
@@ -819,13 +953,9 @@ __global__ void __launch_bounds__(THREADS) k_top(const void *x, size_t ld, uint3
         for (int u = 0; u < BATCH; u++) {
             mx[u] = -INFINITY;
             if (b + u * THREADS + tid < c1) {
-                float v[E];
-                unpack<T>(q[u], v);
-                mx[u] = max_of(v);
-#pragma unroll
-                for (int i = 0; i < E; i++) v[i] = capped<CAP>(v[i], sc);
-                G.raise(CAP ? max_of(v) : mx[u], k);
-                G.chunk(v, k);
+                mx[u] = max_of<T>(q[u]);
+                G.raise(capped<CAP>(mx[u], sc), k);
+                G.chunk(q[u], sc);
             }
         }
         // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
@@ -847,13 +977,9 @@ __global__ void __launch_bounds__(THREADS) k_top(const void *x, size_t ld, uint3
     if (tid < 32)
         for (int o = 16; o; o >>= 1) e_max = fmaxf(e_max, __shfl_xor_sync(~0u, e_max, o));
     if (rank == 0 && tid == 0) tile_max[tiles] = e_max;
-    if (edge >= 0) {
-        const float c = capped<CAP>(v_edge, sc);
-        G.raise(c, k);
-        G.add(c, anchor(G.a.m), k);
-    }
+    if (edge >= 0) G.one(capped<CAP>(v_edge, sc), k, false);
     // (its barriers also make the tile maxima visible to CTA 0)
-    const Stat st = row_sum<false, false, true>(G, k, sh);
+    const Stat st = row_sum<false, true>(G.stat(), k, sh);
     if (rank != 0) return;
     if (tid == 0) lse[row] = (float)((double)st.m * (double)sc.m + LN2_D * log2_d(st.s));
 
@@ -931,10 +1057,15 @@ __global__ void __launch_bounds__(THREADS) k_top(const void *x, size_t ld, uint3
             const uint32_t t = ts.tiles[i], c = t * TOP_TILE + (tid & 7);
             if (t < tiles && c < R.chunks) {
                 const uint4 q = ld_stream(body + (size_t)c * E);
-                float v[E];
+                f2 v[E / 2];
                 unpack<T>(q, v);
 #pragma unroll
-                for (int j = 0; j < E; j++) offer(v[j], R.lead + c * E + j);
+                for (int j = 0; j < E; j += 2) {
+                    float a, b;
+                    halves(v[j / 2], a, b);
+                    offer(a, R.lead + c * E + j);
+                    offer(b, R.lead + c * E + j + 1);
+                }
             }
         }
         if (edge >= 0) offer(v_edge, (uint32_t)edge);
@@ -998,6 +1129,7 @@ static bs_status check_logits(const bs_logits *x, Scale *sc, float *out_scale, b
     if (!(k >= 1.2e-38) || !(k <= 3.0e38)) return BS_EINVAL;
     sc->m = (float)m;
     sc->k = (float)k;
+    sc->dk = k / (double)sc->k - 1.0;
     sc->inv_t = 1.0 / (double)x->temperature;
     *cap = x->final_logit_softcapping > 0.0f;
     sc->cap = *cap ? x->final_logit_softcapping : 1.0f;

@@ -133,14 +133,18 @@ class _Rows:
     def on(self):
         """Context whose value is the stream to launch on."""
         import torch
-        if self._stream is None and torch.cuda.current_device() == self.device.index:
-            return contextlib.nullcontext(torch.cuda.current_stream().cuda_stream)
+        index = self.device.index
+        if self._stream is None and torch.cuda.current_device() == index:
+            return contextlib.nullcontext(torch.cuda.current_stream(index).cuda_stream)
         return self._switched()
 
     def floats(self, t, what, shape=None):
         """A float32 input on the logits' device, packed."""
         import torch
         shape = (self.rows,) if shape is None else shape
+        if isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.device == self.device and t.shape == shape \
+                and t.is_contiguous():
+            return t
         if not isinstance(t, torch.Tensor) or t.device != self.device or not t.is_floating_point():
             raise ValueError(f"{what} must be a floating tensor on the logits' device")
         if tuple(t.shape) != shape and not (shape == (1,) and t.dim() == 0):
@@ -154,6 +158,9 @@ class _Rows:
         every vocabulary and becomes -1."""
         import torch
         shape = (self.rows,) if shape is None else shape
+        if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == self.device and t.shape == shape \
+                and t.is_contiguous():
+            return t
         if not isinstance(t, torch.Tensor) or t.device != self.device or t.is_floating_point() or t.is_complex() \
                 or t.dtype == torch.bool:
             raise ValueError(f"{what} must be an integer tensor on the logits' device")
@@ -211,8 +218,8 @@ def token_logprobs(logits, tokens, *, temperature: float = 1.0, final_logit_soft
     r = _Rows(logits, temperature, final_logit_softcapping, logit_scale, stream)
     with r.on() as st:
         t = r.ids(tokens, "tokens")
-        buf = r.empty(4, r.rows)
-        lp, ent, stats = buf[0], buf[1], buf[2:].view(r.rows, 2)
+        lp, ent = r.empty(2, r.rows).unbind()
+        stats = r.empty(r.rows, 2)
         _s._check(_s.lib().bs_token_logprobs(ctypes.byref(r.desc), t.data_ptr(), lp.data_ptr(), ent.data_ptr(),
                                              stats.data_ptr(), st), "bs_token_logprobs")
     return TokenLogprobs(lp, ent, stats)
@@ -278,8 +285,7 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
         lse = None if teacher_lse is None else r.floats(teacher_lse, "teacher_lse")
         w = None if weights is None else r.floats(weights, "weights")
         g, ld = r.grad_out(out) if grad else (None, 0)
-        buf = r.empty(r.rows + 1)
-        loss, rows = buf[r.rows], buf[:r.rows]
+        loss, rows = r.empty(), r.empty(r.rows)
         _s._check(_s.lib().bs_distill_loss(ctypes.byref(r.desc), ids.data_ptr(), tl.data_ptr(), _ptr(lse), shape[1],
                                            _ptr(w), loss.data_ptr(), rows.data_ptr(), _ptr(g), ld, st),
                   "bs_distill_loss")
@@ -311,9 +317,8 @@ def policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs=None, wei
         ref = None if ref_logprobs is None else r.floats(ref_logprobs, "ref_logprobs")
         w = None if weights is None else r.floats(weights, "weights")
         g, ld = r.grad_out(out) if grad else (None, 0)
-        buf = r.empty(4 * r.rows + 1)
-        rows, lp, ent, kl, loss = buf.split([r.rows] * 4 + [1])
-        loss = loss[0]
+        loss = r.empty()
+        rows, lp, ent, kl = r.empty(4, r.rows).unbind()
         _s._check(_s.lib().bs_policy_loss(ctypes.byref(r.desc), t.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref),
                                           _ptr(w), ctypes.byref(cfg), loss.data_ptr(), rows.data_ptr(), lp.data_ptr(),
                                           ent.data_ptr(), kl.data_ptr(), _ptr(g), ld, st), "bs_policy_loss")
