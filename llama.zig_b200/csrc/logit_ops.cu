@@ -49,6 +49,8 @@ struct RowArgs {
     size_t ld;
     uint32_t vocab;
     uint32_t keep;              // 16-byte chunks of a CTA's slice that stay in shared memory
+    uint32_t log_ranks;         // CTAs of a row
+    uint32_t bit_words;         // teacher's tail: words of one bit per element of a slice
     Scale sc;
     const int32_t *tokens;
     // outputs (null where not asked for)
@@ -87,29 +89,13 @@ template <> __device__ __forceinline__ __half from_f<__half>(float v) { return _
 
 // Two f32 in one 64-bit register: Blackwell's FMA pipe does both halves in
 // one issue slot, and issue slots are what the 16-bit types run short of.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pair(float a, float b) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ f2 both(float a) { return pair(a, a); }
-__device__ __forceinline__ void halves(f2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    f2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
+typedef float2 f2;
+__device__ __forceinline__ f2 pair(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ f2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ void halves(f2 v, float &a, float &b) { a = v.x; b = v.y; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ f2 ex2_2(f2 v) {
     float a, b;
     halves(v, a, b);
@@ -241,6 +227,24 @@ template <typename T> __device__ __forceinline__ float max_of(const uint4 &q) {
         return fmaxf(a, b);
     }
 }
+template <typename T, int N> __device__ __forceinline__ float max_of(const uint4 (&q)[N]) {
+    uint4 m = q[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) {
+        if constexpr (sizeof(T) == 4) {
+            m.x = __float_as_uint(fmaxf(__uint_as_float(m.x), __uint_as_float(q[i].x)));
+            m.y = __float_as_uint(fmaxf(__uint_as_float(m.y), __uint_as_float(q[i].y)));
+            m.z = __float_as_uint(fmaxf(__uint_as_float(m.z), __uint_as_float(q[i].z)));
+            m.w = __float_as_uint(fmaxf(__uint_as_float(m.w), __uint_as_float(q[i].w)));
+        } else {
+            m.x = max_pair(m.x, q[i].x, T());
+            m.y = max_pair(m.y, q[i].y, T());
+            m.z = max_pair(m.z, q[i].z, T());
+            m.w = max_pair(m.w, q[i].w, T());
+        }
+    }
+    return max_of<T>(m);
+}
 // What a thread writes of a chunk where 16-byte stores do not fit.
 template <typename T> __device__ __forceinline__ void store_each(T *g, const uint4 &q) {
     const T *e = reinterpret_cast<const T *>(&q);
@@ -306,7 +310,7 @@ __device__ __forceinline__ Stat merge(Stat a, const Stat &b, float k) {
 template <typename T, bool CAP, bool ENT, bool TAIL> struct Gather {
     static constexpr int E = 16 / sizeof(T);
     float m = -INFINITY, top = 0.0f;
-    f2 s = 0, u = 0;
+    f2 s = {0.0f, 0.0f}, u = {0.0f, 0.0f};
     __device__ __forceinline__ void raise(float to, float k) {
         if (to > m) {
             const float d = fmaxf((m - to) * k, D_MIN), f = ex2(d);
@@ -390,16 +394,6 @@ __device__ __forceinline__ double log2_d(float s) {
     return (double)e + (double)log2f(f);
 }
 
-template <typename V> __device__ __forceinline__ V block_sum(V v, V *scratch) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    V r = 0;
-    for (int w = 0; w < WARPS; w++) r += scratch[w];
-    return r;
-}
-
 // The sums of all threads of the row's CTAs, in a fixed order, on one scale
 // (with TAIL: s over the rest, u over the teacher's tokens).
 struct RowShared {
@@ -449,9 +443,8 @@ template <bool ENT> struct GradRow {
         const float l = fmaf(c - m, k, -l2s), p = ex2(l);
         return ENT ? p * fmaf(cb, max_nan(l, D_MIN), ca) : p * ca;
     }
-    // a chunk of it; ct is added at element t (none: ~0u)
-    template <typename T, bool CAP>
-    __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc, uint32_t t, float ct) const {
+    // a chunk of it
+    template <typename T, bool CAP> __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
         constexpr int N = 8 / sizeof(T);
         f2 v[N], o[N];
         unpack<T>(q, v);
@@ -461,11 +454,6 @@ template <bool ENT> struct GradRow {
             const f2 l = fma2(add2(v[i], both(-m)), both(k), both(-l2s));
             o[i] = mul2(ex2_2(l), ENT ? fma2(both(cb), floor2(l), both(ca)) : both(ca));
         }
-        if (t != ~0u) {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                o[i] = add2(o[i], pair(t == 2u * i ? ct : 0.0f, t == 2u * i + 1 ? ct : 0.0f));
-        }
         if (CAP) {
 #pragma unroll
             for (int i = 0; i < N; i++) o[i] = mul2(o[i], slope2<CAP>(v[i], sc));
@@ -474,285 +462,640 @@ template <bool ENT> struct GradRow {
     }
 };
 
-// Chunks of a thread in one batch: 8 16-byte loads are under way before the
-// first is used.
-constexpr int BATCH = 8;
+// ---------------------------------------------------------------------------
+// The row kernel: statistics, results and (for the losses) the gradient of
+// whole rows, each logit read from memory once.
+//
+// What bounds it is HBM: V s bytes read and V s written a row, against some
+// ten issue slots and two ex2 a logit.  A row must be known whole before its
+// gradient starts, so it is kept on chip: a cluster of CTAs (one per SM) takes
+// a row, each CTA a slice of up to 1/3 of its shared memory, and the three
+// buffers hold the row whose gradient is being written, the row being summed
+// and the row being loaded.  So that no SM waits while a row's sums travel
+// between its CTAs, the sums of row i travel while the gradient of row i - 1
+// is written and row i + 1 is loaded:
+//
+//   compute warps       iteration i: wait for row i; sum it; write row i - 1's
+//                       gradient.
+//   warp A              adds up the CTA's sums and exchanges them with the
+//                       other CTAs of the row; the row's results and its
+//                       gradient's coefficients; the single elements before
+//                       and behind the 16-byte chunks.
+//   warp C              bulk copies of the rows to come.
+//   warps B (4)         losses with a teacher: the slots of row i + 2 (shares
+//                       q, the student's logits there), and after the gradient
+//                       of row i - 1 the tokens that the teacher names.
+//
+// The barriers, each in two copies (Z: four) that take turns: X (compute -> A: the sums
+// of row i), Y (A -> compute: row i's coefficients), P (B -> compute: slots of
+// row i), Z (compute -> B, C: row i done with).
+constexpr int COMPUTE = 384;
+constexpr uint32_t COPY = 512;       // chunks of one copy
+constexpr int STEP = 4;              // chunks of a thread summed at a time
+constexpr int CWARPS = COMPUTE / 32;
+constexpr int BTHREADS = 128;
+enum Bar { BAR_X = 1, BAR_Y = 3, BAR_P = 5, BAR_Z = 7, BAR_B = 11 };
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void copy_bulk(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(dst)),
+                 "l"(src), "r"(bytes), "r"((uint32_t)__cvta_generic_to_shared(bar))
+                 : "memory");
+}
 
-// One cluster of CTAs per row, each with a slice of the row's chunks.  First
-// pass: the slice is read once from memory for the row's statistics, and as
-// much of it as fits stays in shared memory (each thread keeps the chunks it
-// read itself, so nothing waits for other threads).  The CTAs exchange their
-// sums through the cluster's shared memory.  Second pass: the gradient, from
-// the kept chunks (what did not fit is read again, mostly from L2).
-template <typename T, int OP, bool CAP>
-__global__ void __launch_bounds__(THREADS) k_row(RowArgs A) {
-    constexpr bool DIST = OP == OP_DISTILL || OP == OP_DISTILL_TAIL;
-    constexpr bool TAIL = OP == OP_DISTILL_TAIL;
-    constexpr bool POLICY = OP == OP_POLICY || OP == OP_POLICY_ENT;
-    constexpr int E = Row<T>::E;
-    extern __shared__ uint4 dyn[];
-    __shared__ RowShared sh;
-    __shared__ float sh_f[WARPS];
-    __shared__ double sh_d[WARPS];
-    const uint32_t ranks = cluster_size(), rank = cluster_rank();
-    const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, V = A.vocab;
-    if (ranks > 1) cluster_arrive();
-    const float k = A.sc.k;
-    Row<T> R(A.x, A.ld, row, V);
-    T *gout = A.grad ? (T *)A.grad + (size_t)row * A.ld_grad : nullptr;
-    // this CTA's chunks of the body; rank 0 also has the single elements
-    const uint32_t per = (R.chunks + ranks - 1) / ranks;
-    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
-    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
+__host__ __device__ constexpr bool is_distill(int op) { return op == OP_DISTILL || op == OP_DISTILL_TAIL; }
+__host__ __device__ constexpr bool is_policy(int op) { return op == OP_POLICY || op == OP_POLICY_ENT; }
+__host__ __device__ constexpr int row_threads(int op) { return COMPUTE + 64 + (is_distill(op) ? BTHREADS : 0); }
 
-    const float w = DIST || POLICY ? (A.weights ? A.weights[row] : A.w_all) : 1.0f;
-    bool live = w != 0.0f;
-    const int32_t tok = DIST ? -1 : A.tokens[row];
-    if (!DIST) live = live && (uint32_t)tok < V;
-    const float adv = POLICY ? A.adv[row] : 0.0f, old_lp = POLICY ? A.old_lp[row] : 0.0f;
-    const float ref_lp = POLICY && A.ref_lp ? A.ref_lp[row] : 0.0f;
+// Row i's results as the gradient needs them.
+struct Coef {
+    float m, l2s;        // maximum, log2 S
+    float ca, cb, ct;    // dv_j = c'(v_j) p_j (ca + cb log2 p_j), + c'(v_t) ct at the token
+    float q_all, wm;     // teacher's ids: c'(v_j) (p_j q_all - wm q_j)
+    float c_tok;         // the token's c(v)
+    uint32_t live;       // 0: the row is left out
+};
+struct RowsShared {
+    float4 part[2][CWARPS];          // (m, s, u) of the compute warps
+    float4 mail[2][MAX_CLUSTER];     // and of the row's CTAs
+    Coef coef[4];
+    int32_t code[8];                 // the row's token (0 for a teacher's row); -1: left out
+    // B's
+    double scratch_d[BTHREADS / 32];
+    float scratch_f[BTHREADS / 32];
+    uint32_t slots_live[4], edge_marks[4];
+    uint64_t mail_bar[2], full_bar[3];
+};
 
-    // the teacher's slots; every CTA of the row has them
-    uint4 *kept = dyn;                           // [keep]
-    int32_t *s_id = (int32_t *)(dyn + A.keep);   // n_ids; -1: empty
-    float *s_q = (float *)(s_id + A.n_ids);      // share q of the slot
-    float *s_c = s_q + A.n_ids;                  // the student's c(v) there
-    uint32_t *s_bits = (uint32_t *)(s_c + A.n_ids);  // tail: one bit per element of the slice
-    const uint32_t e0 = R.lead + c0 * E;         // first element of the slice
-    bool edge_marked = false;
-    if (DIST && live) {
-        const size_t at = (size_t)row * A.n_ids;
-        float umax = -INFINITY;
-        bool any = false;
-        if (TAIL)
-            for (uint32_t i = tid; i < ((c1 - c0) * E + 31) / 32; i += THREADS) s_bits[i] = 0;
-        for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
-            int32_t id = A.t_ids[at + i];
-            if ((uint32_t)id >= V) id = -1;
-            s_id[i] = id;
-            if (id >= 0) {
-                any = true;
-                umax = max_nan(umax, A.t_logits[at + i]);
-                s_c[i] = capped<CAP>(to_f(R.x[id]), A.sc);
-            }
-        }
-        live = __syncthreads_or(any);
-        if (live) {
-            if (!TAIL) {
-                for (int o = 16; o; o >>= 1) umax = max_nan(umax, __shfl_xor_sync(~0u, umax, o));
-                if ((tid & 31) == 0) sh_f[tid >> 5] = umax;
-                __syncthreads();
-                for (int i = 0; i < WARPS; i++) umax = max_nan(umax, sh_f[i]);
-                live = umax != -INFINITY;   // no share to give: as without ids
-            }
-        }
-        if (live) {
-            const double ref = TAIL ? (double)A.t_lse[row] : (double)umax * A.sc.inv_t;
-            float q_sum = 0.0f;
-            for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
-                float q = 0.0f;
-                if (s_id[i] >= 0) {
-                    q = expf((float)((double)A.t_logits[at + i] * A.sc.inv_t - ref));
-                    const uint32_t j = (uint32_t)s_id[i] - e0;
-                    if (TAIL && j < (c1 - c0) * E) atomicOr(&s_bits[j >> 5], 1u << (j & 31));
-                }
-                s_q[i] = q;
-                q_sum += q;
-            }
-            if (!TAIL) {
-                const float total = (float)block_sum((double)q_sum, sh_d);
-                for (uint32_t i = tid; i < A.n_ids; i += THREADS) s_q[i] /= total;
-            }
-            __syncthreads();
-            if (TAIL && edge >= 0)
-                for (uint32_t i = 0; i < A.n_ids; i++) edge_marked |= s_id[i] == edge;
-        }
-    }
-
-    // 16-byte stores where the gradient's rows are aligned like the logits'
-    const bool wide = gout && (((uintptr_t)(gout + R.lead)) & 15u) == 0;
-    auto store = [&](uint32_t c, const uint4 &q) {
-        T *g = gout + R.lead + (size_t)c * E;
-        if (wide) *reinterpret_cast<uint4 *>(g) = q;
-        else store_each<T>(g, q);
-    };
-
-    if (!live) {  // the row is left out: zeros, and its logits are not read
-        if (rank == 0 && tid == 0) {
-            if (A.logprobs) A.logprobs[row] = 0.0f;
-            if (A.entropy) A.entropy[row] = 0.0f;
-            if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
-            if (A.kl) A.kl[row] = 0.0f;
-            if (A.row_loss) A.row_loss[row] = 0.0f;
-        }
-        if (gout) {
-            for (uint32_t c = c0 + tid; c < c1; c += THREADS) store(c, make_uint4(0, 0, 0, 0));
-            if (edge >= 0) gout[edge] = from_f<T>(0.0f);
-        }
-        if (ranks > 1) cluster_wait();
-        return;
-    }
-
-    const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(R.x[tok]), A.sc);
-    const float c_edge = edge >= 0 ? capped<CAP>(to_f(R.x[edge]), A.sc) : -INFINITY;
-
-    // statistics
-    Gather<T, CAP, !DIST, TAIL> G;
-    const T *body = R.at(0);
-    auto marks = [&](uint32_t c) -> uint32_t {
-        if (!TAIL) return 0u;
-        const uint32_t b = (c - c0) * E;
-        return s_bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
-    };
-    const uint32_t keep_end = gout ? c0 + A.keep : c0;   // the first `keep` chunks stay
-    auto keep = [&](uint32_t c, const uint4 &q) {
-        if (c < keep_end) kept[c - c0] = q;
-    };
-    uint32_t c = c0 + tid;
-    for (; c + (BATCH - 1) * THREADS < c1; c += BATCH * THREADS) {
-        uint4 q[BATCH];
+// The sum of a warp's (or of each group of W lanes') Stats, the same in all its
+// lanes: the largest maximum first, then every lane's sums on that scale.
+template <bool TAIL, int W> __device__ __forceinline__ Stat fold_lanes(Stat a, float k) {
+    float m = a.m;
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) q[u] = ld_stream(body + (size_t)(c + u * THREADS) * E);
+    for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float d = fmaxf((a.m - m) * k, D_MIN), f = ex2(d);
+    a.u = f * (TAIL ? a.u : fmaf(d, a.s, a.u));   // (with TAIL, u is another sum, not one of 2^d d)
+    a.s *= f;
 #pragma unroll
-        for (int u = 0; u < BATCH; u += 2) {
-            const uint32_t cu = c + u * THREADS;
-            keep(cu, q[u]);
-            keep(cu + THREADS, q[u + 1]);
-            G.raise(capped<CAP>(fmaxf(max_of<T>(q[u]), max_of<T>(q[u + 1])), A.sc), k);
-            G.chunk(q[u], A.sc, marks(cu));
-            G.chunk(q[u + 1], A.sc, marks(cu + THREADS));
-        }
+    for (int o = W / 2; o; o >>= 1) {
+        a.s += __shfl_xor_sync(~0u, a.s, o);
+        a.u += __shfl_xor_sync(~0u, a.u, o);
     }
-    if (c < c1) {   // the slice's end: fewer than BATCH chunks
-        uint4 q[BATCH];
-#pragma unroll
-        for (int u = 0; u < BATCH; u++)
-            if (c + u * THREADS < c1) q[u] = ld_stream(body + (size_t)(c + u * THREADS) * E);
-#pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const uint32_t cu = c + u * THREADS;
-            if (cu < c1) {
-                keep(cu, q[u]);
-                G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
-                G.chunk(q[u], A.sc, marks(cu));
-            }
-        }
+    a.m = m;
+    return a;
+}
+
+// The exchange between a row's CTAs: 16 bytes into every CTA's mail, which
+// count on its mbarrier.
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t *bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mail_send(const float4 *slot, const uint64_t *bar, uint32_t rank, const Stat &a, float w) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %5}, [%4];" ::"r"(
+                     remote(slot, rank)),
+                 "r"(__float_as_uint(a.m)), "r"(__float_as_uint(a.s)), "r"(__float_as_uint(a.u)), "r"(remote(bar, rank)), "r"(__float_as_uint(w))
+                 : "memory");
+}
+// Waits for all bytes of a phase; false if it gave up (a second at the least).
+__device__ __forceinline__ bool bar_wait(const uint64_t *bar, uint32_t parity) {
+    for (uint32_t tries = 0; tries < (1u << 24); tries++) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+        if (done) return true;
     }
-    if (edge >= 0) G.one(c_edge, k, edge_marked);
-    const Stat st = row_sum<TAIL>(G.stat(), k, sh);
-    const float m = st.m, rest = st.s, u = st.u;
-    const float s = TAIL ? st.s + st.u : st.s;
-    double l2s = log2_d(s);
+    return false;
+}
+
+// Results and coefficients of a row with a token.
+struct TokenIn {
+    float w, adv, old_lp, ref_lp, c_tok;
+};
+template <int OP>
+__device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const Stat &st, const TokenIn &in, bool write) {
+    const double m = st.m, ratio = (double)(st.u / st.s);
     // k is m log2 e in f32: to first order, what its rounding did to the sum
-    if (!DIST) l2s += A.sc.dk * (double)u / (double)s;
-    const double k_all = (double)k * (1.0 + A.sc.dk);
-
-    // the row's results and the gradient's coefficients:
-    //   dv_j = c'(v_j) p_j (ca + cb log2 p_j), + c'(v_t) ct at the token
-    float ca = 0.0f, cb = 0.0f, ct = 0.0f, q_all = 0.0f;
-    if (!DIST) {
-        const double lp = LN2_D * (((double)c_tok - (double)m) * k_all - l2s);
-        const float H = (float)(LN2_D * (l2s - (1.0 + A.sc.dk) * (double)u / (double)s));
-        float g = 0.0f, kl = 0.0f, loss = 0.0f;
-        if (POLICY) {
-            const float r = expf((float)(lp - (double)old_lp));
-            // min(r A, clip(r) A) is the clipped one only beyond the bound that A favours
-            const bool over = adv > 0.0f && r > A.clip_hi, under = adv < 0.0f && r < A.clip_lo;
-            loss = -adv * (over ? A.clip_hi : under ? A.clip_lo : r);
-            g = over || under ? 0.0f : -r * adv;
-            if (A.ref_lp) {
-                const float dr = (float)((double)ref_lp - lp);
-                const float x1 = expm1f(dr);
-                kl = x1 - dr;
-                if (A.kl_coef != 0.0f) {
-                    loss += A.kl_coef * kl;
-                    g -= A.kl_coef * x1;
-                }
-            }
-            if (OP == OP_POLICY_ENT) loss -= A.ent_coef * H;
-            const float wm = w * A.sc.m;
-            ct = wm * g;
-            ca = wm * (OP == OP_POLICY_ENT ? A.ent_coef * H - g : -g);
-            cb = OP == OP_POLICY_ENT ? wm * A.ent_coef * LN2 : 0.0f;
-        }
-        if (rank == 0 && tid == 0) {
-            if (POLICY) A.row_loss[row] = loss;
-            if (A.logprobs) A.logprobs[row] = (float)lp;
-            if (A.entropy) A.entropy[row] = H;
-            if (A.kl) A.kl[row] = kl;
-            if (A.stats) A.stats[row] = make_float2(m, (float)(LN2_D * l2s));
-        }
-    } else {
-        // sum q (log q - log p) over the slots, and the rest as one outcome
-        double loss = 0.0, mass = 0.0;
-        for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
-            const float q = s_q[i];
-            if (s_id[i] >= 0 && !(q <= 0.0f)) {
-                const double l2p = ((double)s_c[i] - (double)m) * k_all - l2s;
-                loss += (double)q * (log2_d(q) - l2p);
-                mass += (double)q;
+    const double l2s = log2_d(st.s) + A.sc.dk * ratio;
+    const double lp = LN2_D * (((double)in.c_tok - m) * ((double)A.sc.k * (1.0 + A.sc.dk)) - l2s);
+    const float H = (float)(LN2_D * (l2s - (1.0 + A.sc.dk) * ratio));
+    Coef c{st.m, (float)l2s, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, in.c_tok, 1u};
+    float kl = 0.0f, loss = 0.0f;
+    if (is_policy(OP)) {
+        const float r = expf((float)(lp - (double)in.old_lp));
+        // min(r A, clip(r) A) is the clipped one only beyond the bound that A favours
+        const bool over = in.adv > 0.0f && r > A.clip_hi, under = in.adv < 0.0f && r < A.clip_lo;
+        loss = -in.adv * (over ? A.clip_hi : under ? A.clip_lo : r);
+        float g = over || under ? 0.0f : -r * in.adv;
+        if (A.ref_lp) {
+            const float dr = (float)((double)in.ref_lp - lp);
+            const float x1 = expm1f(dr);
+            kl = x1 - dr;
+            if (A.kl_coef != 0.0f) {
+                loss += A.kl_coef * kl;
+                g -= A.kl_coef * x1;
             }
         }
-        loss = block_sum(loss, sh_d);
-        mass = block_sum(mass, sh_d);
-        float share = 0.0f;
-        if (TAIL) {
-            const float qr = mass >= 1.0 ? 0.0f : (float)(1.0 - mass);
-            if (!(qr <= 0.0f) && !(rest == 0.0f)) {
-                const double l2r = log2_d(rest) - l2s;
-                loss += (double)qr * (log2_d(qr) - l2r);
-                mass += (double)qr;
-                share = (float)((double)qr * (double)s / (double)rest);
-            }
-        }
-        if (rank == 0 && tid == 0) A.row_loss[row] = (float)(LN2_D * loss);
-        q_all = w * A.sc.m * (float)mass;
-        ca = w * A.sc.m * ((float)mass - share);
+        if (OP == OP_POLICY_ENT) loss -= A.ent_coef * H;
+        const float wm = in.w * A.sc.m;
+        c.ct = wm * g;
+        c.ca = wm * (OP == OP_POLICY_ENT ? A.ent_coef * H - g : -g);
+        c.cb = OP == OP_POLICY_ENT ? wm * A.ent_coef * LN2 : 0.0f;
     }
-    if (!gout) return;
+    if (write) {
+        if (is_policy(OP)) A.row_loss[row] = loss;
+        if (A.logprobs) A.logprobs[row] = (float)lp;
+        if (A.entropy) A.entropy[row] = H;
+        if (A.kl) A.kl[row] = kl;
+        if (A.stats) A.stats[row] = make_float2(st.m, (float)(LN2_D * l2s));
+    }
+    return c;
+}
 
-    const float l2f = (float)l2s;
-    const GradRow<OP == OP_POLICY_ENT> gr{m, k, l2f, ca, cb};
-    // the token's chunk of the body (none where the token is a single element)
-    const uint32_t t_at = (uint32_t)tok - R.lead;
-    const uint32_t t_chunk = !DIST && (uint32_t)tok >= R.lead && t_at / E < R.chunks ? t_at / E : ~0u;
-    auto gradient = [&](uint32_t cu, const uint4 &q) {
-        store(cu, gr.template chunk<T, CAP>(q, A.sc, cu == t_chunk ? t_at % E : ~0u, ct));
+// The teacher's slots of a row, in one of four sets.
+struct Slots {
+    int32_t *id;      // -1: empty; padded to a multiple of 4 with empty ones
+    float *q;         // the slot's share
+    float *c;         // the student's c(v) there
+    uint32_t *bits;   // tail: one bit per element of the CTA's slice
+};
+__host__ __device__ __forceinline__ uint32_t slots_padded(uint32_t n_ids) { return (n_ids + 3u) & ~3u; }
+
+// Results and coefficients of a row with a teacher; one warp.
+template <bool TAIL>
+__device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, const Slots &sl, float w, bool write) {
+    const float s = TAIL ? st.s + st.u : st.s;
+    const double l2s = log2_d(s), k_all = (double)A.sc.k * (1.0 + A.sc.dk);
+    // sum q (log q - log p) over the slots, and the rest as one outcome
+    double loss = 0.0, mass = 0.0;
+    for (uint32_t i = threadIdx.x & 31; i < A.n_ids; i += 32) {
+        const float q = sl.q[i];
+        if (sl.id[i] >= 0 && !(q <= 0.0f)) {
+            const double l2p = ((double)sl.c[i] - (double)st.m) * k_all - l2s;
+            loss += (double)q * (log2_d(q) - l2p);
+            mass += (double)q;
+        }
+    }
+    for (int o = 16; o; o >>= 1) {
+        loss += __shfl_xor_sync(~0u, loss, o);
+        mass += __shfl_xor_sync(~0u, mass, o);
+    }
+    float share = 0.0f;
+    if (TAIL) {
+        const float qr = mass >= 1.0 ? 0.0f : (float)(1.0 - mass);
+        if (!(qr <= 0.0f) && !(st.s == 0.0f)) {
+            const double l2r = log2_d(st.s) - l2s;
+            loss += (double)qr * (log2_d(qr) - l2r);
+            mass += (double)qr;
+            share = (float)((double)qr * (double)s / (double)st.s);
+        }
+    }
+    if (write) A.row_loss[row] = (float)(LN2_D * loss);
+    const float wm = w * A.sc.m;
+    return Coef{st.m, (float)l2s, wm * ((float)mass - share), 0.0f, 0.0f, wm * (float)mass, wm, 0.0f, 1u};
+}
+
+template <typename T, int OP, bool CAP>
+__global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t rows, uint32_t clusters) {
+    constexpr bool DIST = is_distill(OP), TAIL = OP == OP_DISTILL_TAIL;
+    constexpr int E = Row<T>::E;
+    constexpr int ZTHREADS = COMPUTE + 32 + (DIST ? BTHREADS : 0);
+    extern __shared__ uint4 dyn[];
+    __shared__ __align__(16) RowsShared sh;
+    const uint32_t ranks = 1u << A.log_ranks, rank = cluster_rank();
+    const uint32_t cluster = blockIdx.x >> A.log_ranks, tid = threadIdx.x, lane = tid & 31, V = A.vocab;
+    const uint32_t n = (rows - cluster + clusters - 1) / clusters;   // rows of this cluster
+    const float k = A.sc.k;
+    const bool grad = A.grad != nullptr;
+    auto row_of = [&](uint32_t i) { return cluster + i * clusters; };
+    auto weight = [&](uint32_t row) {
+        return OP == OP_LOGPROB ? 1.0f : A.weights ? A.weights[row] : A.w_all;
     };
-    const uint32_t k1 = min(keep_end, c1);
-    for (c = c0 + tid; c < k1; c += THREADS) gradient(c, kept[c - c0]);
-    for (; c < c1; c += BATCH * THREADS) {
-        uint4 q[BATCH];
-#pragma unroll
-        for (int u2 = 0; u2 < BATCH; u2++)
-            if (c + u2 * THREADS < c1) q[u2] = ld_stream(body + (size_t)(c + u2 * THREADS) * E);
-#pragma unroll
-        for (int u2 = 0; u2 < BATCH; u2++)
-            if (c + u2 * THREADS < c1) gradient(c + u2 * THREADS, q[u2]);
+    // the slice [c0, c1) of a row's chunks
+    struct Slice {
+        uint32_t c0, c1;
+    };
+    auto slice_of = [&](const Row<T> &R) {
+        const uint32_t per = (R.chunks + ranks - 1) >> A.log_ranks, c0 = min(rank * per, R.chunks);
+        return Slice{c0, min(c0 + per, R.chunks)};
+    };
+    const uint32_t pad = DIST ? slots_padded(A.n_ids) : 0u;
+    auto slots = [&](uint32_t i) {
+        const uint32_t set = i & 3;
+        char *base = (char *)(dyn + 3 * (size_t)A.keep);
+        Slots s;
+        s.id = (int32_t *)base + set * pad;
+        s.q = (float *)base + (4 + set) * pad;
+        s.c = (float *)base + (8 + set) * pad;
+        s.bits = (uint32_t *)base + 12 * pad + set * A.bit_words;
+        return s;
+    };
+
+    // rows' codes, four ahead
+    if (tid >= COMPUTE && tid < COMPUTE + 32) {
+        if (lane < 4 && lane < n) {
+            const uint32_t row = row_of(lane);
+            const int32_t tok = DIST ? 0 : A.tokens[row];
+            sh.code[lane] = weight(row) != 0.0f && (uint32_t)tok < V ? tok : -1;
+        }
+    } else if (TAIL && tid >= COMPUTE) {
+        for (uint32_t i = tid - COMPUTE - 32; i < 4 * A.bit_words; i += BTHREADS + 32) slots(0).bits[i] = 0;
     }
-    if (edge >= 0) {
-        const float o = gr.one(c_edge) + (!DIST && edge == tok ? ct : 0.0f);
-        gout[edge] = from_f<T>(o * slope<CAP>(c_edge, A.sc));
+    if (tid == 0) {
+        bar_init(&sh.mail_bar[0]);
+        bar_init(&sh.mail_bar[1]);
+        for (int i = 0; i < 3; i++) bar_init(&sh.full_bar[i]);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (DIST) {
-        // the teacher's ids of this slice: p Q - q, where q is the sum over
-        // the slots that hold the id (the first of them writes)
-        __syncthreads();
-        for (uint32_t i = tid; i < A.n_ids; i += THREADS) {
-            const int32_t id = s_id[i];
-            if (id < 0) continue;
-            const bool single = (uint32_t)id < R.lead || (uint32_t)id >= V - R.trail;
-            if (single ? rank != 0 : (uint32_t)id - e0 >= (c1 - c0) * E) continue;
-            float q = 0.0f;
-            bool first = true;
-            for (uint32_t j = 0; j < A.n_ids; j++)
-                if (s_id[j] == id) {
-                    if (j < i) first = false;
-                    q += s_q[j];
+    __syncthreads();
+    if (ranks > 1) {   // every CTA of the row runs, its mail barriers ready
+        cluster_arrive();
+        cluster_wait();
+    }
+
+    if (tid < COMPUTE) {
+        // ---- compute warps; thread tid has the chunks tid, tid + COMPUTE, ... of the slice
+        struct Part {                // a row's slice: its chunks, and how many of them are copied
+            const T *x;
+            uint32_t n, copied;
+            const uint4 *buf;
+        };
+        Part prev{}, cur{};
+        uint32_t at = 0, phase = 0;   // the buffers take turns
+        bool there = true;
+        for (uint32_t i = 0; i <= n; i++) {
+            if (i < n) {
+                const Row<T> R(A.x, A.ld, row_of(i), V);
+                const Slice sl = slice_of(R);
+                cur = Part{R.at(sl.c0), sl.c1 - sl.c0, min(sl.c1 - sl.c0, A.keep), dyn + at * A.keep + tid};
+                there = bar_wait(&sh.full_bar[at], phase) && there;
+                if (++at == 3) at = 0, phase ^= 1;
+                if (DIST) bar_sync(BAR_P + (i & 1), COMPUTE + BTHREADS);
+                Gather<T, CAP, !DIST, TAIL> G;
+                if (sh.code[i & 7] >= 0) {
+                    const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
+                    auto marks = [&](uint32_t c) -> uint32_t {
+                        if (!TAIL) return 0u;
+                        const uint32_t b = c * E;
+                        return bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
+                    };
+                    // several chunks at a time, for one comparison with the running maximum
+                    const uint4 *buf = cur.buf;
+                    uint32_t c = tid;
+                    for (; c + (STEP - 1) * COMPUTE < cur.copied; c += STEP * COMPUTE, buf += STEP * COMPUTE) {
+                        uint4 q[STEP];
+#pragma unroll
+                        for (int u = 0; u < STEP; u++) q[u] = buf[u * COMPUTE];
+                        G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+#pragma unroll
+                        for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, marks(c + u * COMPUTE));
+                    }
+                    for (; c < cur.copied; c += COMPUTE, buf += COMPUTE) {
+                        const uint4 q = buf[0];
+                        G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+                        G.chunk(q, A.sc, marks(c));
+                    }
+                    // what did not fit
+                    for (c = cur.copied + tid; c < cur.n; c += 4 * COMPUTE) {
+                        uint4 q[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            if (c + u * COMPUTE < cur.n) q[u] = ld_stream(cur.x + (size_t)(c + u * COMPUTE) * E);
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            if (c + u * COMPUTE < cur.n) {
+                                G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
+                                G.chunk(q[u], A.sc, marks(c + u * COMPUTE));
+                            }
+                    }
                 }
-            if (!first) continue;
-            const float p = ex2((s_c[i] - m) * k - l2f);
-            gout[id] = from_f<T>((p * q_all - w * A.sc.m * q) * slope<CAP>(s_c[i], A.sc));
+                const Stat st = fold_lanes<TAIL, 32>(G.stat(), k);
+                // (a copy that never came: the row is NaN)
+                if (lane == 0) sh.part[i & 1][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
+                bar_arrive(BAR_X + (i & 1), COMPUTE + 32);
+            }
+            if (i > 0) {
+                const uint32_t j = i - 1;
+                bar_sync(BAR_Y + (j & 1), COMPUTE + 32);
+                if (grad) {
+                    const Coef cf = sh.coef[j & 3];
+                    T *row_out = (T *)A.grad + (size_t)row_of(j) * A.ld_grad;
+                    T *out = row_out + (prev.x - ((const T *)A.x + (size_t)row_of(j) * A.ld));   // of the slice
+                    const bool wide = ((uintptr_t)out & 15u) == 0;   // aligned like the logits
+                    auto store = [&](uint32_t c, const uint4 &q) {
+                        T *g = out + (size_t)c * E;
+                        if (wide) *reinterpret_cast<uint4 *>(g) = q;
+                        else store_each<T>(g, q);
+                    };
+                    if (cf.live) {
+                        const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
+                        const uint4 *buf = prev.buf;
+                        if (wide) {
+                            uint4 *g = reinterpret_cast<uint4 *>(out) + tid;
+#pragma unroll 4
+                            for (uint32_t c = tid; c < prev.copied; c += COMPUTE, buf += COMPUTE, g += COMPUTE)
+                                *g = gr.template chunk<T, CAP>(*buf, A.sc);
+                        } else {
+                            for (uint32_t c = tid; c < prev.copied; c += COMPUTE, buf += COMPUTE)
+                                store(c, gr.template chunk<T, CAP>(*buf, A.sc));
+                        }
+                        for (uint32_t c = prev.copied + tid; c < prev.n; c += 4 * COMPUTE) {
+                            uint4 q[4];
+#pragma unroll
+                            for (int u = 0; u < 4; u++)
+                                if (c + u * COMPUTE < prev.n) q[u] = ld_stream(prev.x + (size_t)(c + u * COMPUTE) * E);
+#pragma unroll
+                            for (int u = 0; u < 4; u++)
+                                if (c + u * COMPUTE < prev.n) store(c + u * COMPUTE, gr.template chunk<T, CAP>(q[u], A.sc));
+                        }
+                        if (!DIST) {
+                            // the token's own element, written again by the thread that wrote its chunk (where
+                            // the token is a single element, warp A has it)
+                            const uint32_t tok = (uint32_t)sh.code[j & 7], t_at = tok - (uint32_t)(out - row_out);
+                            const uint32_t t = t_at / E, mine = t < prev.copied ? t : t - prev.copied;
+                            if (t < prev.n && mine % COMPUTE == tid)
+                                out[t_at] = from_f<T>((gr.one(cf.c_tok) + cf.ct) * slope<CAP>(cf.c_tok, A.sc));
+                        }
+                    } else {   // the row is left out: zeros
+                        for (uint32_t c = tid; c < prev.n; c += COMPUTE) store(c, make_uint4(0, 0, 0, 0));
+                    }
+                }
+                if (grad) bar_arrive(BAR_Z + (j & 3), ZTHREADS);
+            }
+            if (!grad && i < n) bar_arrive(BAR_Z + (i & 3), ZTHREADS);
+            prev = cur;
+        }
+    } else if (tid < COMPUTE + 32) {
+        // ---- warp A
+        struct Params {
+            TokenIn in;
+            T tok, edge;   // as loaded: a conversion here would wait for the load
+        };
+        auto edge_of = [&](uint32_t i) {
+            return rank == 0 ? Row<T>(A.x, A.ld, row_of(i), V).edge(lane) : -1;
+        };
+        auto params = [&](uint32_t i) {   // loads only; used an iteration later
+            Params p{};
+            const int32_t code = sh.code[i & 7];
+            if (code >= 0) {
+                const uint32_t row = row_of(i);
+                const T *x = (const T *)A.x + (size_t)row * A.ld;
+                p.in.w = weight(row);
+                if (!DIST) p.tok = x[code];
+                if (is_policy(OP)) {
+                    p.in.adv = A.adv[row];
+                    p.in.old_lp = A.old_lp[row];
+                    p.in.ref_lp = A.ref_lp ? A.ref_lp[row] : 0.0f;
+                }
+                const int32_t e = edge_of(i);
+                if (e >= 0) p.edge = x[e];
+            }
+            return p;
+        };
+        Params next = params(0);
+        float w4 = 0.0f;          // weight and token of row i + 4
+        int32_t t4 = -1;
+        auto load4 = [&](uint32_t i) {
+            if (i + 4 < n && lane == 0) {
+                w4 = weight(row_of(i + 4));
+                t4 = DIST ? 0 : A.tokens[row_of(i + 4)];
+            }
+        };
+        load4(0);
+        for (uint32_t i = 0; i < n; i++) {
+            const Params cur = next;
+            const uint32_t row = row_of(i);
+            if (i + 1 < n) next = params(i + 1);
+            if (lane == 0 && i + 4 < n) sh.code[(i + 4) & 7] = w4 != 0.0f && (uint32_t)t4 < V ? t4 : -1;
+            load4(i + 1);
+            bar_sync(BAR_X + (i & 1), COMPUTE + 32);
+            bool live = sh.code[i & 7] >= 0;
+            if (DIST && live) live = sh.slots_live[i & 3] != 0u;
+            const int32_t edge = edge_of(i);
+            const float c_edge = capped<CAP>(to_f(cur.edge), A.sc);
+            const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(cur.tok), A.sc);
+            Stat st{-INFINITY, 0.0f, 0.0f};
+            if (lane < CWARPS) {
+                const float4 f = sh.part[i & 1][lane];
+                st = Stat{f.x, f.y, f.z};
+            }
+            if (live && edge >= 0) {
+                const bool marked = TAIL && (sh.edge_marks[i & 3] >> lane & 1u);
+                // one logit: 2^0 at itself, nothing where it is -inf (or a sum of NaN)
+                const float one = c_edge == -INFINITY ? 0.0f : c_edge - c_edge == 0.0f ? 1.0f : NAN;
+                const Stat e{c_edge, marked ? 0.0f : one, marked ? one : 0.0f};
+                const float m = c_edge != c_edge ? st.m : fmaxf(st.m, c_edge);
+                const float fa = ex2(fmaxf((st.m - m) * k, D_MIN)), fb = ex2(fmaxf((e.m - m) * k, D_MIN));
+                if (TAIL) {
+                    st = Stat{m, st.s * fa + e.s * fb, st.u * fa + e.u * fb};
+                } else {
+                    const float da = fmaxf((st.m - m) * k, D_MIN), db = fmaxf((e.m - m) * k, D_MIN);
+                    st = Stat{m, st.s * fa + e.s * fb, fa * fmaf(da, st.s, st.u) + fb * (db * e.s)};
+                }
+            }
+            st = fold_lanes<TAIL, 32>(st, k);
+            if (ranks > 1) {
+                // A CTA sends row i's only after all have sent row i - 1's, so have read row i - 2's.  The token's
+                // logit goes along so that it has been read before another CTA may write the gradient over it.
+                if (lane < ranks) mail_send(&sh.mail[i & 1][rank], &sh.mail_bar[i & 1], lane, st, c_tok);
+                if (lane == 0) bar_expect(&sh.mail_bar[i & 1], ranks * 16);
+                const bool there = bar_wait(&sh.mail_bar[i & 1], i >> 1 & 1);
+                st = Stat{-INFINITY, 0.0f, 0.0f};
+                if (lane < ranks) {
+                    const float4 f = sh.mail[i & 1][lane];
+                    st = Stat{f.x, there ? f.y : NAN, f.z};   // (a CTA that never sent: the row is NaN)
+                }
+                st = fold_lanes<TAIL, MAX_CLUSTER>(st, k);
+                st.m = __shfl_sync(~0u, st.m, 0);
+                st.s = __shfl_sync(~0u, st.s, 0);
+                st.u = __shfl_sync(~0u, st.u, 0);
+            }
+            const bool write = rank == 0 && lane == 0;
+            Coef cf{};
+            if (live) {
+                if constexpr (DIST) {
+                    cf = teacher_row<TAIL>(A, row, st, slots(i), cur.in.w, write);
+                } else {
+                    TokenIn in = cur.in;
+                    in.c_tok = c_tok;
+                    cf = token_row<OP>(A, row, st, in, write);
+                }
+            } else if (write) {
+                if (A.logprobs) A.logprobs[row] = 0.0f;
+                if (A.entropy) A.entropy[row] = 0.0f;
+                if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
+                if (A.kl) A.kl[row] = 0.0f;
+                if (A.row_loss) A.row_loss[row] = 0.0f;
+            }
+            if (grad && edge >= 0) {
+                float o = 0.0f;
+                if (live) {
+                    const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
+                    o = (gr.one(c_edge) + (!DIST && edge == sh.code[i & 7] ? cf.ct : 0.0f)) * slope<CAP>(c_edge, A.sc);
+                }
+                ((T *)A.grad)[(size_t)row * A.ld_grad + edge] = from_f<T>(o);
+            }
+            if (lane == 0) sh.coef[i & 3] = cf;
+            __syncwarp();
+            bar_arrive(BAR_Y + (i & 1), COMPUTE + 32);
+        }
+    } else if (tid < COMPUTE + 64) {
+        // ---- warp C: row i + 3 into row i's buffer
+        auto copy = [&](uint32_t i) {
+            uint64_t *bar = &sh.full_bar[i % 3];
+            const Row<T> R(A.x, A.ld, row_of(i), V);
+            const Slice sl = slice_of(R);
+            const uint32_t copied = sh.code[i & 7] < 0 ? 0u : min(sl.c1 - sl.c0, A.keep);
+            if (lane == 0) bar_expect(bar, copied * 16);
+            __syncwarp();
+            uint4 *buf = dyn + (i % 3) * A.keep;
+            for (uint32_t c = lane * COPY; c < copied; c += 32 * COPY)
+                copy_bulk(buf + c, R.at(sl.c0 + c), min(copied - c, COPY) * 16, bar);
+        };
+        for (uint32_t i = 0; i < 3 && i < n; i++) copy(i);
+        for (uint32_t i = 0; i < n; i++) {
+            bar_sync(BAR_Z + (i & 3), ZTHREADS);
+            if (i + 3 < n) copy(i + 3);
+        }
+    } else if constexpr (DIST) {
+        // ---- warps B
+        const uint32_t b = tid - COMPUTE - 64;
+        auto b_max = [&](float v) {   // (a NaN stays)
+            for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+            bar_sync(BAR_B, BTHREADS);
+            if (lane == 0) sh.scratch_f[b >> 5] = v;
+            bar_sync(BAR_B, BTHREADS);
+            for (int i = 0; i < BTHREADS / 32; i++) v = max_nan(v, sh.scratch_f[i]);
+            return v;
+        };
+        // loads of the first slot of a thread, an iteration before their use
+        int32_t id_next = -1;
+        float t_next = 0.0f;
+        auto fetch = [&](uint32_t i) {
+            if (i < n && b < A.n_ids) {
+                id_next = A.t_ids[(size_t)row_of(i) * A.n_ids + b];
+                t_next = A.t_logits[(size_t)row_of(i) * A.n_ids + b];
+            }
+        };
+        auto prepare = [&](uint32_t i) {
+            const uint32_t row = row_of(i), set = i & 3;
+            const size_t at = (size_t)row * A.n_ids;
+            const Slots sl = slots(i);
+            const Row<T> R(A.x, A.ld, row, V);
+            const Slice part = slice_of(R);
+            const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
+            const bool wanted = weight(row) != 0.0f;
+            const float ref_lse = TAIL ? A.t_lse[row] : 0.0f;
+            float umax = -INFINITY, any = 0.0f;
+            if (b == 0) sh.edge_marks[set] = 0u;
+            if (wanted) {
+                for (uint32_t j = b; j < pad; j += BTHREADS) {
+                    int32_t id = -1;
+                    float t = 0.0f;
+                    if (j < A.n_ids) {
+                        id = j == b ? id_next : A.t_ids[at + j];
+                        t = j == b ? t_next : A.t_logits[at + j];
+                    }
+                    if ((uint32_t)id >= V) id = -1;
+                    sl.id[j] = id;
+                    sl.q[j] = t;
+                    if (id >= 0) {
+                        sl.c[j] = capped<CAP>(to_f(R.x[id]), A.sc);
+                        any = 1.0f;
+                        umax = max_nan(umax, t);
+                    }
+                }
+            }
+            fetch(i + 1);
+            bool live = b_max(any) != 0.0f;
+            if (!TAIL) {
+                umax = b_max(umax);
+                live = live && umax != -INFINITY;   // no share to give: as without ids
+            }
+            if (live) {
+                const double ref = TAIL ? (double)ref_lse : (double)umax * A.sc.inv_t;
+                double sum = 0.0;
+                for (uint32_t j = b; j < pad; j += BTHREADS) {
+                    const int32_t id = sl.id[j];
+                    const float q = id < 0 ? 0.0f : expf((float)((double)sl.q[j] * A.sc.inv_t - ref));
+                    sl.q[j] = q;
+                    sum += (double)q;
+                    if (TAIL && id >= 0) {
+                        const uint32_t e = (uint32_t)id - e0;
+                        if (e < span) atomicOr(&sl.bits[e >> 5], 1u << (e & 31));
+                        else if ((uint32_t)id < R.lead) atomicOr(&sh.edge_marks[set], 1u << id);
+                        else if ((uint32_t)id >= V - R.trail) atomicOr(&sh.edge_marks[set], 256u << (id - (V - R.trail)));
+                    }
+                }
+                if (!TAIL) {
+                    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+                    bar_sync(BAR_B, BTHREADS);
+                    if (lane == 0) sh.scratch_d[b >> 5] = sum;
+                    bar_sync(BAR_B, BTHREADS);
+                    sum = 0.0;
+                    for (int j = 0; j < BTHREADS / 32; j++) sum += sh.scratch_d[j];
+                    for (uint32_t j = b; j < pad; j += BTHREADS) sl.q[j] /= (float)sum;
+                }
+            }
+            if (b == 0) sh.slots_live[set] = live ? 1u : 0u;
+        };
+        auto finish = [&](uint32_t i) {
+            const uint32_t row = row_of(i), set = i & 3;
+            const Slots sl = slots(i);
+            const Coef cf = sh.coef[set];
+            const Row<T> R(A.x, A.ld, row, V);
+            const Slice part = slice_of(R);
+            const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
+            if (!sh.slots_live[set]) return;
+            T *out = (T *)A.grad + (size_t)row * A.ld_grad;
+            for (uint32_t j = b; j < A.n_ids; j += BTHREADS) {
+                const int32_t id = sl.id[j];
+                if (id < 0) continue;
+                const uint32_t e = (uint32_t)id - e0;
+                const bool single = (uint32_t)id < R.lead || (uint32_t)id >= V - R.trail;
+                if (single ? rank != 0 : e >= span) continue;
+                if (TAIL && !single) sl.bits[e >> 5] = 0u;
+                if (!grad) continue;
+                // p Q - q, where q is the sum over the slots that hold the id (the first of them writes)
+                float q = 0.0f;
+                bool first = true;
+                for (uint32_t o = 0; o < pad; o += 4) {
+                    const int4 v = *reinterpret_cast<const int4 *>(sl.id + o);
+                    if (v.x == id) q += sl.q[o], first = first && o >= j;
+                    if (v.y == id) q += sl.q[o + 1], first = first && o + 1 >= j;
+                    if (v.z == id) q += sl.q[o + 2], first = first && o + 2 >= j;
+                    if (v.w == id) q += sl.q[o + 3], first = first && o + 3 >= j;
+                }
+                if (!first) continue;
+                const float p = ex2(fmaf(sl.c[j] - cf.m, k, -cf.l2s));
+                out[id] = from_f<T>((p * cf.q_all - cf.wm * q) * slope<CAP>(sl.c[j], A.sc));
+            }
+        };
+        // P of row i may be signalled once P of row i - 2 has been waited for: after Z of row i - 3
+        fetch(0);
+        for (uint32_t i = 0; i < 3 && i < n; i++) {
+            prepare(i);
+            if (i < 2) bar_arrive(BAR_P + (i & 1), COMPUTE + BTHREADS);
+        }
+        for (uint32_t i = 0; i < n; i++) {
+            bar_sync(BAR_Z + (i & 3), ZTHREADS);   // row i's gradient is written
+            if (i + 2 < n) bar_arrive(BAR_P + (i & 1), COMPUTE + BTHREADS);
+            finish(i);
+            if (i + 3 < n) {
+                bar_sync(BAR_B, BTHREADS);
+                prepare(i + 3);   // (its set was row i - 1's)
+            }
         }
     }
 }
@@ -775,9 +1118,12 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
     const int32_t edge = slice == 0 && tid < 32 ? R.edge(tid) : -1;
     const int32_t tok = A.tokens[row];
     const bool live = (uint32_t)tok < V;
-    float m = 0.0f, l2s = 0.0f, g = 0.0f, ca = 0.0f, cb = 0.0f;
+    const uint32_t t = ((uint32_t)tok - R.lead) / E;                          // the token's chunk,
+    const bool own = live && t - c0 < c1 - c0 && (t - c0) % THREADS == tid;   // and whether this thread has it
+    float m = 0.0f, l2s = 0.0f, g = 0.0f, ca = 0.0f, cb = 0.0f, c_tok = 0.0f;
     const float k = A.sc.k;
     if (live) {
+        if (own) c_tok = capped<CAP>(to_f(R.x[tok]), A.sc);
         const float2 st = stats[row];
         m = st.x;
         l2s = st.y * (float)(1.0 / LN2_D);
@@ -798,8 +1144,6 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
         return;
     }
     const T *body = R.at(0);
-    const uint32_t t_at = (uint32_t)tok - R.lead;
-    const uint32_t t_chunk = (uint32_t)tok >= R.lead && t_at / E < R.chunks ? t_at / E : ~0u;
     for (uint32_t c = c0 + tid; c < c1; c += GRAD_BATCH * THREADS) {
         uint4 q[GRAD_BATCH];
 #pragma unroll
@@ -808,9 +1152,11 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
 #pragma unroll
         for (int u = 0; u < GRAD_BATCH; u++) {
             const uint32_t cu = c + u * THREADS;
-            if (cu < c1) store(cu, gr.template chunk<T, CAP>(q[u], A.sc, cu == t_chunk ? t_at % E : ~0u, g));
+            if (cu < c1) store(cu, gr.template chunk<T, CAP>(q[u], A.sc));
         }
     }
+    // the token's own element, written again by the thread that wrote its chunk
+    if (own) gout[tok] = from_f<T>((gr.one(c_tok) + g) * slope<CAP>(c_tok, A.sc));
     if (edge >= 0) {
         const float cv = capped<CAP>(to_f(R.x[edge]), A.sc);
         const float o = gr.one(cv) + (edge == tok ? g : 0.0f);
@@ -861,6 +1207,7 @@ __device__ __forceinline__ uint32_t pick_bin(const uint32_t *hist, uint32_t &nee
     return 0u;
 }
 
+constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
 constexpr int TOP_CAND = 2048;       // candidates of a row
 constexpr int TOP_BINS = 2048;
 constexpr int TOP_TILE = 8;          // chunks of a tile: 128 bytes
@@ -1146,75 +1493,126 @@ static bs_status check_grad(const bs_logits *x, const void *grad, size_t ld_grad
 constexpr int MAX_DEVICES = 64;
 constexpr int SMEM_MAX = 227 * 1024;
 
-// Launches kernel K as clusters of `ranks` CTAs, one cluster per row.  The
-// first launch on a device lets the kernel use all of an SM's shared memory
-// (per device, as kernel attributes are; twice does no harm).
+// What a kernel needs to know of a device, found out by the first launch there
+// (twice does no harm).
+struct DeviceInfo {
+    std::atomic<int> sms{0};
+    std::atomic<int> clusters[4] = {};   // clusters of 1, 2, 4, 8 CTAs that run at once
+    std::atomic<bool> ready{false};
+};
+
 template <auto K, typename... Q>
-static bs_status launch_rows(const char *what, uint32_t rows, uint32_t ranks, size_t smem, cudaStream_t st, Q... args) {
-    static std::atomic<bool> ready[MAX_DEVICES];
-    if ((uint64_t)rows * ranks > 0x7FFFFFFFull) return BS_EINVAL;
+static cudaError_t launch_clusters(uint32_t grid, uint32_t ranks, uint32_t threads, size_t smem, cudaStream_t st, Q... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, K, args...);
+}
+
+// The current device's entry of kernel K's table, with K allowed all of an
+// SM's shared memory (per device, as kernel attributes are).
+template <auto K> static cudaError_t device_info(DeviceInfo **out) {
+    static DeviceInfo table[MAX_DEVICES];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && (dev < 0 || dev >= MAX_DEVICES)) e = cudaErrorInvalidDevice;
-    if (e == cudaSuccess && !ready[dev].load(std::memory_order_acquire)) {
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
+    DeviceInfo &d = table[dev];
+    if (!d.ready.load(std::memory_order_acquire)) {
         cudaFuncAttributes fa;
+        int sms = 0;
         e = cudaFuncGetAttributes(&fa, K);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - (int)fa.sharedSizeBytes);
-        if (e == cudaSuccess) ready[dev].store(true, std::memory_order_release);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        d.sms.store(sms);
+        d.ready.store(true, std::memory_order_release);
     }
-    if (e == cudaSuccess) {
+    *out = &d;
+    return cudaSuccess;
+}
+
+static bs_status failed(const char *what, cudaError_t e) {
+    cudaGetLastError();
+    fprintf(stderr, "b200_sampler: %s: launch failed: %s\n", what, cudaGetErrorString(e));
+    return BS_ECUDA;
+}
+
+// CTAs per row of k_top: few rows still fill the GPU, no CTA has less than two
+// chunks a thread.
+static uint32_t top_ranks(uint32_t rows, uint32_t chunks) {
+    uint32_t r = 1;
+    while (r < MAX_CLUSTER && (uint64_t)rows * r < 148 * 4 && chunks / (2 * r) >= 2 * THREADS) r *= 2;
+    return r;
+}
+
+// Shared memory of k_rows: three buffers of a slice, the teacher's slots.
+constexpr size_t ROWS_SMEM = SMEM_MAX - sizeof(RowsShared) - 256;
+constexpr uint32_t SLICE_MIN = 2 * COMPUTE;   // no row is split further than two chunks a thread
+
+template <typename T, int OP, bool CAP>
+static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
+    constexpr auto K = k_rows<T, OP, CAP>;
+    constexpr uint32_t E = 16 / sizeof(T);
+    DeviceInfo *dev;
+    cudaError_t e = device_info<K>(&dev);
+    if (e != cudaSuccess) return failed("logit_ops", e);
+    const uint32_t chunks = A.vocab / E;
+    uint32_t ranks = 1, log_ranks = 0, slice = 0;
+    size_t slots = 0, room = 0;
+    for (;; ranks *= 2, log_ranks++) {
+        slice = (chunks + ranks - 1) / ranks;
+        A.bit_words = OP == OP_DISTILL_TAIL ? (slice * E + 31) / 32 : 0;
+        slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 48 + (size_t)A.bit_words * 16 : 0;
+        room = slots < ROWS_SMEM ? (ROWS_SMEM - slots) / 48 : 0;
+        // enough CTAs to hold the row, and to use the GPU where the rows are few
+        if (ranks == MAX_CLUSTER ||
+            (slice <= room && !((uint64_t)rows * ranks * 2 <= (uint64_t)dev->sms.load() && slice / 2 >= SLICE_MIN)))
+            break;
+    }
+    if (slots >= ROWS_SMEM) return BS_ENOTSUP;
+    A.keep = slice < room ? slice : (uint32_t)room;
+    A.log_ranks = log_ranks;
+    // one CTA per SM: all of its shared memory is asked for
+    int most = dev->clusters[log_ranks].load(std::memory_order_relaxed);
+    if (most == 0) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(rows * ranks);
-        cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
+        cfg.gridDim = dim3(ranks);
+        cfg.blockDim = dim3(row_threads(OP));
+        cfg.dynamicSmemBytes = ROWS_SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = ranks;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, K, args...);
+        e = cudaOccupancyMaxActiveClusters(&most, K, &cfg);
+        if (e == cudaSuccess && most <= 0) e = cudaErrorInvalidConfiguration;
+        if (e != cudaSuccess) return failed("logit_ops", e);
+        dev->clusters[log_ranks].store(most, std::memory_order_relaxed);
     }
-    if (e == cudaSuccess) return BS_OK;
-    cudaGetLastError();
-    fprintf(stderr, "b200_sampler: %s: launch failed: %s\n", what, cudaGetErrorString(e));
-    return BS_ECUDA;
-}
-
-constexpr uint32_t KEEP_MAX = 72 * 64;     // chunks kept by a CTA: 72 KB, three CTAs to an SM
-constexpr uint32_t SLICE_MIN = 2 * THREADS;   // no CTA with less than two chunks a thread
-constexpr uint32_t GRID_FULL = 148 * 4;
-
-// CTAs per row: enough that a slice fits in shared memory (where one is kept)
-// and that few rows still fill the GPU.
-static uint32_t row_ranks(uint32_t rows, uint32_t chunks, bool keep) {
-    uint32_t r = 1;
-    while (r < MAX_CLUSTER && ((keep && (chunks + r - 1) / r > KEEP_MAX) ||
-                               ((uint64_t)rows * r < GRID_FULL && chunks / (2 * r) >= SLICE_MIN)))
-        r *= 2;
-    return r;
-}
-
-template <typename T, int OP>
-static bs_status launch_row(RowArgs A, uint32_t rows, bool cap, cudaStream_t st) {
-    constexpr uint32_t E = 16 / sizeof(T);
-    const uint32_t chunks = A.vocab / E, ranks = row_ranks(rows, chunks, A.grad != nullptr);
-    const uint32_t slice = (chunks + ranks - 1) / ranks;
-    A.keep = A.grad ? (slice < KEEP_MAX ? slice : KEEP_MAX) : 0;
-    size_t smem = (size_t)A.keep * 16 + (size_t)A.n_ids * 12;
-    if (OP == OP_DISTILL_TAIL) smem += ((size_t)slice * E + 31) / 32 * 4;
-    return cap ? launch_rows<k_row<T, OP, true>>("logit_ops", rows, ranks, smem, st, A)
-               : launch_rows<k_row<T, OP, false>>("logit_ops", rows, ranks, smem, st, A);
+    const uint32_t clusters = rows < (uint32_t)most ? rows : (uint32_t)most;
+    e = launch_clusters<K>(clusters * ranks, ranks, row_threads(OP), ROWS_SMEM, st, A, rows, clusters);
+    return e == cudaSuccess ? BS_OK : failed("logit_ops", e);
 }
 
 template <int OP>
 static bs_status launch_row_typed(const bs_logits *x, const RowArgs &A, bool cap, cudaStream_t st) {
     switch (x->dtype) {
-        case BS_F32: return launch_row<float, OP>(A, x->rows, cap, st);
-        case BS_BF16: return launch_row<__nv_bfloat16, OP>(A, x->rows, cap, st);
-        default: return launch_row<__half, OP>(A, x->rows, cap, st);
+        case BS_F32: return cap ? launch_row<float, OP, true>(A, x->rows, st) : launch_row<float, OP, false>(A, x->rows, st);
+        case BS_BF16:
+            return cap ? launch_row<__nv_bfloat16, OP, true>(A, x->rows, st)
+                       : launch_row<__nv_bfloat16, OP, false>(A, x->rows, st);
+        default: return cap ? launch_row<__half, OP, true>(A, x->rows, st) : launch_row<__half, OP, false>(A, x->rows, st);
     }
 }
 
@@ -1374,16 +1772,25 @@ extern "C" bs_status bs_distill_loss(const bs_logits *x, const int32_t *d_teache
     return st != BS_OK ? st : total_loss(A, x->rows, d_loss, s);
 }
 
+template <typename T, bool CAP>
+static bs_status launch_top(const bs_logits *x, const Scale &sc, float os, uint32_t k, float *values, int32_t *ids,
+                            float *lse, cudaStream_t st) {
+    constexpr auto K = k_top<T, CAP>;
+    DeviceInfo *dev;
+    cudaError_t e = device_info<K>(&dev);
+    const uint32_t chunks = x->vocab / (16 / sizeof(T)), ranks = top_ranks(x->rows, chunks);
+    if ((uint64_t)x->rows * ranks > 0x7FFFFFFFull) return BS_EINVAL;
+    const size_t smem = ((size_t)chunks / TOP_TILE + 2) * 4;
+    if (e == cudaSuccess)
+        e = launch_clusters<K>(x->rows * ranks, ranks, THREADS, smem, st, x->data, x->ld, x->vocab, sc, os, k, values, ids,
+                               lse);
+    return e == cudaSuccess ? BS_OK : failed("bs_top_logits", e);
+}
 template <typename T>
 static bs_status launch_top(const bs_logits *x, const Scale &sc, float os, bool cap, uint32_t k, float *values,
                             int32_t *ids, float *lse, cudaStream_t st) {
-    const uint32_t chunks = x->vocab / (16 / sizeof(T));
-    const size_t smem = ((size_t)chunks / TOP_TILE + 2) * 4;
-    const uint32_t ranks = row_ranks(x->rows, chunks, false);
-    return cap ? launch_rows<k_top<T, true>>("bs_top_logits", x->rows, ranks, smem, st, x->data, x->ld, x->vocab, sc, os,
-                                             k, values, ids, lse)
-               : launch_rows<k_top<T, false>>("bs_top_logits", x->rows, ranks, smem, st, x->data, x->ld, x->vocab, sc,
-                                              os, k, values, ids, lse);
+    return cap ? launch_top<T, true>(x, sc, os, k, values, ids, lse, st)
+               : launch_top<T, false>(x, sc, os, k, values, ids, lse, st);
 }
 
 extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t *d_ids, float *d_lse,
