@@ -27,7 +27,7 @@ namespace ops {
 
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int MAX_CLUSTER = 8;       // CTAs of a row
+constexpr int MAX_CLUSTER = 16;      // CTAs of a row (8 is the portable limit; 16 where a row needs it)
 constexpr float LN2 = 0.6931471805599453f;
 constexpr double LN2_D = 0.6931471805599453;
 // 2^d is zero in f32 below this; products with d stop here, so that a logit
@@ -475,26 +475,29 @@ template <bool ENT> struct GradRow {
 // between its CTAs, the sums of row i travel while the gradient of row i - 1
 // is written and row i + 1 is loaded:
 //
-//   compute warps       iteration i: wait for row i; sum it; write row i - 1's
-//                       gradient.
-//   warp A              adds up the CTA's sums and exchanges them with the
-//                       other CTAs of the row; the row's results and its
-//                       gradient's coefficients; the single elements before
-//                       and behind the 16-byte chunks.
-//   warp C              bulk copies of the rows to come.
-//   warps B (4)         losses with a teacher: the slots of row i + 2 (shares
-//                       q, the student's logits there), and after the gradient
-//                       of row i - 1 the tokens that the teacher names.
+//   warps S             sum row i as soon as its copy is there,
+//   warps A             (two, taking turns) add up the CTA's sums and exchange
+//                       them with the row's other CTAs; the row's results and
+//                       its gradient's coefficients; the single elements
+//                       before and behind the 16-byte chunks,
+//   warps G             write the gradient (without one, these sum too),
+//   warp C              starts the copy of row i + 3 into row i's buffer,
+//   warps B             losses with a teacher: prepare the slots of the rows
+//                       to come (shares q, the student's logits there), and
+//                       after row i's gradient write the tokens that its
+//                       teacher names.
 //
-// The barriers, each in two copies (Z: four) that take turns: X (compute -> A: the sums
-// of row i), Y (A -> compute: row i's coefficients), P (B -> compute: slots of
-// row i), Z (compute -> B, C: row i done with).
-constexpr int COMPUTE = 384;
+// Summing and gradient each need one ex2 a logit, so half of the warps do
+// either, and the special-function unit always has work while a row's sums
+// travel.  Barriers, in as many copies as rows can be between the two sides:
+// X (S -> A: row i summed), Y (A -> G: its coefficients), P (B -> S: its
+// slots), Z (-> C, B: done with; from G, or without a gradient from S and A).
+constexpr int COMPUTE = 512;
 constexpr uint32_t COPY = 512;       // chunks of one copy
 constexpr int STEP = 4;              // chunks of a thread summed at a time
 constexpr int CWARPS = COMPUTE / 32;
 constexpr int BTHREADS = 128;
-enum Bar { BAR_X = 1, BAR_Y = 3, BAR_P = 5, BAR_Z = 7, BAR_B = 11 };
+enum Bar { BAR_X = 1, BAR_Y = 5, BAR_Z = 9, BAR_P = 13, BAR_B = 15 };
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -510,7 +513,7 @@ __device__ __forceinline__ void copy_bulk(void *dst, const void *src, uint32_t b
 
 __host__ __device__ constexpr bool is_distill(int op) { return op == OP_DISTILL || op == OP_DISTILL_TAIL; }
 __host__ __device__ constexpr bool is_policy(int op) { return op == OP_POLICY || op == OP_POLICY_ENT; }
-__host__ __device__ constexpr int row_threads(int op) { return COMPUTE + 64 + (is_distill(op) ? BTHREADS : 0); }
+__host__ __device__ constexpr int row_threads(int op) { return COMPUTE + 96 + (is_distill(op) ? BTHREADS : 0); }
 
 // Row i's results as the gradient needs them.
 struct Coef {
@@ -521,10 +524,10 @@ struct Coef {
     uint32_t live;       // 0: the row is left out
 };
 struct RowsShared {
-    float4 part[2][CWARPS];          // (m, s, u) of the compute warps
+    float4 part[4][CWARPS];          // (m, s, u) of the warps S
     float4 mail[2][MAX_CLUSTER];     // and of the row's CTAs
     Coef coef[4];
-    int32_t code[8];                 // the row's token (0 for a teacher's row); -1: left out
+    int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
     // B's
     double scratch_d[BTHREADS / 32];
     float scratch_f[BTHREADS / 32];
@@ -670,7 +673,6 @@ template <typename T, int OP, bool CAP>
 __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t rows, uint32_t clusters) {
     constexpr bool DIST = is_distill(OP), TAIL = OP == OP_DISTILL_TAIL;
     constexpr int E = Row<T>::E;
-    constexpr int ZTHREADS = COMPUTE + 32 + (DIST ? BTHREADS : 0);
     extern __shared__ uint4 dyn[];
     __shared__ __align__(16) RowsShared sh;
     const uint32_t ranks = 1u << A.log_ranks, rank = cluster_rank();
@@ -678,6 +680,10 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
     const uint32_t n = (rows - cluster + clusters - 1) / clusters;   // rows of this cluster
     const float k = A.sc.k;
     const bool grad = A.grad != nullptr;
+    // threads of S and G, and of the barriers
+    const uint32_t sum_threads = grad ? COMPUTE / 2 : COMPUTE, x_threads = sum_threads + 32;
+    const uint32_t y_threads = COMPUTE / 2 + 32, p_threads = sum_threads + BTHREADS;
+    const uint32_t z_threads = (grad ? COMPUTE / 2 : COMPUTE + 32) + 32 + (DIST ? BTHREADS : 0);
     auto row_of = [&](uint32_t i) { return cluster + i * clusters; };
     auto weight = [&](uint32_t row) {
         return OP == OP_LOGPROB ? 1.0f : A.weights ? A.weights[row] : A.w_all;
@@ -710,7 +716,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             sh.code[lane] = weight(row) != 0.0f && (uint32_t)tok < V ? tok : -1;
         }
     } else if (TAIL && tid >= COMPUTE) {
-        for (uint32_t i = tid - COMPUTE - 32; i < 4 * A.bit_words; i += BTHREADS + 32) slots(0).bits[i] = 0;
+        for (uint32_t i = tid - COMPUTE - 32; i < 4 * A.bit_words; i += BTHREADS + 64) slots(0).bits[i] = 0;
     }
     if (tid == 0) {
         bar_init(&sh.mail_bar[0]);
@@ -724,120 +730,117 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
         cluster_wait();
     }
 
-    if (tid < COMPUTE) {
-        // ---- compute warps; thread tid has the chunks tid, tid + COMPUTE, ... of the slice
-        struct Part {                // a row's slice: its chunks, and how many of them are copied
-            const T *x;
-            uint32_t n, copied;
-            const uint4 *buf;
-        };
-        Part prev{}, cur{};
+    if (tid < sum_threads) {
+        // ---- warps S; thread tid has the chunks tid, tid + sum_threads, ... of the slice
         uint32_t at = 0, phase = 0;   // the buffers take turns
         bool there = true;
-        for (uint32_t i = 0; i <= n; i++) {
-            if (i < n) {
-                const Row<T> R(A.x, A.ld, row_of(i), V);
-                const Slice sl = slice_of(R);
-                cur = Part{R.at(sl.c0), sl.c1 - sl.c0, min(sl.c1 - sl.c0, A.keep), dyn + at * A.keep + tid};
-                there = bar_wait(&sh.full_bar[at], phase) && there;
-                if (++at == 3) at = 0, phase ^= 1;
-                if (DIST) bar_sync(BAR_P + (i & 1), COMPUTE + BTHREADS);
-                Gather<T, CAP, !DIST, TAIL> G;
-                if (sh.code[i & 7] >= 0) {
-                    const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
-                    auto marks = [&](uint32_t c) -> uint32_t {
-                        if (!TAIL) return 0u;
-                        const uint32_t b = c * E;
-                        return bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
-                    };
-                    // several chunks at a time, for one comparison with the running maximum
-                    const uint4 *buf = cur.buf;
-                    uint32_t c = tid;
-                    for (; c + (STEP - 1) * COMPUTE < cur.copied; c += STEP * COMPUTE, buf += STEP * COMPUTE) {
-                        uint4 q[STEP];
+        for (uint32_t i = 0; i < n; i++) {
+            const Row<T> R(A.x, A.ld, row_of(i), V);
+            const Slice sl = slice_of(R);
+            const uint32_t count = sl.c1 - sl.c0, copied = min(count, A.keep);
+            const uint4 *buf = dyn + at * A.keep + tid;
+            there = bar_wait(&sh.full_bar[at], phase) && there;
+            if (++at == 3) at = 0, phase ^= 1;
+            if (DIST) bar_sync(BAR_P + (i & 1), p_threads);
+            Gather<T, CAP, !DIST, TAIL> G;
+            if (sh.code[i & 15] >= 0) {
+                const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
+                auto marks = [&](uint32_t c) -> uint32_t {
+                    if (!TAIL) return 0u;
+                    const uint32_t b = c * E;
+                    return bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
+                };
+                // several chunks at a time, for one comparison with the running maximum
+                uint32_t c = tid;
+                for (; c + (STEP - 1) * sum_threads < copied; c += STEP * sum_threads, buf += STEP * sum_threads) {
+                    uint4 q[STEP];
 #pragma unroll
-                        for (int u = 0; u < STEP; u++) q[u] = buf[u * COMPUTE];
-                        G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+                    for (int u = 0; u < STEP; u++) q[u] = buf[u * sum_threads];
+                    G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
 #pragma unroll
-                        for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, marks(c + u * COMPUTE));
-                    }
-                    for (; c < cur.copied; c += COMPUTE, buf += COMPUTE) {
-                        const uint4 q = buf[0];
-                        G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
-                        G.chunk(q, A.sc, marks(c));
-                    }
-                    // what did not fit
-                    for (c = cur.copied + tid; c < cur.n; c += 4 * COMPUTE) {
-                        uint4 q[4];
-#pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            if (c + u * COMPUTE < cur.n) q[u] = ld_stream(cur.x + (size_t)(c + u * COMPUTE) * E);
-#pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            if (c + u * COMPUTE < cur.n) {
-                                G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
-                                G.chunk(q[u], A.sc, marks(c + u * COMPUTE));
-                            }
-                    }
+                    for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, marks(c + u * sum_threads));
                 }
-                const Stat st = fold_lanes<TAIL, 32>(G.stat(), k);
-                // (a copy that never came: the row is NaN)
-                if (lane == 0) sh.part[i & 1][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
-                bar_arrive(BAR_X + (i & 1), COMPUTE + 32);
-            }
-            if (i > 0) {
-                const uint32_t j = i - 1;
-                bar_sync(BAR_Y + (j & 1), COMPUTE + 32);
-                if (grad) {
-                    const Coef cf = sh.coef[j & 3];
-                    T *row_out = (T *)A.grad + (size_t)row_of(j) * A.ld_grad;
-                    T *out = row_out + (prev.x - ((const T *)A.x + (size_t)row_of(j) * A.ld));   // of the slice
-                    const bool wide = ((uintptr_t)out & 15u) == 0;   // aligned like the logits
-                    auto store = [&](uint32_t c, const uint4 &q) {
-                        T *g = out + (size_t)c * E;
-                        if (wide) *reinterpret_cast<uint4 *>(g) = q;
-                        else store_each<T>(g, q);
-                    };
-                    if (cf.live) {
-                        const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
-                        const uint4 *buf = prev.buf;
-                        if (wide) {
-                            uint4 *g = reinterpret_cast<uint4 *>(out) + tid;
-#pragma unroll 4
-                            for (uint32_t c = tid; c < prev.copied; c += COMPUTE, buf += COMPUTE, g += COMPUTE)
-                                *g = gr.template chunk<T, CAP>(*buf, A.sc);
-                        } else {
-                            for (uint32_t c = tid; c < prev.copied; c += COMPUTE, buf += COMPUTE)
-                                store(c, gr.template chunk<T, CAP>(*buf, A.sc));
-                        }
-                        for (uint32_t c = prev.copied + tid; c < prev.n; c += 4 * COMPUTE) {
-                            uint4 q[4];
-#pragma unroll
-                            for (int u = 0; u < 4; u++)
-                                if (c + u * COMPUTE < prev.n) q[u] = ld_stream(prev.x + (size_t)(c + u * COMPUTE) * E);
-#pragma unroll
-                            for (int u = 0; u < 4; u++)
-                                if (c + u * COMPUTE < prev.n) store(c + u * COMPUTE, gr.template chunk<T, CAP>(q[u], A.sc));
-                        }
-                        if (!DIST) {
-                            // the token's own element, written again by the thread that wrote its chunk (where
-                            // the token is a single element, warp A has it)
-                            const uint32_t tok = (uint32_t)sh.code[j & 7], t_at = tok - (uint32_t)(out - row_out);
-                            const uint32_t t = t_at / E, mine = t < prev.copied ? t : t - prev.copied;
-                            if (t < prev.n && mine % COMPUTE == tid)
-                                out[t_at] = from_f<T>((gr.one(cf.c_tok) + cf.ct) * slope<CAP>(cf.c_tok, A.sc));
-                        }
-                    } else {   // the row is left out: zeros
-                        for (uint32_t c = tid; c < prev.n; c += COMPUTE) store(c, make_uint4(0, 0, 0, 0));
-                    }
+                for (; c < copied; c += sum_threads, buf += sum_threads) {
+                    const uint4 q = buf[0];
+                    G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+                    G.chunk(q, A.sc, marks(c));
                 }
-                if (grad) bar_arrive(BAR_Z + (j & 3), ZTHREADS);
+                // what did not fit
+                const T *x = R.at(sl.c0);
+                for (c = copied + tid; c < count; c += STEP * sum_threads) {
+                    uint4 q[STEP];
+#pragma unroll
+                    for (int u = 0; u < STEP; u++)
+                        if (c + u * sum_threads < count) q[u] = ld_stream(x + (size_t)(c + u * sum_threads) * E);
+#pragma unroll
+                    for (int u = 0; u < STEP; u++)
+                        if (c + u * sum_threads < count) {
+                            G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
+                            G.chunk(q[u], A.sc, marks(c + u * sum_threads));
+                        }
+                }
             }
-            if (!grad && i < n) bar_arrive(BAR_Z + (i & 3), ZTHREADS);
-            prev = cur;
+            const Stat st = fold_lanes<TAIL, 32>(G.stat(), k);
+            // (a copy that never came: the row is NaN)
+            if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
+            bar_arrive(BAR_X + (i & 3), x_threads);
+            if (!grad) bar_arrive(BAR_Z + (i & 3), z_threads);
         }
-    } else if (tid < COMPUTE + 32) {
-        // ---- warp A
+    } else if (tid < COMPUTE) {
+        // ---- warps G
+        constexpr uint32_t GT = COMPUTE / 2;
+        const uint32_t g = tid - GT;
+        uint32_t at = 0;
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t row = row_of(i);
+            const Row<T> R(A.x, A.ld, row, V);
+            const Slice sl = slice_of(R);
+            const uint32_t count = sl.c1 - sl.c0, copied = min(count, A.keep);
+            const uint4 *buf = dyn + at * A.keep + g;
+            at = at == 2 ? 0 : at + 1;
+            T *out = (T *)A.grad + (size_t)row * A.ld_grad + R.lead + (size_t)sl.c0 * E;
+            const bool wide = ((uintptr_t)out & 15u) == 0;   // aligned like the logits
+            auto store = [&](uint32_t c, const uint4 &q) {
+                if (wide) *reinterpret_cast<uint4 *>(out + (size_t)c * E) = q;
+                else store_each<T>(out + (size_t)c * E, q);
+            };
+            bar_sync(BAR_Y + (i & 3), y_threads);
+            const Coef cf = sh.coef[i & 3];
+            if (cf.live) {
+                const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
+                if (wide) {
+                    uint4 *o = reinterpret_cast<uint4 *>(out) + g;
+#pragma unroll 4
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT) *o = gr.template chunk<T, CAP>(*buf, A.sc);
+                } else {
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT) store(c, gr.template chunk<T, CAP>(*buf, A.sc));
+                }
+                const T *x = R.at(sl.c0);
+                for (uint32_t c = copied + g; c < count; c += STEP * GT) {
+                    uint4 q[STEP];
+#pragma unroll
+                    for (int u = 0; u < STEP; u++)
+                        if (c + u * GT < count) q[u] = ld_stream(x + (size_t)(c + u * GT) * E);
+#pragma unroll
+                    for (int u = 0; u < STEP; u++)
+                        if (c + u * GT < count) store(c + u * GT, gr.template chunk<T, CAP>(q[u], A.sc));
+                }
+                if (!DIST) {
+                    // the token's own element, written again by the thread that wrote its chunk (where the token
+                    // is a single element, warp A has it)
+                    const uint32_t t_at = (uint32_t)sh.code[i & 15] - R.lead - sl.c0 * E;
+                    const uint32_t t = t_at / E, mine = t < copied ? t : t - copied;
+                    if (t < count && mine % GT == g)
+                        out[t_at] = from_f<T>((gr.one(cf.c_tok) + cf.ct) * slope<CAP>(cf.c_tok, A.sc));
+                }
+            } else {   // the row is left out: zeros
+                for (uint32_t c = g; c < count; c += GT) store(c, make_uint4(0, 0, 0, 0));
+            }
+            bar_arrive(BAR_Z + (i & 3), z_threads);
+        }
+    } else if (tid < COMPUTE + 64) {
+        // ---- warps A; this one has every other row
+        const uint32_t which = (tid - COMPUTE) >> 5;
         struct Params {
             TokenIn in;
             T tok, edge;   // as loaded: a conversion here would wait for the load
@@ -847,8 +850,8 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
         };
         auto params = [&](uint32_t i) {   // loads only; used an iteration later
             Params p{};
-            const int32_t code = sh.code[i & 7];
-            if (code >= 0) {
+            const int32_t code = sh.code[i & 15];
+            if (i < n && code >= 0) {
                 const uint32_t row = row_of(i);
                 const T *x = (const T *)A.x + (size_t)row * A.ld;
                 p.in.w = weight(row);
@@ -863,7 +866,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             }
             return p;
         };
-        Params next = params(0);
+        Params next = params(which);
         float w4 = 0.0f;          // weight and token of row i + 4
         int32_t t4 = -1;
         auto load4 = [&](uint32_t i) {
@@ -872,22 +875,22 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                 t4 = DIST ? 0 : A.tokens[row_of(i + 4)];
             }
         };
-        load4(0);
-        for (uint32_t i = 0; i < n; i++) {
+        load4(which);
+        for (uint32_t i = which; i < n; i += 2) {
             const Params cur = next;
             const uint32_t row = row_of(i);
-            if (i + 1 < n) next = params(i + 1);
-            if (lane == 0 && i + 4 < n) sh.code[(i + 4) & 7] = w4 != 0.0f && (uint32_t)t4 < V ? t4 : -1;
-            load4(i + 1);
-            bar_sync(BAR_X + (i & 1), COMPUTE + 32);
-            bool live = sh.code[i & 7] >= 0;
+            if (i + 2 < n) next = params(i + 2);
+            if (lane == 0 && i + 4 < n) sh.code[(i + 4) & 15] = w4 != 0.0f && (uint32_t)t4 < V ? t4 : -1;
+            load4(i + 2);
+            bar_sync(BAR_X + (i & 3), x_threads);
+            bool live = sh.code[i & 15] >= 0;
             if (DIST && live) live = sh.slots_live[i & 3] != 0u;
             const int32_t edge = edge_of(i);
             const float c_edge = capped<CAP>(to_f(cur.edge), A.sc);
             const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(cur.tok), A.sc);
             Stat st{-INFINITY, 0.0f, 0.0f};
-            if (lane < CWARPS) {
-                const float4 f = sh.part[i & 1][lane];
+            if (lane < sum_threads / 32) {
+                const float4 f = sh.part[i & 3][lane];
                 st = Stat{f.x, f.y, f.z};
             }
             if (live && edge >= 0) {
@@ -942,21 +945,22 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                 float o = 0.0f;
                 if (live) {
                     const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
-                    o = (gr.one(c_edge) + (!DIST && edge == sh.code[i & 7] ? cf.ct : 0.0f)) * slope<CAP>(c_edge, A.sc);
+                    o = (gr.one(c_edge) + (!DIST && edge == sh.code[i & 15] ? cf.ct : 0.0f)) * slope<CAP>(c_edge, A.sc);
                 }
                 ((T *)A.grad)[(size_t)row * A.ld_grad + edge] = from_f<T>(o);
             }
             if (lane == 0) sh.coef[i & 3] = cf;
             __syncwarp();
-            bar_arrive(BAR_Y + (i & 1), COMPUTE + 32);
+            if (grad) bar_arrive(BAR_Y + (i & 3), y_threads);
+            else bar_arrive(BAR_Z + (i & 3), z_threads);
         }
-    } else if (tid < COMPUTE + 64) {
+    } else if (tid < COMPUTE + 96) {
         // ---- warp C: row i + 3 into row i's buffer
         auto copy = [&](uint32_t i) {
             uint64_t *bar = &sh.full_bar[i % 3];
             const Row<T> R(A.x, A.ld, row_of(i), V);
             const Slice sl = slice_of(R);
-            const uint32_t copied = sh.code[i & 7] < 0 ? 0u : min(sl.c1 - sl.c0, A.keep);
+            const uint32_t copied = sh.code[i & 15] < 0 ? 0u : min(sl.c1 - sl.c0, A.keep);
             if (lane == 0) bar_expect(bar, copied * 16);
             __syncwarp();
             uint4 *buf = dyn + (i % 3) * A.keep;
@@ -965,12 +969,12 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
         };
         for (uint32_t i = 0; i < 3 && i < n; i++) copy(i);
         for (uint32_t i = 0; i < n; i++) {
-            bar_sync(BAR_Z + (i & 3), ZTHREADS);
+            bar_sync(BAR_Z + (i & 3), z_threads);
             if (i + 3 < n) copy(i + 3);
         }
     } else if constexpr (DIST) {
         // ---- warps B
-        const uint32_t b = tid - COMPUTE - 64;
+        const uint32_t b = tid - COMPUTE - 96;
         auto b_max = [&](float v) {   // (a NaN stays)
             for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
             bar_sync(BAR_B, BTHREADS);
@@ -979,14 +983,28 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             for (int i = 0; i < BTHREADS / 32; i++) v = max_nan(v, sh.scratch_f[i]);
             return v;
         };
-        // loads of the first slot of a thread, an iteration before their use
-        int32_t id_next = -1;
-        float t_next = 0.0f;
+        // Loads of a row ahead of their use: its weight, lse and (first of a thread) slot two iterations, the
+        // student's logit there one.
+        struct Ahead {
+            float w, lse, t;
+            int32_t id;
+        } one{}, two{};
+        T logit{};
         auto fetch = [&](uint32_t i) {
-            if (i < n && b < A.n_ids) {
-                id_next = A.t_ids[(size_t)row_of(i) * A.n_ids + b];
-                t_next = A.t_logits[(size_t)row_of(i) * A.n_ids + b];
+            Ahead f{0.0f, 0.0f, 0.0f, -1};
+            if (i < n) {
+                const uint32_t row = row_of(i);
+                f.w = weight(row);
+                if (TAIL) f.lse = A.t_lse[row];
+                if (b < A.n_ids) {
+                    f.id = A.t_ids[(size_t)row * A.n_ids + b];
+                    f.t = A.t_logits[(size_t)row * A.n_ids + b];
+                }
             }
+            return f;
+        };
+        auto fetch_logit = [&](uint32_t i) {
+            if (i < n && one.w != 0.0f && (uint32_t)one.id < V) logit = ((const T *)A.x)[(size_t)row_of(i) * A.ld + one.id];
         };
         auto prepare = [&](uint32_t i) {
             const uint32_t row = row_of(i), set = i & 3;
@@ -995,8 +1013,12 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             const Row<T> R(A.x, A.ld, row, V);
             const Slice part = slice_of(R);
             const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
-            const bool wanted = weight(row) != 0.0f;
-            const float ref_lse = TAIL ? A.t_lse[row] : 0.0f;
+            const Ahead cur = one;
+            const T cur_logit = logit;
+            one = two;
+            two = fetch(i + 2);
+            fetch_logit(i + 1);
+            const bool wanted = cur.w != 0.0f;
             float umax = -INFINITY, any = 0.0f;
             if (b == 0) sh.edge_marks[set] = 0u;
             if (wanted) {
@@ -1004,27 +1026,26 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                     int32_t id = -1;
                     float t = 0.0f;
                     if (j < A.n_ids) {
-                        id = j == b ? id_next : A.t_ids[at + j];
-                        t = j == b ? t_next : A.t_logits[at + j];
+                        id = j == b ? cur.id : A.t_ids[at + j];
+                        t = j == b ? cur.t : A.t_logits[at + j];
                     }
                     if ((uint32_t)id >= V) id = -1;
                     sl.id[j] = id;
                     sl.q[j] = t;
                     if (id >= 0) {
-                        sl.c[j] = capped<CAP>(to_f(R.x[id]), A.sc);
+                        sl.c[j] = capped<CAP>(to_f(j == b ? cur_logit : R.x[id]), A.sc);
                         any = 1.0f;
                         umax = max_nan(umax, t);
                     }
                 }
             }
-            fetch(i + 1);
             bool live = b_max(any) != 0.0f;
             if (!TAIL) {
                 umax = b_max(umax);
                 live = live && umax != -INFINITY;   // no share to give: as without ids
             }
             if (live) {
-                const double ref = TAIL ? (double)ref_lse : (double)umax * A.sc.inv_t;
+                const double ref = TAIL ? (double)cur.lse : (double)umax * A.sc.inv_t;
                 double sum = 0.0;
                 for (uint32_t j = b; j < pad; j += BTHREADS) {
                     const int32_t id = sl.id[j];
@@ -1083,14 +1104,16 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             }
         };
         // P of row i may be signalled once P of row i - 2 has been waited for: after Z of row i - 3
-        fetch(0);
+        one = fetch(0);
+        two = fetch(1);
+        fetch_logit(0);
         for (uint32_t i = 0; i < 3 && i < n; i++) {
             prepare(i);
-            if (i < 2) bar_arrive(BAR_P + (i & 1), COMPUTE + BTHREADS);
+            if (i < 2) bar_arrive(BAR_P + (i & 1), p_threads);
         }
         for (uint32_t i = 0; i < n; i++) {
-            bar_sync(BAR_Z + (i & 3), ZTHREADS);   // row i's gradient is written
-            if (i + 2 < n) bar_arrive(BAR_P + (i & 1), COMPUTE + BTHREADS);
+            bar_sync(BAR_Z + (i & 3), z_threads);   // row i's gradient is written
+            if (i + 2 < n) bar_arrive(BAR_P + (i & 1), p_threads);
             finish(i);
             if (i + 3 < n) {
                 bar_sync(BAR_B, BTHREADS);
@@ -1497,7 +1520,7 @@ constexpr int SMEM_MAX = 227 * 1024;
 // (twice does no harm).
 struct DeviceInfo {
     std::atomic<int> sms{0};
-    std::atomic<int> clusters[4] = {};   // clusters of 1, 2, 4, 8 CTAs that run at once
+    std::atomic<int> clusters[5] = {};   // clusters of 1, 2, 4, 8, 16 CTAs that run at once
     std::atomic<bool> ready{false};
 };
 
@@ -1518,8 +1541,8 @@ static cudaError_t launch_clusters(uint32_t grid, uint32_t ranks, uint32_t threa
 }
 
 // The current device's entry of kernel K's table, with K allowed all of an
-// SM's shared memory (per device, as kernel attributes are).
-template <auto K> static cudaError_t device_info(DeviceInfo **out) {
+// SM's shared memory (per device, as kernel attributes are) and, if `wide`, clusters of 16.
+template <auto K> static cudaError_t device_info(DeviceInfo **out, bool wide) {
     static DeviceInfo table[MAX_DEVICES];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1532,6 +1555,7 @@ template <auto K> static cudaError_t device_info(DeviceInfo **out) {
         e = cudaFuncGetAttributes(&fa, K);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - (int)fa.sharedSizeBytes);
+        if (e == cudaSuccess && wide) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return e;
         d.sms.store(sms);
@@ -1551,7 +1575,7 @@ static bs_status failed(const char *what, cudaError_t e) {
 // chunks a thread.
 static uint32_t top_ranks(uint32_t rows, uint32_t chunks) {
     uint32_t r = 1;
-    while (r < MAX_CLUSTER && (uint64_t)rows * r < 148 * 4 && chunks / (2 * r) >= 2 * THREADS) r *= 2;
+    while (r < 8 && (uint64_t)rows * r < 148 * 4 && chunks / (2 * r) >= 2 * THREADS) r *= 2;
     return r;
 }
 
@@ -1564,7 +1588,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     constexpr auto K = k_rows<T, OP, CAP>;
     constexpr uint32_t E = 16 / sizeof(T);
     DeviceInfo *dev;
-    cudaError_t e = device_info<K>(&dev);
+    cudaError_t e = device_info<K>(&dev, true);
     if (e != cudaSuccess) return failed("logit_ops", e);
     const uint32_t chunks = A.vocab / E;
     uint32_t ranks = 1, log_ranks = 0, slice = 0;
@@ -1576,7 +1600,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
         room = slots < ROWS_SMEM ? (ROWS_SMEM - slots) / 48 : 0;
         // enough CTAs to hold the row, and to use the GPU where the rows are few
         if (ranks == MAX_CLUSTER ||
-            (slice <= room && !((uint64_t)rows * ranks * 2 <= (uint64_t)dev->sms.load() && slice / 2 >= SLICE_MIN)))
+            (slice <= room && !(ranks < 8 && (uint64_t)rows * ranks * 2 <= (uint64_t)dev->sms.load() && slice / 2 >= SLICE_MIN)))
             break;
     }
     if (slots >= ROWS_SMEM) return BS_ENOTSUP;
@@ -1777,7 +1801,7 @@ static bs_status launch_top(const bs_logits *x, const Scale &sc, float os, uint3
                             float *lse, cudaStream_t st) {
     constexpr auto K = k_top<T, CAP>;
     DeviceInfo *dev;
-    cudaError_t e = device_info<K>(&dev);
+    cudaError_t e = device_info<K>(&dev, false);
     const uint32_t chunks = x->vocab / (16 / sizeof(T)), ranks = top_ranks(x->rows, chunks);
     if ((uint64_t)x->rows * ranks > 0x7FFFFFFFull) return BS_EINVAL;
     const size_t smem = ((size_t)chunks / TOP_TILE + 2) * 4;
