@@ -382,8 +382,8 @@ __device__ __forceinline__ uint32_t remote(const void *p, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void st_remote(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void st_remote4(uint32_t addr, float a, float b, float c) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %1};" ::"r"(addr), "f"(a), "f"(b), "f"(c) : "memory");
 }
 
 // log2 S as exponent + log2 of the mantissa: exact to 2^-24 for any S.
@@ -392,48 +392,6 @@ __device__ __forceinline__ double log2_d(float s) {
     int e;
     float f = frexpf(s, &e);
     return (double)e + (double)log2f(f);
-}
-
-// The sums of all threads of the row's CTAs, in a fixed order, on one scale
-// (with TAIL: s over the rest, u over the teacher's tokens).
-struct RowShared {
-    Stat warp[WARPS];
-    float cta[MAX_CLUSTER][4];
-};
-// RUNS: the caller has made sure that all CTAs of the row run.
-template <bool TAIL, bool RUNS = false>
-__device__ __forceinline__ Stat row_sum(Stat a, float k, RowShared &sh) {
-    const uint32_t tid = threadIdx.x, ranks = cluster_size();
-    auto fold = [&](const Stat &a, const Stat &b) {
-        if (!TAIL) return merge(a, b, k);
-        const float m = fmaxf(a.m, b.m);   // (u is another sum)
-        const float fa = ex2(fmaxf((a.m - m) * k, D_MIN)), fb = ex2(fmaxf((b.m - m) * k, D_MIN));
-        return Stat{m, a.s * fa + b.s * fb, a.u * fa + b.u * fb};
-    };
-    for (int o = 16; o; o >>= 1) {
-        Stat b{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.u, o)};
-        // both lanes of a pair fold in the same order: the same bits
-        a = (tid & o) ? fold(b, a) : fold(a, b);
-    }
-    if ((tid & 31) == 0) sh.warp[tid >> 5] = a;
-    __syncthreads();
-    a = sh.warp[0];
-    for (int i = 1; i < WARPS; i++) a = fold(a, sh.warp[i]);
-    if (ranks > 1) {
-        if (!RUNS) cluster_wait();   // (the arrival is at the kernel's start: every CTA of the row runs)
-        const uint32_t me = cluster_rank();
-        if (tid < ranks) {
-            st_remote(remote(&sh.cta[me][0], tid), a.m);
-            st_remote(remote(&sh.cta[me][1], tid), a.s);
-            st_remote(remote(&sh.cta[me][2], tid), a.u);
-        }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        a = Stat{sh.cta[0][0], sh.cta[0][1], sh.cta[0][2]};
-        for (uint32_t i = 1; i < ranks; i++) a = fold(a, Stat{sh.cta[i][0], sh.cta[i][1], sh.cta[i][2]});
-    }
-    return a;
 }
 
 // The gradient of one row: c'(v_j) p_j (ca + cb log2 p_j), log2 p_j = d_j - log2 S.
@@ -893,6 +851,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                 const float4 f = sh.part[i & 3][lane];
                 st = Stat{f.x, f.y, f.z};
             }
+            if (!grad && !DIST) bar_arrive(BAR_Z + (i & 3), z_threads);   // the sums are read: S may go on
             if (live && edge >= 0) {
                 const bool marked = TAIL && (sh.edge_marks[i & 3] >> lane & 1u);
                 // one logit: 2^0 at itself, nothing where it is -inf (or a sum of NaN)
@@ -952,7 +911,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             if (lane == 0) sh.coef[i & 3] = cf;
             __syncwarp();
             if (grad) bar_arrive(BAR_Y + (i & 3), y_threads);
-            else bar_arrive(BAR_Z + (i & 3), z_threads);
+            else if (DIST) bar_arrive(BAR_Z + (i & 3), z_threads);   // (done with the slots)
         }
     } else if (tid < COMPUTE + 96) {
         // ---- warp C: row i + 3 into row i's buffer
@@ -1207,6 +1166,123 @@ __global__ void __launch_bounds__(1024) k_loss(const float *row_loss, const floa
     }
 }
 
+// ---------------------------------------------------------------------------
+// One pass over the rows without a gradient: log-probability and entropy of
+// the rows' tokens, or (TOP) the rows' lse and the largest logit of each
+// 128-byte tile for k_select.  Bound by HBM reads, so many small CTAs with
+// their loads under way at once; few rows are split over clusters of CTAs.
+constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
+constexpr int TOP_TILE = 8;          // chunks of a tile
+struct StreamShared {
+    Stat warp[WARPS];
+    float4 cta[8];
+};
+template <typename T, bool CAP, bool TOP>
+__global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, float *lse, float *maxima, uint32_t max_ld) {
+    constexpr int E = Row<T>::E;
+    __shared__ __align__(16) StreamShared sh;
+    const uint32_t ranks = 1u << A.log_ranks, rank = ranks > 1 ? cluster_rank() : 0u;
+    const uint32_t row = blockIdx.x >> A.log_ranks, tid = threadIdx.x, lane = tid & 31;
+    const float k = A.sc.k;
+    Row<T> R(A.x, A.ld, row, A.vocab);
+    if (ranks > 1) cluster_arrive();             // (waited for before the first remote store)
+    const int32_t tok = TOP ? 0 : A.tokens[row];
+    if ((uint32_t)tok >= A.vocab) {              // left out: not read
+        if (rank == 0 && tid == 0) {
+            A.logprobs[row] = 0.0f;
+            if (A.entropy) A.entropy[row] = 0.0f;
+            if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
+        }
+        if (ranks > 1) cluster_wait();
+        return;
+    }
+    // slices of whole tiles; rank 0 also has the single elements
+    const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE;
+    const uint32_t per = ((tiles + ranks - 1) >> A.log_ranks) * TOP_TILE;
+    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
+    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
+    const T *body = R.at(0);
+    const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
+    const T v_tok = !TOP && rank == 0 && tid == 0 ? R.x[tok] : from_f<T>(0.0f);
+    float *tile_max = TOP ? maxima + (size_t)row * max_ld : nullptr;
+    Gather<T, CAP, !TOP, false> G;
+
+    // whole batches of the CTA, so that a warp's lanes stay together
+    for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
+        uint4 q[BATCH];
+        if (b + BATCH * THREADS <= c1) {
+#pragma unroll
+            for (int u = 0; u < BATCH; u++) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
+            if (!TOP) {
+                G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+#pragma unroll
+                for (int u = 0; u < BATCH; u++) G.chunk(q[u], A.sc);
+                continue;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < BATCH; u++)
+                if (b + u * THREADS + tid < c1) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
+        }
+        float mx[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            mx[u] = -INFINITY;
+            if (b + u * THREADS + tid < c1) {
+                mx[u] = max_of<T>(q[u]);
+                G.raise(capped<CAP>(mx[u], A.sc), k);
+                G.chunk(q[u], A.sc);
+            }
+        }
+        if (TOP) {
+            // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
+            // the maximum of batch step l & 7 over the group, one tile
+            static_assert(BATCH == 8 && TOP_TILE == 8, "one tile per lane and batch");
+#pragma unroll
+            for (int o = 4; o; o >>= 1) {
+#pragma unroll
+                for (int u = 0; u < o; u++) {
+                    const bool up = lane & o;
+                    const float keep = up ? mx[u + o] : mx[u], give = up ? mx[u] : mx[u + o];
+                    mx[u] = fmaxf(keep, __shfl_xor_sync(~0u, give, o));
+                }
+            }
+            const uint32_t first = b + (lane & 7) * THREADS + (tid & ~7u);   // the tile's first chunk
+            if (first < c1) tile_max[first / TOP_TILE] = mx[0];
+        }
+    }
+    if (edge >= 0) G.one(capped<CAP>(v_edge, A.sc), k, false);
+    if (TOP && rank == 0 && tid < 32) {          // the single elements as one more tile
+        float m = v_edge;
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        if (tid == 0) tile_max[tiles] = m;
+    }
+    Stat st = fold_lanes<false, 32>(G.stat(), k);
+    if (lane == 0) sh.warp[tid >> 5] = st;
+    __syncthreads();
+    if (tid < 32) {
+        st = lane < WARPS ? sh.warp[lane] : Stat{-INFINITY, 0.0f, 0.0f};
+        st = fold_lanes<false, 32>(st, k);
+    }
+    if (ranks > 1) {
+        cluster_wait();
+        if (tid == 0) st_remote4(remote(&sh.cta[rank], 0), st.m, st.s, st.u);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (tid < 32) {
+            const float4 f = lane < ranks ? sh.cta[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            st = fold_lanes<false, 32>(Stat{f.x, f.y, f.z}, k);
+        }
+    }
+    if (rank != 0 || tid != 0) return;
+    if (TOP) {
+        lse[row] = (float)((double)st.m * (double)A.sc.m + LN2_D * log2_d(st.s));
+    } else {
+        token_row<OP_LOGPROB>(A, row, st, TokenIn{1.0f, 0.0f, 0.0f, 0.0f, capped<CAP>(to_f(v_tok), A.sc)}, true);
+    }
+}
+
 // Order of the logits as whole numbers: larger logit, larger key; +0 and -0
 // alike; a NaN below everything (it never wins, as in the argmax).
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -1230,10 +1306,8 @@ __device__ __forceinline__ uint32_t pick_bin(const uint32_t *hist, uint32_t &nee
     return 0u;
 }
 
-constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
 constexpr int TOP_CAND = 2048;       // candidates of a row
 constexpr int TOP_BINS = 2048;
-constexpr int TOP_TILE = 8;          // chunks of a tile: 128 bytes
 struct TopShared {
     unsigned long long cand[TOP_CAND];   // key << 32 | ~id
     uint32_t hist[TOP_BINS];
@@ -1281,77 +1355,24 @@ template <typename T> __device__ __noinline__ void select_whole_row(const T *x, 
     __syncthreads();
 }
 
-// One cluster of CTAs per row.  Each CTA streams its slice once: the row's
-// statistics, and the largest logit of each 128-byte tile, written into CTA
-// 0's shared memory.  CTA 0 then selects: a tile maximum that at least k tiles
-// reach is a floor that all of the k largest logits reach; the few tiles
-// above it are read again (from L2), their logits above the floor sorted.
+// The floor's selection and the sort of one row; one CTA per row.  The tile
+// maxima come from k_stream: a maximum that at least `top` tiles reach is a
+// floor that all of the `top` largest logits reach, so only the few tiles above
+// it are read again and only their logits above it sorted.
 template <typename T, bool CAP>
-__global__ void __launch_bounds__(THREADS) k_top(const void *x, size_t ld, uint32_t vocab, Scale sc, float out_scale,
-                                                 uint32_t top, float *values, int32_t *ids, float *lse) {
+__global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, uint32_t vocab, Scale sc, float out_scale,
+                                                    uint32_t top, const float *maxima, uint32_t max_ld, float *values,
+                                                    int32_t *ids) {
     constexpr int E = Row<T>::E;
-    extern __shared__ float tile_max[];          // CTA 0's: the row's tiles, then the single elements as one more
-    __shared__ RowShared sh;
     __shared__ TopShared ts;
-    const uint32_t ranks = cluster_size(), rank = cluster_rank();
-    const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31;
-    if (ranks > 1) {
-        cluster_arrive();
-        cluster_wait();                          // every CTA of the row runs: its shared memory can be written
-    }
+    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     Row<T> R(x, ld, row, vocab);
     const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE;
-    const uint32_t per = (tiles + ranks - 1) / ranks * TOP_TILE;
-    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
-    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
+    const int32_t edge = tid < 32 ? R.edge(tid) : -1;
     const T *body = R.at(0);
-    const uint32_t dst = remote(tile_max, 0);
-    const float k = sc.k;
+    const float *tile_max = maxima + (size_t)row * max_ld;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // k_stream is done
     const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
-    Gather<T, CAP, false, false> G;
-
-    // whole batches of the CTA, so that a warp's lanes stay together
-    for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
-        uint4 q[BATCH];
-#pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const uint32_t cu = b + u * THREADS + tid;
-            if (cu < c1) q[u] = ld_stream(body + (size_t)cu * E);
-        }
-        float mx[BATCH];
-#pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            mx[u] = -INFINITY;
-            if (b + u * THREADS + tid < c1) {
-                mx[u] = max_of<T>(q[u]);
-                G.raise(capped<CAP>(mx[u], sc), k);
-                G.chunk(q[u], sc);
-            }
-        }
-        // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
-        // the maximum of batch step l & 7 over the group, one tile
-        static_assert(BATCH == 8 && TOP_TILE == 8, "one tile per lane and batch");
-#pragma unroll
-        for (int o = 4; o; o >>= 1) {
-#pragma unroll
-            for (int u = 0; u < o; u++) {
-                const bool up = lane & o;
-                const float keep = up ? mx[u + o] : mx[u], give = up ? mx[u] : mx[u + o];
-                mx[u] = fmaxf(keep, __shfl_xor_sync(~0u, give, o));
-            }
-        }
-        const uint32_t first = b + (lane & 7) * THREADS + (tid & ~7u);   // the tile's first chunk
-        if (first < c1) st_remote(dst + first / TOP_TILE * 4, mx[0]);
-    }
-    float e_max = v_edge;
-    if (tid < 32)
-        for (int o = 16; o; o >>= 1) e_max = fmaxf(e_max, __shfl_xor_sync(~0u, e_max, o));
-    if (rank == 0 && tid == 0) tile_max[tiles] = e_max;
-    if (edge >= 0) G.one(capped<CAP>(v_edge, sc), k, false);
-    // (its barriers also make the tile maxima visible to CTA 0)
-    const Stat st = row_sum<false, true>(G.stat(), k, sh);
-    if (rank != 0) return;
-    if (tid == 0) lse[row] = (float)((double)st.m * (double)sc.m + LN2_D * log2_d(st.s));
 
     // a floor that at least `top` tile maxima reach, by a histogram of their
     // keys below the largest: 2^-10 of an octave a bin, coarser while the
@@ -1541,8 +1562,8 @@ static cudaError_t launch_clusters(uint32_t grid, uint32_t ranks, uint32_t threa
 }
 
 // The current device's entry of kernel K's table, with K allowed all of an
-// SM's shared memory (per device, as kernel attributes are) and, if `wide`, clusters of 16.
-template <auto K> static cudaError_t device_info(DeviceInfo **out, bool wide) {
+// SM's shared memory (per device, as kernel attributes are) and clusters of 16.
+template <auto K> static cudaError_t device_info(DeviceInfo **out) {
     static DeviceInfo table[MAX_DEVICES];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1555,7 +1576,7 @@ template <auto K> static cudaError_t device_info(DeviceInfo **out, bool wide) {
         e = cudaFuncGetAttributes(&fa, K);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - (int)fa.sharedSizeBytes);
-        if (e == cudaSuccess && wide) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return e;
         d.sms.store(sms);
@@ -1571,12 +1592,37 @@ static bs_status failed(const char *what, cudaError_t e) {
     return BS_ECUDA;
 }
 
-// CTAs per row of k_top: few rows still fill the GPU, no CTA has less than two
-// chunks a thread.
-static uint32_t top_ranks(uint32_t rows, uint32_t chunks) {
-    uint32_t r = 1;
-    while (r < 8 && (uint64_t)rows * r < 148 * 4 && chunks / (2 * r) >= 2 * THREADS) r *= 2;
-    return r;
+// CTAs per row of k_stream: few rows still fill the GPU (four to an SM), no CTA
+// has less than two chunks a thread.
+static uint32_t stream_log_ranks(uint32_t rows, uint32_t chunks) {
+    uint32_t l = 0;
+    while (l < 3 && ((uint64_t)rows << l) < 148 * 4 && (chunks >> (l + 1)) >= 2 * THREADS) l++;
+    return l;
+}
+
+template <typename T, bool CAP, bool TOP>
+static bs_status launch_stream(const char *what, RowArgs A, uint32_t rows, float *lse, float *maxima, uint32_t max_ld,
+                               cudaStream_t st) {
+    constexpr auto K = k_stream<T, CAP, TOP>;
+    A.log_ranks = stream_log_ranks(rows, A.vocab / (16 / sizeof(T)));
+    if (((uint64_t)rows << A.log_ranks) > 0x7FFFFFFFull) return BS_EINVAL;
+    cudaError_t e = launch_clusters<K>(rows << A.log_ranks, 1u << A.log_ranks, THREADS, 0, st, A, lse, maxima, max_ld);
+    return e == cudaSuccess ? BS_OK : failed(what, e);
+}
+template <bool TOP>
+static bs_status launch_stream_typed(const char *what, const bs_logits *x, const RowArgs &A, bool cap, float *lse,
+                                     float *maxima, uint32_t max_ld, cudaStream_t st) {
+    switch (x->dtype) {
+        case BS_F32:
+            return cap ? launch_stream<float, true, TOP>(what, A, x->rows, lse, maxima, max_ld, st)
+                       : launch_stream<float, false, TOP>(what, A, x->rows, lse, maxima, max_ld, st);
+        case BS_BF16:
+            return cap ? launch_stream<__nv_bfloat16, true, TOP>(what, A, x->rows, lse, maxima, max_ld, st)
+                       : launch_stream<__nv_bfloat16, false, TOP>(what, A, x->rows, lse, maxima, max_ld, st);
+        default:
+            return cap ? launch_stream<__half, true, TOP>(what, A, x->rows, lse, maxima, max_ld, st)
+                       : launch_stream<__half, false, TOP>(what, A, x->rows, lse, maxima, max_ld, st);
+    }
 }
 
 // Shared memory of k_rows: three buffers of a slice, the teacher's slots.
@@ -1588,7 +1634,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     constexpr auto K = k_rows<T, OP, CAP>;
     constexpr uint32_t E = 16 / sizeof(T);
     DeviceInfo *dev;
-    cudaError_t e = device_info<K>(&dev, true);
+    cudaError_t e = device_info<K>(&dev);
     if (e != cudaSuccess) return failed("logit_ops", e);
     const uint32_t chunks = A.vocab / E;
     uint32_t ranks = 1, log_ranks = 0, slice = 0;
@@ -1682,7 +1728,7 @@ extern "C" bs_status bs_token_logprobs(const bs_logits *x, const int32_t *d_toke
     A.logprobs = d_logprobs;
     A.entropy = d_entropy;
     A.stats = (float2 *)d_stats;
-    return launch_row_typed<OP_LOGPROB>(x, A, cap, (cudaStream_t)stream);
+    return launch_stream_typed<false>("bs_token_logprobs", x, A, cap, nullptr, nullptr, 0, (cudaStream_t)stream);
 }
 
 template <typename T>
@@ -1796,29 +1842,33 @@ extern "C" bs_status bs_distill_loss(const bs_logits *x, const int32_t *d_teache
     return st != BS_OK ? st : total_loss(A, x->rows, d_loss, s);
 }
 
-template <typename T, bool CAP>
-static bs_status launch_top(const bs_logits *x, const Scale &sc, float os, uint32_t k, float *values, int32_t *ids,
-                            float *lse, cudaStream_t st) {
-    constexpr auto K = k_top<T, CAP>;
-    DeviceInfo *dev;
-    cudaError_t e = device_info<K>(&dev, false);
-    const uint32_t chunks = x->vocab / (16 / sizeof(T)), ranks = top_ranks(x->rows, chunks);
-    if ((uint64_t)x->rows * ranks > 0x7FFFFFFFull) return BS_EINVAL;
-    const size_t smem = ((size_t)chunks / TOP_TILE + 2) * 4;
-    if (e == cudaSuccess)
-        e = launch_clusters<K>(x->rows * ranks, ranks, THREADS, smem, st, x->data, x->ld, x->vocab, sc, os, k, values, ids,
-                               lse);
-    return e == cudaSuccess ? BS_OK : failed("bs_top_logits", e);
+// Floats of tile maxima per row: the body's tiles and one more.
+static uint32_t top_tiles(const bs_logits *x) { return x->vocab / (16 / (uint32_t)elem_size(x->dtype)) / TOP_TILE + 2; }
+
+extern "C" size_t bs_top_logits_workspace(const bs_logits *x) {
+    if (!x || x->dtype > BS_F16 || x->vocab > BS_MAX_VOCAB) return 0;
+    return (size_t)x->rows * top_tiles(x) * 4;
 }
-template <typename T>
-static bs_status launch_top(const bs_logits *x, const Scale &sc, float os, bool cap, uint32_t k, float *values,
-                            int32_t *ids, float *lse, cudaStream_t st) {
-    return cap ? launch_top<T, true>(x, sc, os, k, values, ids, lse, st)
-               : launch_top<T, false>(x, sc, os, k, values, ids, lse, st);
+
+template <typename T, bool CAP>
+static bs_status launch_select(const bs_logits *x, const Scale &sc, float os, uint32_t k, const float *maxima, float *values,
+                               int32_t *ids, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(x->rows);
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps k_stream's end
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, k_select<T, CAP>, x->data, x->ld, x->vocab, sc, os, k, maxima, top_tiles(x),
+                                       values, ids);
+    return e == cudaSuccess ? BS_OK : failed("bs_top_logits", e);
 }
 
 extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t *d_ids, float *d_lse,
-                                   void *stream) {
+                                   void *d_work, size_t work_bytes, void *stream) {
     Scale sc;
     float os;
     bool cap;
@@ -1827,11 +1877,21 @@ extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_valu
     if (k == 0 || k > x->vocab) return BS_EINVAL;
     if (k > BS_MAX_TOP) return BS_ENOTSUP;
     if (x->rows == 0) return BS_OK;
-    if (!d_values || !d_ids || !d_lse) return BS_EINVAL;
+    if (!d_values || !d_ids || !d_lse || !d_work || (uintptr_t)d_work % 4 || work_bytes < bs_top_logits_workspace(x))
+        return BS_EINVAL;
     cudaStream_t s = (cudaStream_t)stream;
+    float *maxima = (float *)d_work;
+    st = launch_stream_typed<true>("bs_top_logits", x, row_args(x, sc), cap, d_lse, maxima, top_tiles(x), s);
+    if (st != BS_OK) return st;
     switch (x->dtype) {
-        case BS_F32: return launch_top<float>(x, sc, os, cap, k, d_values, d_ids, d_lse, s);
-        case BS_BF16: return launch_top<__nv_bfloat16>(x, sc, os, cap, k, d_values, d_ids, d_lse, s);
-        default: return launch_top<__half>(x, sc, os, cap, k, d_values, d_ids, d_lse, s);
+        case BS_F32:
+            return cap ? launch_select<float, true>(x, sc, os, k, maxima, d_values, d_ids, s)
+                       : launch_select<float, false>(x, sc, os, k, maxima, d_values, d_ids, s);
+        case BS_BF16:
+            return cap ? launch_select<__nv_bfloat16, true>(x, sc, os, k, maxima, d_values, d_ids, s)
+                       : launch_select<__nv_bfloat16, false>(x, sc, os, k, maxima, d_values, d_ids, s);
+        default:
+            return cap ? launch_select<__half, true>(x, sc, os, k, maxima, d_values, d_ids, s)
+                       : launch_select<__half, false>(x, sc, os, k, maxima, d_values, d_ids, s);
     }
 }

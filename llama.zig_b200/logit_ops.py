@@ -17,7 +17,6 @@ call can be captured in a CUDA graph.  Results are stream-ordered and live on
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import NamedTuple, Optional
 
@@ -91,6 +90,13 @@ def _codes():
     return _dtypes
 
 
+def _raw_stream(index):
+    """The current stream of a device, as a pointer."""
+    import torch
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return fast(index) if fast is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 class _Rows:
     """Checked logits of one call: the descriptor, and where to run."""
 
@@ -114,29 +120,22 @@ class _Rows:
                              logit_scale)
         self._stream = stream
 
-    @contextlib.contextmanager
-    def _switched(self):
-        """The logits' device and the caller's stream made current: results
-        are allocated on the stream that writes them."""
+    def run(self, call):
+        """``call(stream)`` with the logits' device and the caller's stream
+        current: results are allocated on the stream that writes them."""
         import torch
-        s = self._stream
-        if s is None or isinstance(s, torch.cuda.Stream):
-            with torch.cuda.device(self.device), torch.cuda.stream(s):
-                yield (torch.cuda.current_stream() if s is None else s).cuda_stream
-        else:
-            ptr = int(getattr(s, "cuda_stream", s))
-            with torch.cuda.device(self.device):
-                ext = torch.cuda.ExternalStream(ptr, device=self.device) if ptr else torch.cuda.default_stream()
-                with torch.cuda.stream(ext):
-                    yield ptr
-
-    def on(self):
-        """Context whose value is the stream to launch on."""
-        import torch
-        index = self.device.index
-        if self._stream is None and torch.cuda.current_device() == index:
-            return contextlib.nullcontext(torch.cuda.current_stream(index).cuda_stream)
-        return self._switched()
+        s, index = self._stream, self.device.index
+        if s is None:
+            if torch.cuda.current_device() == index:
+                return call(_raw_stream(index))
+            with torch.cuda.device(index):
+                return call(_raw_stream(index))
+        with torch.cuda.device(index):
+            if not isinstance(s, torch.cuda.Stream):
+                ptr = int(getattr(s, "cuda_stream", s))
+                s = torch.cuda.ExternalStream(ptr, device=self.device) if ptr else torch.cuda.default_stream()
+            with torch.cuda.stream(s):
+                return call(s.cuda_stream)
 
     def floats(self, t, what, shape=None):
         """A float32 input on the logits' device, packed."""
@@ -216,13 +215,18 @@ def token_logprobs(logits, tokens, *, temperature: float = 1.0, final_logit_soft
     :func:`token_logprobs_grad` needs.
     """
     r = _Rows(logits, temperature, final_logit_softcapping, logit_scale, stream)
-    with r.on() as st:
+
+    def call(st):
         t = r.ids(tokens, "tokens")
-        lp, ent = r.empty(2, r.rows).unbind()
-        stats = r.empty(r.rows, 2)
-        _s._check(_s.lib().bs_token_logprobs(ctypes.byref(r.desc), t.data_ptr(), lp.data_ptr(), ent.data_ptr(),
-                                             stats.data_ptr(), st), "bs_token_logprobs")
-    return TokenLogprobs(lp, ent, stats)
+        n = r.rows
+        buf = r.empty(4 * n)
+        p = buf.data_ptr()
+        _s._check(_s.lib().bs_token_logprobs(ctypes.byref(r.desc), t.data_ptr(), p, p + 4 * n, p + 8 * n, st),
+                  "bs_token_logprobs")
+        lp, ent, stats = buf.split_with_sizes((n, n, 2 * n))
+        return TokenLogprobs(lp, ent, stats.view(n, 2))
+
+    return r.run(call)
 
 
 def token_logprobs_grad(logits, tokens, fwd: TokenLogprobs, grad_logprobs=None, grad_entropy=None, *,
@@ -234,7 +238,8 @@ def token_logprobs_grad(logits, tokens, fwd: TokenLogprobs, grad_logprobs=None, 
     r = _Rows(logits, temperature, final_logit_softcapping, logit_scale, stream)
     if grad_logprobs is None and grad_entropy is None:
         raise ValueError("neither grad_logprobs nor grad_entropy is given")
-    with r.on() as st:
+
+    def call(st):
         t = r.ids(tokens, "tokens")
         stats, ent = r.floats(fwd.stats, "fwd.stats", (r.rows, 2)), r.floats(fwd.entropy, "fwd.entropy")
         gl = None if grad_logprobs is None else r.floats(grad_logprobs, "grad_logprobs")
@@ -242,7 +247,9 @@ def token_logprobs_grad(logits, tokens, fwd: TokenLogprobs, grad_logprobs=None, 
         g, ld = r.grad_out(out)
         _s._check(_s.lib().bs_token_logprobs_grad(ctypes.byref(r.desc), t.data_ptr(), stats.data_ptr(), ent.data_ptr(),
                                                   _ptr(gl), _ptr(gh), g.data_ptr(), ld, st), "bs_token_logprobs_grad")
-    return _like(logits, g)
+        return _like(logits, g)
+
+    return r.run(call)
 
 
 def top_logits(logits, k: int, *, temperature: float = 1.0, final_logit_softcapping: float = 0.0,
@@ -254,11 +261,17 @@ def top_logits(logits, k: int, *, temperature: float = 1.0, final_logit_softcapp
     if not 1 <= int(k) <= min(r.vocab, MAX_TOP):
         raise ValueError(f"k must be between 1 and the vocabulary (and {MAX_TOP})")
     import torch
-    with r.on() as st:
+
+    def call(st):
         values, ids, lse = r.empty(r.rows, k), r.empty(r.rows, k, dtype=torch.int32), r.empty(r.rows)
-        _s._check(_s.lib().bs_top_logits(ctypes.byref(r.desc), k, values.data_ptr(), ids.data_ptr(), lse.data_ptr(),
-                                         st), "bs_top_logits")
-    return TopLogits(values, ids, lse)
+        L, d = _s.lib(), ctypes.byref(r.desc)
+        size = L.bs_top_logits_workspace(d)
+        work = r.empty(size // 4)
+        _s._check(L.bs_top_logits(d, k, values.data_ptr(), ids.data_ptr(), lse.data_ptr(), work.data_ptr(), size, st),
+                  "bs_top_logits")
+        return TopLogits(values, ids, lse)
+
+    return r.run(call)
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=None, *, temperature: float = 1.0,
@@ -280,7 +293,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
     if teacher_ids.dim() != 2 or not 1 <= teacher_ids.shape[1] <= MAX_TOP:
         raise ValueError(f"teacher_ids must be rows x K with K between 1 and {MAX_TOP}")
     shape = (r.rows, teacher_ids.shape[1])
-    with r.on() as st:
+
+    def call(st):
         ids, tl = r.ids(teacher_ids, "teacher_ids", shape), r.floats(teacher_logits, "teacher_logits", shape)
         lse = None if teacher_lse is None else r.floats(teacher_lse, "teacher_lse")
         w = None if weights is None else r.floats(weights, "weights")
@@ -289,7 +303,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
         _s._check(_s.lib().bs_distill_loss(ctypes.byref(r.desc), ids.data_ptr(), tl.data_ptr(), _ptr(lse), shape[1],
                                            _ptr(w), loss.data_ptr(), rows.data_ptr(), _ptr(g), ld, st),
                   "bs_distill_loss")
-    return DistillLoss(loss, rows, _like(logits, g))
+        return DistillLoss(loss, rows, _like(logits, g))
+
+    return r.run(call)
 
 
 def policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs=None, weights=None, *, clip_low: float = 0.2,
@@ -311,15 +327,20 @@ def policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs=None, wei
     if kl_coef != 0.0 and ref_logprobs is None:
         raise ValueError("kl_coef needs ref_logprobs")
     cfg = BsPolicyConfig(clip_low, clip_high, kl_coef, entropy_coef)
-    with r.on() as st:
+
+    def call(st):
         t = r.ids(tokens, "tokens")
         old, adv = r.floats(old_logprobs, "old_logprobs"), r.floats(advantages, "advantages")
         ref = None if ref_logprobs is None else r.floats(ref_logprobs, "ref_logprobs")
         w = None if weights is None else r.floats(weights, "weights")
         g, ld = r.grad_out(out) if grad else (None, 0)
-        loss = r.empty()
-        rows, lp, ent, kl = r.empty(4, r.rows).unbind()
+        n = r.rows
+        buf = r.empty(4 * n + 1)
+        p = buf.data_ptr()
         _s._check(_s.lib().bs_policy_loss(ctypes.byref(r.desc), t.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref),
-                                          _ptr(w), ctypes.byref(cfg), loss.data_ptr(), rows.data_ptr(), lp.data_ptr(),
-                                          ent.data_ptr(), kl.data_ptr(), _ptr(g), ld, st), "bs_policy_loss")
-    return PolicyLoss(loss, rows, lp, ent, kl, _like(logits, g))
+                                          _ptr(w), ctypes.byref(cfg), p + 16 * n, p, p + 4 * n, p + 8 * n, p + 12 * n,
+                                          _ptr(g), ld, st), "bs_policy_loss")
+        rows, lp, ent, kl, loss = buf.split_with_sizes((n, n, n, n, 1))
+        return PolicyLoss(loss[0], rows, lp, ent, kl, _like(logits, g))
+
+    return r.run(call)

@@ -35,7 +35,8 @@ EXPORTS = [
     "bs_get_rng_state", "bs_set_rng_state", "bs_last_device_status", "bs_destroy",
     "bs_status_string", "bs_profile_enable", "bs_profile_read", "bs_argmax_ex", "bs_set_logit_prologue",
     "bs_sample_static", "bs_seed_state",
-    "bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_distill_loss", "bs_policy_loss",
+    "bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_top_logits_workspace",
+    "bs_distill_loss", "bs_policy_loss",
 ]
 
 
@@ -146,7 +147,9 @@ def lib() -> ctypes.CDLL:
         f32p, sz = vp, ctypes.c_size_t
         L.bs_token_logprobs.argtypes = [vp, vp, f32p, f32p, f32p, vp]
         L.bs_token_logprobs_grad.argtypes = [vp, vp, f32p, f32p, f32p, f32p, vp, sz, vp]
-        L.bs_top_logits.argtypes = [vp, u32, f32p, vp, f32p, vp]
+        L.bs_top_logits.argtypes = [vp, u32, f32p, vp, f32p, vp, sz, vp]
+        L.bs_top_logits_workspace.argtypes = [vp]
+        L.bs_top_logits_workspace.restype = sz
         L.bs_distill_loss.argtypes = [vp, vp, f32p, f32p, u32, f32p, f32p, f32p, vp, sz, vp]
         L.bs_policy_loss.argtypes = [vp, vp, f32p, f32p, f32p, f32p, vp, f32p, f32p, f32p, f32p, f32p, vp, sz, vp]
         for name in ("bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_distill_loss",

@@ -24,7 +24,7 @@ def calls(pkg, d):
     return {
         "logprobs": lambda: L.bs_token_logprobs(d, P, P, P, P, None),
         "grad": lambda: L.bs_token_logprobs_grad(d, P, P, P, P, None, P, 100, None),
-        "top": lambda: L.bs_top_logits(d, 5, P, P, P, None),
+        "top": lambda: L.bs_top_logits(d, 5, P, P, P, P, 1 << 20, None),
         "distill": lambda: L.bs_distill_loss(d, P, P, None, 3, None, P, P, P, 100, None),
         "policy": lambda: L.bs_policy_loss(d, P, P, P, None, None, cfg, P, P, None, None, None, P, 100, None),
     }
@@ -64,10 +64,15 @@ def test_argument_refusals(pkg):
     assert g(d, P, P, P, P, None, None, 100, None) == EINVAL
     assert g(d, P, P, P, P, None, P, 99, None) == EINVAL
     assert g(d, P, P, P, P, None, odd, 100, None) == EINVAL
-    assert L.bs_top_logits(d, 0, P, P, P, None) == EINVAL
-    assert L.bs_top_logits(d, 101, P, P, P, None) == EINVAL
-    assert L.bs_top_logits(desc(pkg, vocab=5000, ld=5000), 1025, P, P, P, None) == ENOTSUP
-    assert L.bs_top_logits(d, 5, None, P, P, None) == EINVAL
+    assert L.bs_top_logits(d, 0, P, P, P, P, 1 << 20, None) == EINVAL
+    assert L.bs_top_logits(d, 101, P, P, P, P, 1 << 20, None) == EINVAL
+    assert L.bs_top_logits(desc(pkg, vocab=5000, ld=5000), 1025, P, P, P, P, 1 << 20, None) == ENOTSUP
+    assert L.bs_top_logits(d, 5, None, P, P, P, 1 << 20, None) == EINVAL
+    need = L.bs_top_logits_workspace(d)
+    assert need > 0
+    assert L.bs_top_logits(d, 5, P, P, P, None, need, None) == EINVAL
+    assert L.bs_top_logits(d, 5, P, P, P, P, need - 1, None) == EINVAL
+    assert L.bs_top_logits(d, 5, P, P, P, ctypes.c_void_p(4098), need, None) == EINVAL
     f = L.bs_distill_loss
     assert f(d, P, P, None, 0, None, P, P, P, 100, None) == EINVAL
     assert f(d, P, P, None, 1025, None, P, P, P, 100, None) == ENOTSUP
@@ -94,7 +99,7 @@ def test_no_rows_need_no_device(pkg):
     L = pkg.lib()
     assert L.bs_token_logprobs(d, None, None, None, None, None) == OK
     assert L.bs_token_logprobs_grad(d, None, None, None, None, None, None, 0, None) == OK
-    assert L.bs_top_logits(d, 5, None, None, None, None) == OK
+    assert L.bs_top_logits(d, 5, None, None, None, None, 0, None) == OK
 
 
 def test_python_refuses_host_tensors(pkg):
