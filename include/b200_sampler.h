@@ -287,7 +287,7 @@ bs_status bs_token_logprobs_grad(const bs_logits *x, const int32_t *d_tokens, co
 /* The k largest logits of each row in falling order, the lowest id first
  * among equals (NaN below everything), as c(v) / logit_scale, with their ids;
  * and the row's lse at the temperature.  k <= BS_MAX_TOP and <= vocab.
- * d_work: scratch of bs_top_logits_workspace(x) bytes (4-byte aligned), this
+ * d_work: scratch of bs_top_logits_workspace(x) bytes (16-byte aligned), this
  * call's alone until the stream has passed it. */
 size_t bs_top_logits_workspace(const bs_logits *x);
 bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t *d_ids, float *d_lse, void *d_work,

@@ -1307,14 +1307,18 @@ __device__ __forceinline__ uint32_t pick_bin(const uint32_t *hist, uint32_t &nee
 }
 
 constexpr int TOP_CAND = 2048;       // candidates of a row
-constexpr int TOP_BINS = 2048;
+constexpr uint32_t TOP_EACH = 40960; // most logits whose keys are searched in shared memory
+constexpr int TOP_MORE = 16;          // candidate tiles that are not worth another step of the search
 struct TopShared {
     unsigned long long cand[TOP_CAND];   // key << 32 | ~id
-    uint32_t hist[TOP_BINS];
-    uint32_t tiles[TOP_CAND];
-    uint32_t warp[WARPS];
+    union {
+        uint16_t tiles[TOP_CAND];
+        uint32_t hist[256];
+    };
+    uint32_t warp[2][WARPS];
     uint32_t bin, need, n, n_tiles;
 };
+static_assert(BS_MAX_VOCAB / (16 / 4) / TOP_TILE + 2 <= 65536, "tile numbers fit 16 bits");
 
 // Selection over the whole row by its keys' digits (four passes over the row
 // in L2; ties are cut by the same selection over the ids): for rows whose
@@ -1355,142 +1359,255 @@ template <typename T> __device__ __noinline__ void select_whole_row(const T *x, 
     __syncthreads();
 }
 
-// The floor's selection and the sort of one row; one CTA per row.  The tile
-// maxima come from k_stream: a maximum that at least `top` tiles reach is a
-// floor that all of the `top` largest logits reach, so only the few tiles above
-// it are read again and only their logits above it sorted.
+// The top logits of one row from its tile maxima (k_stream's); one CTA per
+// row.  A value that at least `top` tile maxima reach is a floor that all of
+// the `top` largest logits reach, so only the few tiles above it are read
+// again (mostly from L2) and only their logits above it sorted.  Latency
+// bound: the search for the floor counts keys in shared memory (a histogram's
+// atomics would meet in a few bins), the tiles' loads are under way together,
+// and the sort is one of 64 elements in a warp's registers and a rank by
+// binary searches in the other warps' runs.  Where there are hardly more tiles
+// than wanted logits (`each`), the logits themselves are searched.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, uint32_t vocab, Scale sc, float out_scale,
-                                                    uint32_t top, const float *maxima, uint32_t max_ld, float *values,
+                                                    uint32_t top, const float *maxima, uint32_t max_ld, bool each, float *values,
                                                     int32_t *ids) {
     constexpr int E = Row<T>::E;
+    extern __shared__ __align__(16) uint32_t keys[];   // of the tile maxima, or (each) of the logits; padded with 0
     __shared__ TopShared ts;
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Row<T> R(x, ld, row, vocab);
-    const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE;
+    const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE, n_max = each ? vocab : tiles + 1;
     const int32_t edge = tid < 32 ? R.edge(tid) : -1;
     const T *body = R.at(0);
     const float *tile_max = maxima + (size_t)row * max_ld;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // k_stream is done
     const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
-
-    // a floor that at least `top` tile maxima reach, by a histogram of their
-    // keys below the largest: 2^-10 of an octave a bin, coarser while the
-    // floor is not among the bins
-    const uint32_t n_max = tiles + 1;
-    uint32_t floor_key = 0;
     if (tid == 0) ts.n = ts.n_tiles = 0;
-    float hi = -INFINITY;
-    for (uint32_t i = tid; i < n_max; i += THREADS) hi = fmaxf(hi, tile_max[i]);
-    for (int o = 16; o; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-    __syncthreads();
-    if (lane == 0) ts.warp[tid >> 5] = order_key(hi);
-    __syncthreads();
-    uint32_t hi_key = ts.warp[0];
-    for (int i = 1; i < WARPS; i++) hi_key = max(hi_key, ts.warp[i]);
-    if (n_max > top) {
-        constexpr int PER = TOP_BINS / THREADS;
-        for (int shift = 13; shift <= 21; shift += 4) {
-            __syncthreads();
-            for (uint32_t i = tid; i < TOP_BINS; i += THREADS) ts.hist[i] = 0;
-            if (tid == 0) ts.bin = TOP_BINS - 1;
-            __syncthreads();
-            for (uint32_t i = tid; i < n_max; i += THREADS)
-                atomicAdd(&ts.hist[min((hi_key - order_key(tile_max[i])) >> shift, TOP_BINS - 1u)], 1u);
-            __syncthreads();
-            uint32_t h[PER], sum = 0;
-#pragma unroll
-            for (int i = 0; i < PER; i++) sum += h[i] = ts.hist[tid * PER + i];
-            uint32_t before = sum;
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t t = __shfl_up_sync(~0u, before, o);
-                if (lane >= (uint32_t)o) before += t;
-            }
-            if (lane == 31) ts.warp[tid >> 5] = before;
-            __syncthreads();
-            before -= sum;
-            for (uint32_t i = 0; i < tid >> 5; i++) before += ts.warp[i];
-            if (before < top && before + sum >= top) {
-                for (int i = 0; i < PER; i++) {
-                    before += h[i];
-                    if (before >= top) {
-                        ts.bin = tid * PER + i;
-                        break;
-                    }
-                }
-            }
-            __syncthreads();
-            const uint32_t bin = ts.bin;
-            if (bin < TOP_BINS - 1) {
-                const uint32_t depth = ((bin + 1) << shift) - 1;
-                floor_key = hi_key > depth ? hi_key - depth : 0u;
-                break;
-            }
-        }
-    }
-    // the tiles that reach it, then their logits that do
-    for (uint32_t i = tid; i < n_max; i += THREADS)
-        if (order_key(tile_max[i]) >= floor_key) {
-            const uint32_t at = atomicAdd(&ts.n_tiles, 1u);
-            if (at < TOP_CAND) ts.tiles[at] = i;
-        }
-    __syncthreads();
-    const uint32_t n_tiles = ts.n_tiles;
-    if (n_tiles <= TOP_CAND) {
-        auto offer = [&](float v, uint32_t id) {
-            const uint32_t key = order_key(v);
-            if (key >= floor_key) {
-                const uint32_t at = atomicAdd(&ts.n, 1u);
-                if (at < TOP_CAND) ts.cand[at] = (unsigned long long)key << 32 | (uint32_t)~id;
-            }
-        };
-        for (uint32_t i = tid >> 3; i < n_tiles; i += THREADS / 8) {
-            const uint32_t t = ts.tiles[i], c = t * TOP_TILE + (tid & 7);
-            if (t < tiles && c < R.chunks) {
-                const uint4 q = ld_stream(body + (size_t)c * E);
-                f2 v[E / 2];
-                unpack<T>(q, v);
-#pragma unroll
-                for (int j = 0; j < E; j += 2) {
-                    float a, b;
-                    halves(v[j / 2], a, b);
-                    offer(a, R.lead + c * E + j);
-                    offer(b, R.lead + c * E + j + 1);
-                }
-            }
-        }
-        if (edge >= 0) offer(v_edge, (uint32_t)edge);
-    }
-    __syncthreads();
-    if (n_tiles > TOP_CAND || ts.n > TOP_CAND || ts.n < top) select_whole_row(R.x, vocab, top, ts);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // k_stream is done
 
-    // sort by (key, lower id): a bitonic network; strides below 64 stay
-    // within a warp's 64 elements
-    const uint32_t n = ts.n;
-    uint32_t size = 64;
-    while (size < n) size <<= 1;
-    for (uint32_t i = n + tid; i < size; i += THREADS) ts.cand[i] = 0ull;
+    const uint32_t quads = (n_max + 3) / 4;
+    uint4 *const key4 = reinterpret_cast<uint4 *>(keys);
+    uint32_t hi_key = 0;
+    if (each) {
+        for (uint32_t i = tid; i < quads * 4; i += 8 * THREADS) {
+            float m[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) m[u] = i + u * THREADS < n_max ? to_f(R.x[i + u * THREADS]) : NAN;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const uint32_t key = order_key(m[u]);
+                hi_key = max(hi_key, key);
+                if (i + u * THREADS < quads * 4) keys[i + u * THREADS] = key;
+            }
+        }
+    } else {
+        for (uint32_t i = tid; i < quads; i += 4 * THREADS) {
+            float4 m[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                m[u] = i + u * THREADS < quads ? __ldcg(reinterpret_cast<const float4 *>(tile_max) + i + u * THREADS)
+                                               : make_float4(NAN, NAN, NAN, NAN);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const uint32_t j = (i + u * THREADS) * 4;   // (behind the last maximum the scratch holds nothing)
+                const uint4 key = make_uint4(order_key(m[u].x), j + 1 < n_max ? order_key(m[u].y) : 0u,
+                                             j + 2 < n_max ? order_key(m[u].z) : 0u, j + 3 < n_max ? order_key(m[u].w) : 0u);
+                hi_key = max(max(max(hi_key, key.x), max(key.y, key.z)), key.w);
+                if (i + u * THREADS < quads) key4[i + u * THREADS] = key;
+            }
+        }
+    }
+    hi_key = __reduce_max_sync(~0u, hi_key);
+    if (lane == 0) ts.warp[0][warp] = hi_key;
     __syncthreads();
-    for (uint32_t run = 2; run <= size; run <<= 1)
-        for (uint32_t stride = run >> 1; stride; stride >>= 1) {
-            for (uint32_t i = tid; i < size / 2; i += THREADS) {
-                const uint32_t lo = 2 * i - (i & (stride - 1)), up = lo + stride;
-                const unsigned long long p = ts.cand[lo], r = ts.cand[up];
-                if ((p < r) == ((lo & run) == 0)) {
-                    ts.cand[lo] = r;
-                    ts.cand[up] = p;
+    for (int i = 0; i < WARPS; i++) hi_key = max(hi_key, ts.warp[0][i]);
+
+    // The largest floor that `top` keys reach, or a little below it: down from
+    // the largest key in steps that grow, then by halves.
+    uint32_t turn = 1;
+    auto reach = [&](uint32_t key) {   // keys of at least `key`
+        uint32_t c = 0;
+        for (uint32_t i = tid; i < quads; i += 4 * THREADS) {
+            uint4 q[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) q[u] = i + u * THREADS < quads ? key4[i + u * THREADS] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 4; u++) c += (q[u].x >= key) + (q[u].y >= key) + (q[u].z >= key) + (q[u].w >= key);
+        }
+        c = __reduce_add_sync(~0u, c);
+        if (lane == 0) ts.warp[turn][warp] = c;
+        __syncthreads();
+        c = 0;
+        for (int i = 0; i < WARPS; i++) c += ts.warp[turn][i];
+        turn ^= 1u;
+        return c;
+    };
+    uint32_t lo = 0, count = n_max;
+    bool exact = false;     // no key between lo and the next larger floor, which too few reach
+    if (n_max > top) {
+        uint32_t hi = hi_key;
+        const uint32_t enough = top + top / 8 + TOP_MORE;
+        for (uint32_t step = 1u << 22;; step = step < 1u << 30 ? step << 2 : ~0u) {
+            lo = hi_key > step ? hi_key - step : 0u;
+            count = reach(lo);
+            if (count >= top) break;
+            hi = lo - 1;                   // (too few reach lo, so lo > 0)
+        }
+        // `top` keys reach lo; the answer is at most hi
+        while (count > enough && lo < hi) {
+            const uint32_t mid = lo + (hi - lo + 1) / 2, c = reach(mid);
+            if (c >= top) lo = mid, count = c;
+            else hi = mid - 1;
+        }
+        exact = count > enough;
+    }
+    // the tiles above the floor, then their logits above it; many tiles that
+    // just reach it are left to the search for ties below
+    const uint32_t floor_key = exact ? lo + 1 : lo;
+    // (one place in the list per warp and round; a lane's own by a prefix sum)
+    auto place = [&](uint32_t *n, uint32_t mine) {
+        uint32_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(~0u, sum, o);
+            if (lane >= (uint32_t)o) sum += t;
+        }
+        uint32_t at = 0;
+        if (lane == 31 && sum) at = atomicAdd(n, sum);
+        return __shfl_sync(~0u, at, 31) + sum - mine;
+    };
+    for (uint32_t i0 = tid - lane; i0 < quads; i0 += 4 * THREADS) {
+        uint4 q[4];
+        uint32_t mine = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const uint32_t i = i0 + lane + u * THREADS;
+            q[u] = i < quads ? key4[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (i * 4 + e < n_max && (&q[u].x)[e] >= floor_key) mine |= 1u << (u * 4 + e);
+        }
+        uint32_t at = place(each ? &ts.n : &ts.n_tiles, __popc(mine));
+#pragma unroll
+        for (int b = 0; b < 16; b++)
+            if (mine >> b & 1u) {
+                const uint32_t i = (i0 + lane + (b / 4) * THREADS) * 4 + b % 4;
+                if (at < TOP_CAND) {
+                    if (each) ts.cand[at] = (unsigned long long)(&q[b / 4].x)[b % 4] << 32 | (uint32_t)~i;
+                    else ts.tiles[at] = (uint16_t)i;
+                }
+                at++;
+            }
+    }
+    __syncthreads();
+    const uint32_t n_tiles = min(ts.n_tiles, (uint32_t)TOP_CAND);   // (fewer than 1024 + 1024 / 8 + TOP_MORE, in fact)
+    constexpr int SOME = 4;
+    for (uint32_t i0 = (tid - lane) >> 3; i0 < n_tiles; i0 += SOME * (THREADS / 8)) {
+        uint4 q[SOME];
+        uint32_t c[SOME], mine = 0;
+#pragma unroll
+        for (int u = 0; u < SOME; u++) {
+            const uint32_t j = i0 + (lane >> 3) + u * (THREADS / 8), t = j < n_tiles ? ts.tiles[j] : tiles;
+            c[u] = t < tiles ? t * TOP_TILE + (lane & 7) : R.chunks;
+            if (c[u] < R.chunks) q[u] = ld_stream(body + (size_t)c[u] * E);
+        }
+#pragma unroll
+        for (int u = 0; u < SOME; u++) {
+            if (c[u] >= R.chunks || order_key(max_of<T>(q[u])) < floor_key) continue;
+            f2 v[E / 2];
+            unpack<T>(q[u], v);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (order_key(e & 1 ? v[e / 2].y : v[e / 2].x) >= floor_key) mine |= 1u << (u * E + e);
+        }
+        uint32_t at = place(&ts.n, __popc(mine));
+        while (mine) {
+            const uint32_t b = __ffs(mine) - 1, u = b / E, e = b % E;
+            mine &= mine - 1;
+            const uint32_t id = R.lead + (u == 0 ? c[0] : u == 1 ? c[1] : u == 2 ? c[2] : c[3]) * E + e;
+            if (at < TOP_CAND) ts.cand[at] = (unsigned long long)order_key(to_f(R.x[id])) << 32 | (uint32_t)~id;
+            at++;
+        }
+    }
+    if (edge >= 0 && !each && order_key(v_edge) >= floor_key) {
+        const uint32_t at = atomicAdd(&ts.n, 1u);
+        if (at < TOP_CAND) ts.cand[at] = (unsigned long long)order_key(v_edge) << 32 | (uint32_t)~edge;
+    }
+    __syncthreads();
+    uint32_t n = ts.n;
+    if (exact && n < top) {
+        // the rest are ties at lo: the lowest ids that have it, in order
+        for (uint32_t j0 = 0; n < top && j0 < vocab; j0 += THREADS) {
+            const uint32_t j = j0 + tid;
+            const bool is = j < vocab && order_key(to_f(R.x[j])) == lo;
+            const uint32_t who = __ballot_sync(~0u, is);
+            if (lane == 0) ts.warp[turn][warp] = __popc(who);
+            __syncthreads();
+            uint32_t at = n + __popc(who & ((1u << lane) - 1u));
+            for (uint32_t i = 0; i < WARPS; i++) {
+                if (i < warp) at += ts.warp[turn][i];
+                n += ts.warp[turn][i];
+            }
+            turn ^= 1u;
+            if (is && at < TOP_CAND) ts.cand[at] = (unsigned long long)lo << 32 | (uint32_t)~j;
+        }
+        n = min(n, (uint32_t)TOP_CAND);
+        __syncthreads();
+    } else if (n > TOP_CAND || n < top) {
+        select_whole_row(R.x, vocab, top, ts);
+        n = top;
+    }
+
+    // sort by (key, lower id): runs of 64 in a warp's registers, two a lane
+    const uint32_t runs = (n + 63) / 64;
+    for (uint32_t i = n + tid; i < runs * 64; i += THREADS) ts.cand[i] = 0ull;
+    __syncthreads();
+    for (uint32_t r = warp; r < runs; r += WARPS) {
+        unsigned long long a = ts.cand[r * 64 + lane], b = ts.cand[r * 64 + 32 + lane];   // elements lane, lane + 32
+#pragma unroll
+        for (uint32_t size = 2; size <= 64; size <<= 1)
+#pragma unroll
+            for (uint32_t stride = size >> 1; stride; stride >>= 1) {
+                if (stride == 32) {
+                    if (a < b) {
+                        const unsigned long long t = a;
+                        a = b;
+                        b = t;
+                    }
+                } else {
+                    const unsigned long long pa = __shfl_xor_sync(~0u, a, stride), pb = __shfl_xor_sync(~0u, b, stride);
+                    const bool low = (lane & stride) == 0;
+                    // falling where (index & size) == 0; for size 32 that parts a from b, for 64 all fall
+                    const bool fa = size >= 32 || (lane & size) == 0, fb = size == 64 || (size < 32 && (lane & size) == 0);
+                    a = (low == fa) == (a > pa) ? a : pa;
+                    b = (low == fb) == (b > pb) ? b : pb;
                 }
             }
-            // the next stage's stride: this run's, or the next run's first
-            const uint32_t next = stride > 1 ? stride >> 1 : run;
-            if (stride > 32 || next > 32) __syncthreads();
-            else __syncwarp();
-        }
+        ts.cand[r * 64 + lane] = a;
+        ts.cand[r * 64 + 32 + lane] = b;
+    }
     __syncthreads();
-    for (uint32_t i = tid; i < top; i += THREADS) {
-        const unsigned long long b = ts.cand[i];
-        values[(size_t)row * top + i] = capped<CAP>(key_value((uint32_t)(b >> 32)), sc) * out_scale;
-        ids[(size_t)row * top + i] = (int32_t)~(uint32_t)b;
+    // an element's rank: its place in its run and, by binary search, the larger elements of the others
+    for (uint32_t i = tid; i < n; i += THREADS) {
+        const unsigned long long c = ts.cand[i];
+        uint32_t rank = i & 63;
+        for (uint32_t r = 0; r < runs; r += 4) {
+            uint32_t m[4] = {};
+#pragma unroll
+            for (uint32_t h = 32; h; h >>= 1)
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (r + u < runs && ts.cand[(r + u) * 64 + m[u] + h - 1] > c) m[u] += h;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (r + u >= runs || r + u == i >> 6) continue;
+                rank += m[u] + (m[u] == 63 && ts.cand[(r + u) * 64 + 63] > c);
+            }
+        }
+        if (rank < top) {
+            values[(size_t)row * top + rank] = capped<CAP>(key_value((uint32_t)(c >> 32)), sc) * out_scale;
+            ids[(size_t)row * top + rank] = (int32_t)~(uint32_t)c;
+        }
     }
 }
 
@@ -1843,7 +1960,10 @@ extern "C" bs_status bs_distill_loss(const bs_logits *x, const int32_t *d_teache
 }
 
 // Floats of tile maxima per row: the body's tiles and one more.
-static uint32_t top_tiles(const bs_logits *x) { return x->vocab / (16 / (uint32_t)elem_size(x->dtype)) / TOP_TILE + 2; }
+// (a multiple of 4: rows of 16-byte loads)
+static uint32_t top_tiles(const bs_logits *x) {
+    return (x->vocab / (16 / (uint32_t)elem_size(x->dtype)) / TOP_TILE + 2 + 3) & ~3u;
+}
 
 extern "C" size_t bs_top_logits_workspace(const bs_logits *x) {
     if (!x || x->dtype > BS_F16 || x->vocab > BS_MAX_VOCAB) return 0;
@@ -1854,16 +1974,23 @@ template <typename T, bool CAP>
 static bs_status launch_select(const bs_logits *x, const Scale &sc, float os, uint32_t k, const float *maxima, float *values,
                                int32_t *ids, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
+    constexpr auto K = k_select<T, CAP>;
+    DeviceInfo *dev;
+    cudaError_t e = device_info<K>(&dev);
+    if (e != cudaSuccess) return failed("bs_top_logits", e);
     cfg.gridDim = dim3(x->rows);
     cfg.blockDim = dim3(THREADS);
+    // the logits themselves where the tiles are few and all keys fit
+    const bool each = x->vocab <= TOP_EACH && top_tiles(x) < k + k / 2;
+    cfg.dynamicSmemBytes = (size_t)(((each ? x->vocab : top_tiles(x)) + 3) & ~3u) * 4;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps k_stream's end
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, k_select<T, CAP>, x->data, x->ld, x->vocab, sc, os, k, maxima, top_tiles(x),
-                                       values, ids);
+    e = cudaLaunchKernelEx(&cfg, K, x->data, x->ld, x->vocab, sc, os, k, maxima, top_tiles(x),
+                           each, values, ids);
     return e == cudaSuccess ? BS_OK : failed("bs_top_logits", e);
 }
 
@@ -1877,7 +2004,7 @@ extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_valu
     if (k == 0 || k > x->vocab) return BS_EINVAL;
     if (k > BS_MAX_TOP) return BS_ENOTSUP;
     if (x->rows == 0) return BS_OK;
-    if (!d_values || !d_ids || !d_lse || !d_work || (uintptr_t)d_work % 4 || work_bytes < bs_top_logits_workspace(x))
+    if (!d_values || !d_ids || !d_lse || !d_work || (uintptr_t)d_work % 16 || work_bytes < bs_top_logits_workspace(x))
         return BS_EINVAL;
     cudaStream_t s = (cudaStream_t)stream;
     float *maxima = (float *)d_work;

@@ -385,6 +385,25 @@ def test_top_logits_ties_and_odd_values(gpu_pkg, dtype, vocab):
     near(lse[:5], want[:5], tol[:5], "lse")
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("vocab", [9000, 50001, 128256])
+def test_top_logits_hard_rows(gpu_pkg, dtype, vocab):
+    g = torch.Generator(device="cuda").manual_seed(55)
+    x = torch.randn(6, vocab, generator=g, device="cuda")
+    x[0, torch.arange(vocab, device="cuda") % 997 != 5] = -math.inf      # fewer tokens left than wanted
+    x[1] = torch.arange(vocab, device="cuda").float() / 64.0             # the largest side by side
+    x[2] = -torch.arange(vocab, device="cuda").float().div(700).floor()  # long runs of equal ones
+    x[3] = -20.0 - x[3].abs() * 1e-3                                     # all below zero, close together
+    x[4, vocab // 2:vocab // 2 + 3000] += 50.0
+    x[5] = x[5] * 1e-30
+    x = x.to(TYPES[dtype])
+    for k in (1, 50, 700, 1024):
+        got = gpu_pkg.top_logits(x, k)
+        ids, vals = top_ref(x, k)
+        assert np.array_equal(got.ids.cpu().numpy(), ids), k
+        assert np.array_equal(got.logits.cpu().numpy(), vals), k
+
+
 def test_masked_logits(gpu_pkg):
     """-inf and the type's lowest value as masks; a row that the mask empties; NaN and +inf."""
     for dtype in TYPES:

@@ -72,7 +72,7 @@ def test_argument_refusals(pkg):
     assert need > 0
     assert L.bs_top_logits(d, 5, P, P, P, None, need, None) == EINVAL
     assert L.bs_top_logits(d, 5, P, P, P, P, need - 1, None) == EINVAL
-    assert L.bs_top_logits(d, 5, P, P, P, ctypes.c_void_p(4098), need, None) == EINVAL
+    assert L.bs_top_logits(d, 5, P, P, P, ctypes.c_void_p(4104), need, None) == EINVAL
     f = L.bs_distill_loss
     assert f(d, P, P, None, 0, None, P, P, P, 100, None) == EINVAL
     assert f(d, P, P, None, 1025, None, P, P, P, 100, None) == ENOTSUP
