@@ -1166,123 +1166,6 @@ __global__ void __launch_bounds__(1024) k_loss(const float *row_loss, const floa
     }
 }
 
-// ---------------------------------------------------------------------------
-// One pass over the rows without a gradient: log-probability and entropy of
-// the rows' tokens, or (TOP) the rows' lse and the largest logit of each
-// 128-byte tile for k_select.  Bound by HBM reads, so many small CTAs with
-// their loads under way at once; few rows are split over clusters of CTAs.
-constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
-constexpr int TOP_TILE = 8;          // chunks of a tile
-struct StreamShared {
-    Stat warp[WARPS];
-    float4 cta[8];
-};
-template <typename T, bool CAP, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, float *lse, float *maxima, uint32_t max_ld) {
-    constexpr int E = Row<T>::E;
-    __shared__ __align__(16) StreamShared sh;
-    const uint32_t ranks = 1u << A.log_ranks, rank = ranks > 1 ? cluster_rank() : 0u;
-    const uint32_t row = blockIdx.x >> A.log_ranks, tid = threadIdx.x, lane = tid & 31;
-    const float k = A.sc.k;
-    Row<T> R(A.x, A.ld, row, A.vocab);
-    if (ranks > 1) cluster_arrive();             // (waited for before the first remote store)
-    const int32_t tok = TOP ? 0 : A.tokens[row];
-    if ((uint32_t)tok >= A.vocab) {              // left out: not read
-        if (rank == 0 && tid == 0) {
-            A.logprobs[row] = 0.0f;
-            if (A.entropy) A.entropy[row] = 0.0f;
-            if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
-        }
-        if (ranks > 1) cluster_wait();
-        return;
-    }
-    // slices of whole tiles; rank 0 also has the single elements
-    const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE;
-    const uint32_t per = ((tiles + ranks - 1) >> A.log_ranks) * TOP_TILE;
-    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
-    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
-    const T *body = R.at(0);
-    const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
-    const T v_tok = !TOP && rank == 0 && tid == 0 ? R.x[tok] : from_f<T>(0.0f);
-    float *tile_max = TOP ? maxima + (size_t)row * max_ld : nullptr;
-    Gather<T, CAP, !TOP, false> G;
-
-    // whole batches of the CTA, so that a warp's lanes stay together
-    for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
-        uint4 q[BATCH];
-        if (b + BATCH * THREADS <= c1) {
-#pragma unroll
-            for (int u = 0; u < BATCH; u++) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
-            if (!TOP) {
-                G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
-#pragma unroll
-                for (int u = 0; u < BATCH; u++) G.chunk(q[u], A.sc);
-                continue;
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < BATCH; u++)
-                if (b + u * THREADS + tid < c1) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
-        }
-        float mx[BATCH];
-#pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            mx[u] = -INFINITY;
-            if (b + u * THREADS + tid < c1) {
-                mx[u] = max_of<T>(q[u]);
-                G.raise(capped<CAP>(mx[u], A.sc), k);
-                G.chunk(q[u], A.sc);
-            }
-        }
-        if (TOP) {
-            // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
-            // the maximum of batch step l & 7 over the group, one tile
-            static_assert(BATCH == 8 && TOP_TILE == 8, "one tile per lane and batch");
-#pragma unroll
-            for (int o = 4; o; o >>= 1) {
-#pragma unroll
-                for (int u = 0; u < o; u++) {
-                    const bool up = lane & o;
-                    const float keep = up ? mx[u + o] : mx[u], give = up ? mx[u] : mx[u + o];
-                    mx[u] = fmaxf(keep, __shfl_xor_sync(~0u, give, o));
-                }
-            }
-            const uint32_t first = b + (lane & 7) * THREADS + (tid & ~7u);   // the tile's first chunk
-            if (first < c1) tile_max[first / TOP_TILE] = mx[0];
-        }
-    }
-    if (edge >= 0) G.one(capped<CAP>(v_edge, A.sc), k, false);
-    if (TOP && rank == 0 && tid < 32) {          // the single elements as one more tile
-        float m = v_edge;
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        if (tid == 0) tile_max[tiles] = m;
-    }
-    Stat st = fold_lanes<false, 32>(G.stat(), k);
-    if (lane == 0) sh.warp[tid >> 5] = st;
-    __syncthreads();
-    if (tid < 32) {
-        st = lane < WARPS ? sh.warp[lane] : Stat{-INFINITY, 0.0f, 0.0f};
-        st = fold_lanes<false, 32>(st, k);
-    }
-    if (ranks > 1) {
-        cluster_wait();
-        if (tid == 0) st_remote4(remote(&sh.cta[rank], 0), st.m, st.s, st.u);
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        if (tid < 32) {
-            const float4 f = lane < ranks ? sh.cta[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-            st = fold_lanes<false, 32>(Stat{f.x, f.y, f.z}, k);
-        }
-    }
-    if (rank != 0 || tid != 0) return;
-    if (TOP) {
-        lse[row] = (float)((double)st.m * (double)A.sc.m + LN2_D * log2_d(st.s));
-    } else {
-        token_row<OP_LOGPROB>(A, row, st, TokenIn{1.0f, 0.0f, 0.0f, 0.0f, capped<CAP>(to_f(v_tok), A.sc)}, true);
-    }
-}
-
 // Order of the logits as whole numbers: larger logit, larger key; +0 and -0
 // alike; a NaN below everything (it never wins, as in the argmax).
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -1306,6 +1189,7 @@ __device__ __forceinline__ uint32_t pick_bin(const uint32_t *hist, uint32_t &nee
     return 0u;
 }
 
+constexpr int TOP_TILE = 8;          // chunks of a tile
 constexpr int TOP_CAND = 2048;       // candidates of a row
 constexpr uint32_t TOP_EACH = 40960; // most logits whose keys are searched in shared memory
 constexpr int TOP_MORE = 16;          // candidate tiles that are not worth another step of the search
@@ -1316,7 +1200,8 @@ struct TopShared {
         uint32_t hist[256];
     };
     uint32_t warp[2][WARPS];
-    uint32_t bin, need, n, n_tiles;
+    uint32_t chunks[TOP_CAND];
+    uint32_t bin, need, n, n_tiles, n_chunks;
 };
 static_assert(BS_MAX_VOCAB / (16 / 4) / TOP_TILE + 2 <= 65536, "tile numbers fit 16 bits");
 
@@ -1359,31 +1244,37 @@ template <typename T> __device__ __noinline__ void select_whole_row(const T *x, 
     __syncthreads();
 }
 
-// The top logits of one row from its tile maxima (k_stream's); one CTA per
-// row.  A value that at least `top` tile maxima reach is a floor that all of
-// the `top` largest logits reach, so only the few tiles above it are read
-// again (mostly from L2) and only their logits above it sorted.  Latency
-// bound: the search for the floor counts keys in shared memory (a histogram's
-// atomics would meet in a few bins), the tiles' loads are under way together,
-// and the sort is one of 64 elements in a warp's registers and a rank by
-// binary searches in the other warps' runs.  Where there are hardly more tiles
-// than wanted logits (`each`), the logits themselves are searched.
+// The top logits of one row from its tile maxima; one CTA.  A value that at
+// least `top` tile maxima reach is a floor that all of the `top` largest
+// logits reach, so only the few tiles above it are read again (mostly from L2)
+// and only their logits above it sorted.  Latency bound: the search for the
+// floor counts keys in shared memory (a histogram's atomics would meet in a
+// few bins), the tiles' loads are under way together, and the sort is one of
+// 64 elements in a warp's registers and a rank by binary searches in the other
+// warps' runs.  Where there are hardly more tiles than wanted logits (`each`),
+// the logits themselves are searched.
+struct TopArgs {
+    uint32_t top;
+    float out_scale;
+    bool each, fused;    // fused: k_stream's CTA 0 of a row selects; else k_select
+    float *values;
+    int32_t *ids;
+    float *lse, *maxima;
+    uint32_t max_ld;
+};
 template <typename T, bool CAP>
-__global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, uint32_t vocab, Scale sc, float out_scale,
-                                                    uint32_t top, const float *maxima, uint32_t max_ld, bool each, float *values,
-                                                    int32_t *ids) {
+__device__ __forceinline__ void select_top(const Row<T> &R, uint32_t row, const Scale &sc, const TopArgs &P, TopShared &ts,
+                                           uint32_t *keys) {   // keys: of the tile maxima, or (each) of the logits; padded with 0
     constexpr int E = Row<T>::E;
-    extern __shared__ __align__(16) uint32_t keys[];   // of the tile maxima, or (each) of the logits; padded with 0
-    __shared__ TopShared ts;
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    Row<T> R(x, ld, row, vocab);
+    const uint32_t top = P.top, vocab = R.vocab;
+    const bool each = P.each;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE, n_max = each ? vocab : tiles + 1;
     const int32_t edge = tid < 32 ? R.edge(tid) : -1;
     const T *body = R.at(0);
-    const float *tile_max = maxima + (size_t)row * max_ld;
+    const float *tile_max = P.maxima + (size_t)row * P.max_ld;
     const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
-    if (tid == 0) ts.n = ts.n_tiles = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // k_stream is done
+    if (tid == 0) ts.n = ts.n_tiles = ts.n_chunks = 0;
 
     const uint32_t quads = (n_max + 3) / 4;
     uint4 *const key4 = reinterpret_cast<uint4 *>(keys);
@@ -1501,7 +1392,8 @@ __global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, ui
     }
     __syncthreads();
     const uint32_t n_tiles = min(ts.n_tiles, (uint32_t)TOP_CAND);   // (fewer than 1024 + 1024 / 8 + TOP_MORE, in fact)
-    constexpr int SOME = 4;
+    // first the chunks of these tiles that hold one (about one a tile), then those chunks' logits
+    constexpr int SOME = 8;
     for (uint32_t i0 = (tid - lane) >> 3; i0 < n_tiles; i0 += SOME * (THREADS / 8)) {
         uint4 q[SOME];
         uint32_t c[SOME], mine = 0;
@@ -1512,22 +1404,37 @@ __global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, ui
             if (c[u] < R.chunks) q[u] = ld_stream(body + (size_t)c[u] * E);
         }
 #pragma unroll
-        for (int u = 0; u < SOME; u++) {
-            if (c[u] >= R.chunks || order_key(max_of<T>(q[u])) < floor_key) continue;
-            f2 v[E / 2];
-            unpack<T>(q[u], v);
+        for (int u = 0; u < SOME; u++)
+            if (c[u] < R.chunks && order_key(max_of<T>(q[u])) >= floor_key) mine |= 1u << u;
+        uint32_t at = place(&ts.n_chunks, __popc(mine));
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                if (order_key(e & 1 ? v[e / 2].y : v[e / 2].x) >= floor_key) mine |= 1u << (u * E + e);
+        for (int u = 0; u < SOME; u++)
+            if (mine >> u & 1u) {
+                if (at < TOP_CAND) ts.chunks[at] = c[u];
+                at++;
+            }
+    }
+    __syncthreads();
+    const uint32_t n_chunks = min(ts.n_chunks, (uint32_t)TOP_CAND);
+    for (uint32_t i0 = tid - lane; i0 < n_chunks; i0 += THREADS) {
+        const uint32_t c = i0 + lane < n_chunks ? ts.chunks[i0 + lane] : R.chunks;
+        uint32_t key[E], mine = 0;
+        if (c < R.chunks) {
+            f2 v[E / 2];
+            unpack<T>(*reinterpret_cast<const uint4 *>(body + (size_t)c * E), v);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                key[e] = order_key(e & 1 ? v[e / 2].y : v[e / 2].x);
+                if (key[e] >= floor_key) mine |= 1u << e;
+            }
         }
         uint32_t at = place(&ts.n, __popc(mine));
-        while (mine) {
-            const uint32_t b = __ffs(mine) - 1, u = b / E, e = b % E;
-            mine &= mine - 1;
-            const uint32_t id = R.lead + (u == 0 ? c[0] : u == 1 ? c[1] : u == 2 ? c[2] : c[3]) * E + e;
-            if (at < TOP_CAND) ts.cand[at] = (unsigned long long)order_key(to_f(R.x[id])) << 32 | (uint32_t)~id;
-            at++;
-        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (mine >> e & 1u) {
+                if (at < TOP_CAND) ts.cand[at] = (unsigned long long)key[e] << 32 | (uint32_t)~(R.lead + c * E + e);
+                at++;
+            }
     }
     if (edge >= 0 && !each && order_key(v_edge) >= floor_key) {
         const uint32_t at = atomicAdd(&ts.n, 1u);
@@ -1535,6 +1442,7 @@ __global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, ui
     }
     __syncthreads();
     uint32_t n = ts.n;
+    if (ts.n_chunks > TOP_CAND) n = TOP_CAND + 1;   // (too many: as with too many logits)
     if (exact && n < top) {
         // the rest are ties at lo: the lowest ids that have it, in order
         for (uint32_t j0 = 0; n < top && j0 < vocab; j0 += THREADS) {
@@ -1605,10 +1513,138 @@ __global__ void __launch_bounds__(THREADS) k_select(const void *x, size_t ld, ui
             }
         }
         if (rank < top) {
-            values[(size_t)row * top + rank] = capped<CAP>(key_value((uint32_t)(c >> 32)), sc) * out_scale;
-            ids[(size_t)row * top + rank] = (int32_t)~(uint32_t)c;
+            P.values[(size_t)row * top + rank] = capped<CAP>(key_value((uint32_t)(c >> 32)), sc) * P.out_scale;
+            P.ids[(size_t)row * top + rank] = (int32_t)~(uint32_t)c;
         }
     }
+}
+
+// ---------------------------------------------------------------------------
+// One pass over the rows without a gradient: log-probability and entropy of
+// the rows' tokens, or (TOP) the rows' lse and the largest logit of each
+// 128-byte tile, from which CTA 0 of the row then selects.  Bound by HBM reads, so many small CTAs with
+// their loads under way at once; few rows are split over clusters of CTAs.
+constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
+struct StreamShared {
+    Stat warp[WARPS];
+    float4 cta[8];
+};
+template <typename T, bool CAP, bool TOP>
+__global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
+    constexpr int E = Row<T>::E;
+    extern __shared__ __align__(16) uint32_t keys[];
+    __shared__ __align__(16) StreamShared sh;
+    const uint32_t ranks = 1u << A.log_ranks, rank = ranks > 1 ? cluster_rank() : 0u;
+    const uint32_t row = blockIdx.x >> A.log_ranks, tid = threadIdx.x, lane = tid & 31;
+    const float k = A.sc.k;
+    Row<T> R(A.x, A.ld, row, A.vocab);
+    if (ranks > 1) cluster_arrive();             // (waited for before the first remote store)
+    const int32_t tok = TOP ? 0 : A.tokens[row];
+    if ((uint32_t)tok >= A.vocab) {              // left out: not read
+        if (rank == 0 && tid == 0) {
+            A.logprobs[row] = 0.0f;
+            if (A.entropy) A.entropy[row] = 0.0f;
+            if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
+        }
+        if (ranks > 1) cluster_wait();
+        return;
+    }
+    // slices of whole tiles; rank 0 also has the single elements
+    const uint32_t tiles = (R.chunks + TOP_TILE - 1) / TOP_TILE;
+    const uint32_t per = ((tiles + ranks - 1) >> A.log_ranks) * TOP_TILE;
+    const uint32_t c0 = min(rank * per, R.chunks), c1 = min(c0 + per, R.chunks);
+    const int32_t edge = rank == 0 && tid < 32 ? R.edge(tid) : -1;
+    const T *body = R.at(0);
+    const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
+    const T v_tok = !TOP && rank == 0 && tid == 0 ? R.x[tok] : from_f<T>(0.0f);
+    float *tile_max = TOP ? P.maxima + (size_t)row * P.max_ld : nullptr;
+    Gather<T, CAP, !TOP, false> G;
+
+    // whole batches of the CTA, so that a warp's lanes stay together
+    for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
+        uint4 q[BATCH];
+        if (b + BATCH * THREADS <= c1) {
+#pragma unroll
+            for (int u = 0; u < BATCH; u++) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
+            if (!TOP) {
+                G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+#pragma unroll
+                for (int u = 0; u < BATCH; u++) G.chunk(q[u], A.sc);
+                continue;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < BATCH; u++)
+                if (b + u * THREADS + tid < c1) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
+        }
+        float mx[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            mx[u] = -INFINITY;
+            if (b + u * THREADS + tid < c1) {
+                mx[u] = max_of<T>(q[u]);
+                G.raise(capped<CAP>(mx[u], A.sc), k);
+                G.chunk(q[u], A.sc);
+            }
+        }
+        if (TOP) {
+            // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
+            // the maximum of batch step l & 7 over the group, one tile
+            static_assert(BATCH == 8 && TOP_TILE == 8, "one tile per lane and batch");
+#pragma unroll
+            for (int o = 4; o; o >>= 1) {
+#pragma unroll
+                for (int u = 0; u < o; u++) {
+                    const bool up = lane & o;
+                    const float keep = up ? mx[u + o] : mx[u], give = up ? mx[u] : mx[u + o];
+                    mx[u] = fmaxf(keep, __shfl_xor_sync(~0u, give, o));
+                }
+            }
+            const uint32_t first = b + (lane & 7) * THREADS + (tid & ~7u);   // the tile's first chunk
+            if (first < c1) tile_max[first / TOP_TILE] = mx[0];
+        }
+    }
+    if (edge >= 0) G.one(capped<CAP>(v_edge, A.sc), k, false);
+    if (TOP && rank == 0 && tid < 32) {          // the single elements as one more tile
+        float m = v_edge;
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        if (tid == 0) tile_max[tiles] = m;
+    }
+    Stat st = fold_lanes<false, 32>(G.stat(), k);
+    if (lane == 0) sh.warp[tid >> 5] = st;
+    __syncthreads();
+    if (tid < 32) {
+        st = lane < WARPS ? sh.warp[lane] : Stat{-INFINITY, 0.0f, 0.0f};
+        st = fold_lanes<false, 32>(st, k);
+    }
+    if (ranks > 1) {
+        cluster_wait();
+        if (tid == 0) st_remote4(remote(&sh.cta[rank], 0), st.m, st.s, st.u);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (tid < 32) {
+            const float4 f = lane < ranks ? sh.cta[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            st = fold_lanes<false, 32>(Stat{f.x, f.y, f.z}, k);
+        }
+    }
+    if (rank != 0) return;
+    if constexpr (TOP) {
+        // (the barriers above also made the tile maxima of all CTAs visible to this one)
+        __shared__ TopShared ts;
+        if (tid == 0) P.lse[row] = (float)((double)st.m * (double)A.sc.m + LN2_D * log2_d(st.s));
+        if (P.fused) select_top<T, CAP>(R, row, A.sc, P, ts, keys);
+    } else if (tid == 0) {
+        token_row<OP_LOGPROB>(A, row, st, TokenIn{1.0f, 0.0f, 0.0f, 0.0f, capped<CAP>(to_f(v_tok), A.sc)}, true);
+    }
+}
+
+template <typename T, bool CAP> __global__ void __launch_bounds__(THREADS) k_select(RowArgs A, TopArgs P) {
+    extern __shared__ __align__(16) uint32_t keys[];
+    __shared__ TopShared ts;
+    const Row<T> R(A.x, A.ld, blockIdx.x, A.vocab);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // k_stream is done
+    select_top<T, CAP>(R, blockIdx.x, A.sc, P, ts, keys);
 }
 
 // ---------------------------------------------------------------------------
@@ -1679,8 +1715,9 @@ static cudaError_t launch_clusters(uint32_t grid, uint32_t ranks, uint32_t threa
 }
 
 // The current device's entry of kernel K's table, with K allowed all of an
-// SM's shared memory (per device, as kernel attributes are) and clusters of 16.
-template <auto K> static cudaError_t device_info(DeviceInfo **out) {
+// SM's shared memory (per device, as kernel attributes are) and, if `wide`,
+// clusters of 16.
+template <auto K> static cudaError_t device_info(DeviceInfo **out, bool wide) {
     static DeviceInfo table[MAX_DEVICES];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1693,7 +1730,7 @@ template <auto K> static cudaError_t device_info(DeviceInfo **out) {
         e = cudaFuncGetAttributes(&fa, K);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX - (int)fa.sharedSizeBytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess && wide) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return e;
         d.sms.store(sms);
@@ -1709,36 +1746,71 @@ static bs_status failed(const char *what, cudaError_t e) {
     return BS_ECUDA;
 }
 
+constexpr uint32_t STREAM_CTAS = 148 * 4;   // of k_stream that run at once
+
 // CTAs per row of k_stream: few rows still fill the GPU (four to an SM), no CTA
 // has less than two chunks a thread.
 static uint32_t stream_log_ranks(uint32_t rows, uint32_t chunks) {
     uint32_t l = 0;
-    while (l < 3 && ((uint64_t)rows << l) < 148 * 4 && (chunks >> (l + 1)) >= 2 * THREADS) l++;
+    while (l < 3 && ((uint64_t)rows << l) < STREAM_CTAS && (chunks >> (l + 1)) >= 2 * THREADS) l++;
     return l;
 }
 
+// Whether k_stream itself selects.  With many rows (one CTA each) that overlaps
+// other rows' streaming, with few it saves a launch; in between all rows would
+// select at the kernel's end, several to an SM.  Measured, separate against
+// fused: 8 x 128256 f32 16.3 and 14.5 us, 256 rows 37.9 and 44.6, 2048 rows
+// 217 and 210; 512 x 32000 bf16 24.7 and 30.9, 4096 rows 115 and 111.
+static bool top_fused(uint32_t rows) { return rows < 64 || rows >= STREAM_CTAS; }
+
 template <typename T, bool CAP, bool TOP>
-static bs_status launch_stream(const char *what, RowArgs A, uint32_t rows, float *lse, float *maxima, uint32_t max_ld,
-                               cudaStream_t st) {
+static bs_status launch_stream(const char *what, RowArgs A, uint32_t rows, TopArgs P, cudaStream_t st) {
     constexpr auto K = k_stream<T, CAP, TOP>;
+    DeviceInfo *dev;
+    cudaError_t e = device_info<K>(&dev, false);
+    size_t smem = 0;
     A.log_ranks = stream_log_ranks(rows, A.vocab / (16 / sizeof(T)));
+    if (TOP) {
+        // the logits themselves where the tiles are few and all keys fit
+        P.each = A.vocab <= TOP_EACH && P.max_ld < P.top + P.top / 2;
+        P.fused = top_fused(rows);
+        smem = (size_t)(((P.each ? A.vocab : P.max_ld) + 3) & ~3u) * 4;
+    }
     if (((uint64_t)rows << A.log_ranks) > 0x7FFFFFFFull) return BS_EINVAL;
-    cudaError_t e = launch_clusters<K>(rows << A.log_ranks, 1u << A.log_ranks, THREADS, 0, st, A, lse, maxima, max_ld);
+    if (e == cudaSuccess)
+        e = launch_clusters<K>(rows << A.log_ranks, 1u << A.log_ranks, THREADS, P.fused ? smem : 0, st, A, P);
+    if constexpr (TOP) {
+        constexpr auto S = k_select<T, CAP>;
+        if (e == cudaSuccess && !P.fused) e = device_info<S>(&dev, false);
+        if (e == cudaSuccess && !P.fused) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(rows);
+            cfg.blockDim = dim3(THREADS);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream = st;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps k_stream's end
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            e = cudaLaunchKernelEx(&cfg, S, A, P);
+        }
+    }
     return e == cudaSuccess ? BS_OK : failed(what, e);
 }
 template <bool TOP>
-static bs_status launch_stream_typed(const char *what, const bs_logits *x, const RowArgs &A, bool cap, float *lse,
-                                     float *maxima, uint32_t max_ld, cudaStream_t st) {
+static bs_status launch_stream_typed(const char *what, const bs_logits *x, const RowArgs &A, bool cap, const TopArgs &P,
+                                     cudaStream_t st) {
     switch (x->dtype) {
         case BS_F32:
-            return cap ? launch_stream<float, true, TOP>(what, A, x->rows, lse, maxima, max_ld, st)
-                       : launch_stream<float, false, TOP>(what, A, x->rows, lse, maxima, max_ld, st);
+            return cap ? launch_stream<float, true, TOP>(what, A, x->rows, P, st)
+                       : launch_stream<float, false, TOP>(what, A, x->rows, P, st);
         case BS_BF16:
-            return cap ? launch_stream<__nv_bfloat16, true, TOP>(what, A, x->rows, lse, maxima, max_ld, st)
-                       : launch_stream<__nv_bfloat16, false, TOP>(what, A, x->rows, lse, maxima, max_ld, st);
+            return cap ? launch_stream<__nv_bfloat16, true, TOP>(what, A, x->rows, P, st)
+                       : launch_stream<__nv_bfloat16, false, TOP>(what, A, x->rows, P, st);
         default:
-            return cap ? launch_stream<__half, true, TOP>(what, A, x->rows, lse, maxima, max_ld, st)
-                       : launch_stream<__half, false, TOP>(what, A, x->rows, lse, maxima, max_ld, st);
+            return cap ? launch_stream<__half, true, TOP>(what, A, x->rows, P, st)
+                       : launch_stream<__half, false, TOP>(what, A, x->rows, P, st);
     }
 }
 
@@ -1751,7 +1823,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     constexpr auto K = k_rows<T, OP, CAP>;
     constexpr uint32_t E = 16 / sizeof(T);
     DeviceInfo *dev;
-    cudaError_t e = device_info<K>(&dev);
+    cudaError_t e = device_info<K>(&dev, true);
     if (e != cudaSuccess) return failed("logit_ops", e);
     const uint32_t chunks = A.vocab / E;
     uint32_t ranks = 1, log_ranks = 0, slice = 0;
@@ -1845,7 +1917,7 @@ extern "C" bs_status bs_token_logprobs(const bs_logits *x, const int32_t *d_toke
     A.logprobs = d_logprobs;
     A.entropy = d_entropy;
     A.stats = (float2 *)d_stats;
-    return launch_stream_typed<false>("bs_token_logprobs", x, A, cap, nullptr, nullptr, 0, (cudaStream_t)stream);
+    return launch_stream_typed<false>("bs_token_logprobs", x, A, cap, TopArgs{}, (cudaStream_t)stream);
 }
 
 template <typename T>
@@ -1970,30 +2042,6 @@ extern "C" size_t bs_top_logits_workspace(const bs_logits *x) {
     return (size_t)x->rows * top_tiles(x) * 4;
 }
 
-template <typename T, bool CAP>
-static bs_status launch_select(const bs_logits *x, const Scale &sc, float os, uint32_t k, const float *maxima, float *values,
-                               int32_t *ids, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    constexpr auto K = k_select<T, CAP>;
-    DeviceInfo *dev;
-    cudaError_t e = device_info<K>(&dev);
-    if (e != cudaSuccess) return failed("bs_top_logits", e);
-    cfg.gridDim = dim3(x->rows);
-    cfg.blockDim = dim3(THREADS);
-    // the logits themselves where the tiles are few and all keys fit
-    const bool each = x->vocab <= TOP_EACH && top_tiles(x) < k + k / 2;
-    cfg.dynamicSmemBytes = (size_t)(((each ? x->vocab : top_tiles(x)) + 3) & ~3u) * 4;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps k_stream's end
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, K, x->data, x->ld, x->vocab, sc, os, k, maxima, top_tiles(x),
-                           each, values, ids);
-    return e == cudaSuccess ? BS_OK : failed("bs_top_logits", e);
-}
-
 extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t *d_ids, float *d_lse,
                                    void *d_work, size_t work_bytes, void *stream) {
     Scale sc;
@@ -2006,19 +2054,6 @@ extern "C" bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_valu
     if (x->rows == 0) return BS_OK;
     if (!d_values || !d_ids || !d_lse || !d_work || (uintptr_t)d_work % 16 || work_bytes < bs_top_logits_workspace(x))
         return BS_EINVAL;
-    cudaStream_t s = (cudaStream_t)stream;
-    float *maxima = (float *)d_work;
-    st = launch_stream_typed<true>("bs_top_logits", x, row_args(x, sc), cap, d_lse, maxima, top_tiles(x), s);
-    if (st != BS_OK) return st;
-    switch (x->dtype) {
-        case BS_F32:
-            return cap ? launch_select<float, true>(x, sc, os, k, maxima, d_values, d_ids, s)
-                       : launch_select<float, false>(x, sc, os, k, maxima, d_values, d_ids, s);
-        case BS_BF16:
-            return cap ? launch_select<__nv_bfloat16, true>(x, sc, os, k, maxima, d_values, d_ids, s)
-                       : launch_select<__nv_bfloat16, false>(x, sc, os, k, maxima, d_values, d_ids, s);
-        default:
-            return cap ? launch_select<__half, true>(x, sc, os, k, maxima, d_values, d_ids, s)
-                       : launch_select<__half, false>(x, sc, os, k, maxima, d_values, d_ids, s);
-    }
+    const TopArgs P{k, os, false, false, d_values, d_ids, d_lse, (float *)d_work, top_tiles(x)};
+    return launch_stream_typed<true>("bs_top_logits", x, row_args(x, sc), cap, P, (cudaStream_t)stream);
 }
