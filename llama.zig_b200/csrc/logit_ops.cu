@@ -50,7 +50,7 @@ struct RowArgs {
     uint32_t vocab;
     uint32_t keep;              // 16-byte chunks of a CTA's slice that stay in shared memory
     uint32_t log_ranks;         // CTAs of a row
-    uint32_t bit_words;         // teacher's tail: words of one bit per element of a slice
+    uint32_t bit_words;         // with a teacher: words of one bit per element of a slice
     Scale sc;
     const int32_t *tokens;
     // outputs (null where not asked for)
@@ -401,14 +401,15 @@ template <bool ENT> struct GradRow {
         const float l = fmaf(c - m, k, -l2s), p = ex2(l);
         return ENT ? p * fmaf(cb, max_nan(l, D_MIN), ca) : p * ca;
     }
-    // a chunk of it
-    template <typename T, bool CAP> __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
+    // a chunk of it (DONE: q holds c(v) already)
+    template <typename T, bool CAP, bool DONE = false>
+    __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
         constexpr int N = 8 / sizeof(T);
         f2 v[N], o[N];
         unpack<T>(q, v);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            v[i] = capped2<CAP>(v[i], sc);
+            if (!DONE) v[i] = capped2<CAP>(v[i], sc);
             const f2 l = fma2(add2(v[i], both(-m)), both(k), both(-l2s));
             o[i] = mul2(ex2_2(l), ENT ? fma2(both(cb), floor2(l), both(ca)) : both(ca));
         }
@@ -450,10 +451,9 @@ template <bool ENT> struct GradRow {
 // travel.  Barriers, in as many copies as rows can be between the two sides:
 // X (S -> A: row i summed), Y (A -> G: its coefficients), P (B -> S: its
 // slots), Z (-> C, B: done with; from G, or without a gradient from S and A).
-constexpr int COMPUTE = 512;
 constexpr uint32_t COPY = 512;       // chunks of one copy
 constexpr int STEP = 4;              // chunks of a thread summed at a time
-constexpr int CWARPS = COMPUTE / 32;
+constexpr int MAX_CWARPS = 24;       // most warps S and G together
 constexpr int BTHREADS = 128;
 enum Bar { BAR_X = 1, BAR_Y = 5, BAR_Z = 9, BAR_P = 13, BAR_B = 15 };
 __device__ __forceinline__ void bar_sync(int id, int threads) {
@@ -471,7 +471,7 @@ __device__ __forceinline__ void copy_bulk(void *dst, const void *src, uint32_t b
 
 __host__ __device__ constexpr bool is_distill(int op) { return op == OP_DISTILL || op == OP_DISTILL_TAIL; }
 __host__ __device__ constexpr bool is_policy(int op) { return op == OP_POLICY || op == OP_POLICY_ENT; }
-__host__ __device__ constexpr int row_threads(int op) { return COMPUTE + 96 + (is_distill(op) ? BTHREADS : 0); }
+__host__ __device__ constexpr int row_threads(int op, int compute) { return compute + 96 + (is_distill(op) ? BTHREADS : 0); }
 
 // Row i's results as the gradient needs them.
 struct Coef {
@@ -481,15 +481,22 @@ struct Coef {
     float c_tok;         // the token's c(v)
     uint32_t live;       // 0: the row is left out
 };
+// Threads of S and G, and of S alone where there is a gradient to write.  The
+// 16-bit types have twice the logits a byte and want more of both; f32 under a
+// soft-cap leaves most of the work to S (see LEAVE).
+template <typename T> __host__ __device__ constexpr int compute_threads() { return sizeof(T) == 4 ? 512 : 640; }
+template <typename T, bool CAP> __host__ __device__ constexpr int sum_threads_of() {
+    return CAP && sizeof(T) == 4 ? 384 : compute_threads<T>() / 2;
+}
 struct RowsShared {
-    float4 part[4][CWARPS];          // (m, s, u) of the warps S
+    float4 part[4][MAX_CWARPS];          // (m, s, u) of the warps S
     float4 mail[2][MAX_CLUSTER];     // and of the row's CTAs
     Coef coef[4];
     int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
     // B's
     double scratch_d[BTHREADS / 32];
     float scratch_f[BTHREADS / 32];
-    uint32_t slots_live[4], edge_marks[4];
+    uint32_t slots_live[4], edge_marks[4], twice[4];   // twice: an id of the slice comes twice
     uint64_t mail_bar[2], full_bar[3];
 };
 
@@ -589,7 +596,7 @@ struct Slots {
     int32_t *id;      // -1: empty; padded to a multiple of 4 with empty ones
     float *q;         // the slot's share
     float *c;         // the student's c(v) there
-    uint32_t *bits;   // tail: one bit per element of the CTA's slice
+    uint32_t *bits;   // one bit per element of the CTA's slice: named by the teacher
 };
 __host__ __device__ __forceinline__ uint32_t slots_padded(uint32_t n_ids) { return (n_ids + 3u) & ~3u; }
 
@@ -628,8 +635,9 @@ __device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, cons
 }
 
 template <typename T, int OP, bool CAP>
-__global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t rows, uint32_t clusters) {
+__global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_rows(RowArgs A, uint32_t rows, uint32_t clusters) {
     constexpr bool DIST = is_distill(OP), TAIL = OP == OP_DISTILL_TAIL;
+    constexpr uint32_t COMPUTE = compute_threads<T>();
     constexpr int E = Row<T>::E;
     extern __shared__ uint4 dyn[];
     __shared__ __align__(16) RowsShared sh;
@@ -639,9 +647,12 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
     const float k = A.sc.k;
     const bool grad = A.grad != nullptr;
     // threads of S and G, and of the barriers
-    const uint32_t sum_threads = grad ? COMPUTE / 2 : COMPUTE, x_threads = sum_threads + 32;
-    const uint32_t y_threads = COMPUTE / 2 + 32, p_threads = sum_threads + BTHREADS;
-    const uint32_t z_threads = (grad ? COMPUTE / 2 : COMPUTE + 32) + 32 + (DIST ? BTHREADS : 0);
+    constexpr uint32_t ST = sum_threads_of<T, CAP>(), GT = COMPUTE - ST;
+    const uint32_t sum_threads = grad ? ST : COMPUTE, x_threads = sum_threads + 32;
+    const uint32_t y_threads = GT + 32, p_threads = sum_threads + BTHREADS;
+    const uint32_t z_threads = (grad ? GT : COMPUTE + 32) + 32 + (DIST ? BTHREADS : 0);
+    // f32 logits under a soft-cap: S leaves c(v) in the buffer, so that G need not work it out again
+    constexpr bool LEAVE = CAP && sizeof(T) == 4;
     auto row_of = [&](uint32_t i) { return cluster + i * clusters; };
     auto weight = [&](uint32_t row) {
         return OP == OP_LOGPROB ? 1.0f : A.weights ? A.weights[row] : A.w_all;
@@ -673,7 +684,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             const int32_t tok = DIST ? 0 : A.tokens[row];
             sh.code[lane] = weight(row) != 0.0f && (uint32_t)tok < V ? tok : -1;
         }
-    } else if (TAIL && tid >= COMPUTE) {
+    } else if (DIST && tid >= COMPUTE) {
         for (uint32_t i = tid - COMPUTE - 32; i < 4 * A.bit_words; i += BTHREADS + 64) slots(0).bits[i] = 0;
     }
     if (tid == 0) {
@@ -696,7 +707,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             const Row<T> R(A.x, A.ld, row_of(i), V);
             const Slice sl = slice_of(R);
             const uint32_t count = sl.c1 - sl.c0, copied = min(count, A.keep);
-            const uint4 *buf = dyn + at * A.keep + tid;
+            uint4 *buf = dyn + at * A.keep + tid;
             there = bar_wait(&sh.full_bar[at], phase) && there;
             if (++at == 3) at = 0, phase ^= 1;
             if (DIST) bar_sync(BAR_P + (i & 1), p_threads);
@@ -710,18 +721,26 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                 };
                 // several chunks at a time, for one comparison with the running maximum
                 uint32_t c = tid;
+                auto work = [&](const uint4 &q, uint4 *at, uint32_t cu) {
+                    f2 v[E / 2];
+                    unpack<T>(q, v);
+#pragma unroll
+                    for (int e = 0; e < E / 2; e++) v[e] = capped2<CAP>(v[e], A.sc);
+                    if (LEAVE && grad) *at = pack<T>(v);
+                    G.chunk(v, k, marks(cu));
+                };
                 for (; c + (STEP - 1) * sum_threads < copied; c += STEP * sum_threads, buf += STEP * sum_threads) {
                     uint4 q[STEP];
 #pragma unroll
                     for (int u = 0; u < STEP; u++) q[u] = buf[u * sum_threads];
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
 #pragma unroll
-                    for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, marks(c + u * sum_threads));
+                    for (int u = 0; u < STEP; u++) work(q[u], buf + u * sum_threads, c + u * sum_threads);
                 }
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
                     const uint4 q = buf[0];
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
-                    G.chunk(q, A.sc, marks(c));
+                    work(q, buf, c);
                 }
                 // what did not fit
                 const T *x = R.at(sl.c0);
@@ -738,6 +757,8 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                         }
                 }
             }
+            // (the buffer is written by copies again)
+            if (LEAVE && grad) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             const Stat st = fold_lanes<TAIL, 32>(G.stat(), k);
             // (a copy that never came: the row is NaN)
             if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
@@ -746,8 +767,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
         }
     } else if (tid < COMPUTE) {
         // ---- warps G
-        constexpr uint32_t GT = COMPUTE / 2;
-        const uint32_t g = tid - GT;
+        const uint32_t g = tid - ST;
         uint32_t at = 0;
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t row = row_of(i);
@@ -769,9 +789,11 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                 if (wide) {
                     uint4 *o = reinterpret_cast<uint4 *>(out) + g;
 #pragma unroll 4
-                    for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT) *o = gr.template chunk<T, CAP>(*buf, A.sc);
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT) 
+                        *o = gr.template chunk<T, CAP, LEAVE>(*buf, A.sc);
                 } else {
-                    for (uint32_t c = g; c < copied; c += GT, buf += GT) store(c, gr.template chunk<T, CAP>(*buf, A.sc));
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT)
+                        store(c, gr.template chunk<T, CAP, LEAVE>(*buf, A.sc));
                 }
                 const T *x = R.at(sl.c0);
                 for (uint32_t c = copied + g; c < count; c += STEP * GT) {
@@ -979,7 +1001,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             fetch_logit(i + 1);
             const bool wanted = cur.w != 0.0f;
             float umax = -INFINITY, any = 0.0f;
-            if (b == 0) sh.edge_marks[set] = 0u;
+            if (b == 0) sh.edge_marks[set] = sh.twice[set] = 0u;
             if (wanted) {
                 for (uint32_t j = b; j < pad; j += BTHREADS) {
                     int32_t id = -1;
@@ -1011,11 +1033,14 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                     const float q = id < 0 ? 0.0f : expf((float)((double)sl.q[j] * A.sc.inv_t - ref));
                     sl.q[j] = q;
                     sum += (double)q;
-                    if (TAIL && id >= 0) {
+                    if (id >= 0) {
                         const uint32_t e = (uint32_t)id - e0;
-                        if (e < span) atomicOr(&sl.bits[e >> 5], 1u << (e & 31));
-                        else if ((uint32_t)id < R.lead) atomicOr(&sh.edge_marks[set], 1u << id);
-                        else if ((uint32_t)id >= V - R.trail) atomicOr(&sh.edge_marks[set], 256u << (id - (V - R.trail)));
+                        uint32_t *word = &sl.bits[e >> 5], bit = 1u << (e & 31);
+                        if (e >= span) {
+                            word = &sh.edge_marks[set];
+                            bit = (uint32_t)id < R.lead ? 1u << id : (uint32_t)id >= V - R.trail ? 256u << (id - (V - R.trail)) : 0u;
+                        }
+                        if (bit && (atomicOr(word, bit) & bit)) sh.twice[set] = 1u;
                     }
                 }
                 if (!TAIL) {
@@ -1038,6 +1063,7 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
             const Slice part = slice_of(R);
             const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
             if (!sh.slots_live[set]) return;
+            const bool twice = sh.twice[set] != 0u;
             T *out = (T *)A.grad + (size_t)row * A.ld_grad;
             for (uint32_t j = b; j < A.n_ids; j += BTHREADS) {
                 const int32_t id = sl.id[j];
@@ -1045,12 +1071,13 @@ __global__ void __launch_bounds__(row_threads(OP), 1) k_rows(RowArgs A, uint32_t
                 const uint32_t e = (uint32_t)id - e0;
                 const bool single = (uint32_t)id < R.lead || (uint32_t)id >= V - R.trail;
                 if (single ? rank != 0 : e >= span) continue;
-                if (TAIL && !single) sl.bits[e >> 5] = 0u;
+                if (!single) sl.bits[e >> 5] = 0u;
                 if (!grad) continue;
                 // p Q - q, where q is the sum over the slots that hold the id (the first of them writes)
-                float q = 0.0f;
+                float q = sl.q[j];
                 bool first = true;
-                for (uint32_t o = 0; o < pad; o += 4) {
+                if (twice) q = 0.0f;
+                for (uint32_t o = 0; twice && o < pad; o += 4) {
                     const int4 v = *reinterpret_cast<const int4 *>(sl.id + o);
                     if (v.x == id) q += sl.q[o], first = first && o >= j;
                     if (v.y == id) q += sl.q[o + 1], first = first && o + 1 >= j;
@@ -1816,7 +1843,7 @@ static bs_status launch_stream_typed(const char *what, const bs_logits *x, const
 
 // Shared memory of k_rows: three buffers of a slice, the teacher's slots.
 constexpr size_t ROWS_SMEM = SMEM_MAX - sizeof(RowsShared) - 256;
-constexpr uint32_t SLICE_MIN = 2 * COMPUTE;   // no row is split further than two chunks a thread
+constexpr uint32_t SLICE_MIN = 1024;   // no row is split further than two chunks a thread
 
 template <typename T, int OP, bool CAP>
 static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
@@ -1830,7 +1857,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     size_t slots = 0, room = 0;
     for (;; ranks *= 2, log_ranks++) {
         slice = (chunks + ranks - 1) / ranks;
-        A.bit_words = OP == OP_DISTILL_TAIL ? (slice * E + 31) / 32 : 0;
+        A.bit_words = is_distill(OP) ? (slice * E + 31) / 32 : 0;
         slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 48 + (size_t)A.bit_words * 16 : 0;
         room = slots < ROWS_SMEM ? (ROWS_SMEM - slots) / 48 : 0;
         // enough CTAs to hold the row, and to use the GPU where the rows are few
@@ -1846,7 +1873,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     if (most == 0) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(ranks);
-        cfg.blockDim = dim3(row_threads(OP));
+        cfg.blockDim = dim3(row_threads(OP, compute_threads<T>()));
         cfg.dynamicSmemBytes = ROWS_SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1860,7 +1887,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
         dev->clusters[log_ranks].store(most, std::memory_order_relaxed);
     }
     const uint32_t clusters = rows < (uint32_t)most ? rows : (uint32_t)most;
-    e = launch_clusters<K>(clusters * ranks, ranks, row_threads(OP), ROWS_SMEM, st, A, rows, clusters);
+    e = launch_clusters<K>(clusters * ranks, ranks, row_threads(OP, compute_threads<T>()), ROWS_SMEM, st, A, rows, clusters);
     return e == cudaSuccess ? BS_OK : failed("logit_ops", e);
 }
 
