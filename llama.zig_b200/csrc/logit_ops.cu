@@ -490,14 +490,14 @@ template <typename T, bool CAP> __host__ __device__ constexpr int sum_threads_of
 }
 struct RowsShared {
     float4 part[4][MAX_CWARPS];          // (m, s, u) of the warps S
-    float4 mail[2][MAX_CLUSTER];     // and of the row's CTAs
+    float4 mail[4][MAX_CLUSTER];     // and of the row's CTAs; two for each warp A
     Coef coef[4];
     int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
     // B's
     double scratch_d[BTHREADS / 32];
     float scratch_f[BTHREADS / 32];
     uint32_t slots_live[4], edge_marks[4], twice[4];   // twice: an id of the slice comes twice
-    uint64_t mail_bar[2], full_bar[3];
+    uint64_t mail_bar[4], full_bar[3];
 };
 
 // The sum of a warp's (or of each group of W lanes') Stats, the same in all its
@@ -688,8 +688,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         for (uint32_t i = tid - COMPUTE - 32; i < 4 * A.bit_words; i += BTHREADS + 64) slots(0).bits[i] = 0;
     }
     if (tid == 0) {
-        bar_init(&sh.mail_bar[0]);
-        bar_init(&sh.mail_bar[1]);
+        for (int i = 0; i < 4; i++) bar_init(&sh.mail_bar[i]);
         for (int i = 0; i < 3; i++) bar_init(&sh.full_bar[i]);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -759,7 +758,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             }
             // (the buffer is written by copies again)
             if (LEAVE && grad) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            const Stat st = fold_lanes<TAIL, 32>(G.stat(), k);
+            Stat st{-INFINITY, 0.0f, 0.0f};
+            if (sh.code[i & 15] >= 0) st = fold_lanes<TAIL, 32>(G.stat(), k);
             // (a copy that never came: the row is NaN)
             if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
             bar_arrive(BAR_X + (i & 3), x_threads);
@@ -856,6 +856,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             }
         };
         load4(which);
+        uint32_t sent = 0;        // exchanges of this warp so far
         for (uint32_t i = which; i < n; i += 2) {
             const Params cur = next;
             const uint32_t row = row_of(i);
@@ -889,15 +890,19 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 }
             }
             st = fold_lanes<TAIL, 32>(st, k);
-            if (ranks > 1) {
-                // A CTA sends row i's only after all have sent row i - 1's, so have read row i - 2's.  The token's
-                // logit goes along so that it has been read before another CTA may write the gradient over it.
-                if (lane < ranks) mail_send(&sh.mail[i & 1][rank], &sh.mail_bar[i & 1], lane, st, c_tok);
-                if (lane == 0) bar_expect(&sh.mail_bar[i & 1], ranks * 16);
-                const bool there = bar_wait(&sh.mail_bar[i & 1], i >> 1 & 1);
+            if (ranks > 1 && sh.code[i & 15] >= 0) {
+                // The rows that take part in an exchange count the same in every CTA.  A warp's exchanges take turns
+                // with two boxes: a CTA sends into one only after all have sent into the other, so have read what
+                // was in this one.  The token's logit goes along so that it has been read before another CTA may
+                // write the gradient over it.
+                const uint32_t box = which * 2 + (sent & 1), turn = sent >> 1 & 1;
+                sent++;
+                if (lane < ranks) mail_send(&sh.mail[box][rank], &sh.mail_bar[box], lane, st, c_tok);
+                if (lane == 0) bar_expect(&sh.mail_bar[box], ranks * 16);
+                const bool there = bar_wait(&sh.mail_bar[box], turn);
                 st = Stat{-INFINITY, 0.0f, 0.0f};
                 if (lane < ranks) {
-                    const float4 f = sh.mail[i & 1][lane];
+                    const float4 f = sh.mail[box][lane];
                     st = Stat{f.x, there ? f.y : NAN, f.z};   // (a CTA that never sent: the row is NaN)
                 }
                 st = fold_lanes<TAIL, MAX_CLUSTER>(st, k);
@@ -1020,8 +1025,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     }
                 }
             }
-            bool live = b_max(any) != 0.0f;
-            if (!TAIL) {
+            bool live = wanted && b_max(any) != 0.0f;   // (the same in all threads)
+            if (!TAIL && live) {
                 umax = b_max(umax);
                 live = live && umax != -INFINITY;   // no share to give: as without ids
             }

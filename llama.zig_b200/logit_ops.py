@@ -175,6 +175,8 @@ class _Rows:
         """(tensor, row stride) of the gradient."""
         import torch
         if out is None:
+            if self.ld == self.vocab and self.rows > 1:
+                return torch.empty_like(self.x), self.vocab
             g = torch.empty((self.rows, self.vocab), dtype=self.x.dtype, device=self.device)
             return g, self.vocab
         g = out.unsqueeze(0) if isinstance(out, torch.Tensor) and out.dim() == 1 else out
@@ -341,6 +343,6 @@ def policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs=None, wei
                                           _ptr(w), ctypes.byref(cfg), p + 16 * n, p, p + 4 * n, p + 8 * n, p + 12 * n,
                                           _ptr(g), ld, st), "bs_policy_loss")
         rows, lp, ent, kl, loss = buf.split_with_sizes((n, n, n, n, 1))
-        return PolicyLoss(loss[0], rows, lp, ent, kl, _like(logits, g))
+        return PolicyLoss(loss.squeeze(0), rows, lp, ent, kl, _like(logits, g))
 
     return r.run(call)
