@@ -449,13 +449,14 @@ template <bool ENT> struct GradRow {
 // Summing and gradient each need one ex2 a logit, so half of the warps do
 // either, and the special-function unit always has work while a row's sums
 // travel.  Barriers, in as many copies as rows can be between the two sides:
-// X (S -> A: row i summed), Y (A -> G: its coefficients), P (B -> S: its
-// slots), Z (-> C, B: done with; from G, or without a gradient from S and A).
+// X (S -> A: row i summed), Y (A -> G: its coefficients), Z (-> C, B: done
+// with; from G, or without a gradient from S and A); and mbarriers: full_bar
+// (copy -> S), slots_bar (B -> S), mail_bar (A -> A of the other CTAs).
 constexpr uint32_t COPY = 512;       // chunks of one copy
 constexpr int STEP = 4;              // chunks of a thread summed at a time
 constexpr int MAX_CWARPS = 24;       // most warps S and G together
 constexpr int BTHREADS = 128;
-enum Bar { BAR_X = 1, BAR_Y = 5, BAR_Z = 9, BAR_P = 13, BAR_B = 15 };
+enum Bar { BAR_X = 1, BAR_Y = 5, BAR_Z = 9, BAR_B = 13 };
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -497,7 +498,7 @@ struct RowsShared {
     double scratch_d[BTHREADS / 32];
     float scratch_f[BTHREADS / 32];
     uint32_t slots_live[4], edge_marks[4], twice[4];   // twice: an id of the slice comes twice
-    uint64_t mail_bar[4], full_bar[3];
+    uint64_t mail_bar[4], full_bar[3], slots_bar[4];
 };
 
 // The sum of a warp's (or of each group of W lanes') Stats, the same in all its
@@ -526,6 +527,9 @@ __device__ __forceinline__ void bar_init(uint64_t *bar) {
 }
 __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_local(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void mail_send(const float4 *slot, const uint64_t *bar, uint32_t rank, const Stat &a, float w) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %5}, [%4];" ::"r"(
@@ -649,7 +653,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     // threads of S and G, and of the barriers
     constexpr uint32_t ST = sum_threads_of<T, CAP>(), GT = COMPUTE - ST;
     const uint32_t sum_threads = grad ? ST : COMPUTE, x_threads = sum_threads + 32;
-    const uint32_t y_threads = GT + 32, p_threads = sum_threads + BTHREADS;
+    const uint32_t y_threads = GT + 32;
     const uint32_t z_threads = (grad ? GT : COMPUTE + 32) + 32 + (DIST ? BTHREADS : 0);
     // f32 logits under a soft-cap: S leaves c(v) in the buffer, so that G need not work it out again
     constexpr bool LEAVE = CAP && sizeof(T) == 4;
@@ -688,7 +692,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         for (uint32_t i = tid - COMPUTE - 32; i < 4 * A.bit_words; i += BTHREADS + 64) slots(0).bits[i] = 0;
     }
     if (tid == 0) {
-        for (int i = 0; i < 4; i++) bar_init(&sh.mail_bar[i]);
+        for (int i = 0; i < 4; i++) bar_init(&sh.mail_bar[i]), bar_init(&sh.slots_bar[i]);
         for (int i = 0; i < 3; i++) bar_init(&sh.full_bar[i]);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -709,7 +713,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             uint4 *buf = dyn + at * A.keep + tid;
             there = bar_wait(&sh.full_bar[at], phase) && there;
             if (++at == 3) at = 0, phase ^= 1;
-            if (DIST) bar_sync(BAR_P + (i & 1), p_threads);
+            if (DIST) there = bar_wait(&sh.slots_bar[i & 3], i >> 2 & 1) && there;
             Gather<T, CAP, !DIST, TAIL> G;
             if (sh.code[i & 15] >= 0) {
                 const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
@@ -1094,22 +1098,20 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 out[id] = from_f<T>((p * cf.q_all - cf.wm * q) * slope<CAP>(sl.c[j], A.sc));
             }
         };
-        // P of row i may be signalled once P of row i - 2 has been waited for: after Z of row i - 3
         one = fetch(0);
         two = fetch(1);
         fetch_logit(0);
-        for (uint32_t i = 0; i < 3 && i < n; i++) {
+        auto ready = [&](uint32_t i) {
             prepare(i);
-            if (i < 2) bar_arrive(BAR_P + (i & 1), p_threads);
-        }
+            bar_sync(BAR_B, BTHREADS);
+            if (b == 0) bar_arrive_local(&sh.slots_bar[i & 3]);
+        };
+        for (uint32_t i = 0; i < 3 && i < n; i++) ready(i);
         for (uint32_t i = 0; i < n; i++) {
-            bar_sync(BAR_Z + (i & 3), z_threads);   // row i's gradient is written
-            if (i + 2 < n) bar_arrive(BAR_P + (i & 1), p_threads);
+            if (i + 3 < n) ready(i + 3);               // (its set was row i - 1's)
+            bar_sync(BAR_Z + (i & 3), z_threads);      // row i's gradient is written
             finish(i);
-            if (i + 3 < n) {
-                bar_sync(BAR_B, BTHREADS);
-                prepare(i + 3);   // (its set was row i - 1's)
-            }
+            bar_sync(BAR_B, BTHREADS);
         }
     }
 }
