@@ -736,9 +736,29 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     uint4 q[STEP];
 #pragma unroll
                     for (int u = 0; u < STEP; u++) q[u] = buf[u * sum_threads];
-                    G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+                    if constexpr (LEAVE) {
+                        // (the soft-cap of all of them first: that of the largest alone would be waited for)
 #pragma unroll
-                    for (int u = 0; u < STEP; u++) work(q[u], buf + u * sum_threads, c + u * sum_threads);
+                        for (int u = 0; u < STEP; u++) {
+                            f2 v[E / 2];
+                            unpack<T>(q[u], v);
+#pragma unroll
+                            for (int e = 0; e < E / 2; e++) v[e] = capped2<CAP>(v[e], A.sc);
+                            q[u] = pack<T>(v);
+                            if (grad) buf[u * sum_threads] = q[u];
+                        }
+                        G.raise(max_of<T>(q), k);
+#pragma unroll
+                        for (int u = 0; u < STEP; u++) {
+                            f2 v[E / 2];
+                            unpack<T>(q[u], v);
+                            G.chunk(v, k, marks(c + u * sum_threads));
+                        }
+                    } else {
+                        G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
+#pragma unroll
+                        for (int u = 0; u < STEP; u++) work(q[u], buf + u * sum_threads, c + u * sum_threads);
+                    }
                 }
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
                     const uint4 q = buf[0];
