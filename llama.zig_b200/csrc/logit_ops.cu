@@ -1206,6 +1206,7 @@ __global__ void __launch_bounds__(1024) k_loss(const float *row_loss, const floa
                                                float *loss) {
     __shared__ double part[32];
     double s = 0.0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' losses are there
     for (uint32_t i = threadIdx.x; i < rows; i += 1024) {
         const float w = weights ? weights[i] : w_all;
         if (w != 0.0f) s += (double)w * (double)row_loss[i];
@@ -1768,6 +1769,23 @@ static cudaError_t launch_clusters(uint32_t grid, uint32_t ranks, uint32_t threa
     return cudaLaunchKernelEx(&cfg, K, args...);
 }
 
+// A launch that may overlap the end of the stream's previous kernel (the kernel
+// waits for that one before it reads its results).
+template <auto K, typename... Q>
+static cudaError_t launch_after(uint32_t grid, uint32_t threads, size_t smem, cudaStream_t st, Q... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, K, args...);
+}
+
 // The current device's entry of kernel K's table, with K allowed all of an
 // SM's shared memory (per device, as kernel attributes are) and, if `wide`,
 // clusters of 16.
@@ -1836,19 +1854,7 @@ static bs_status launch_stream(const char *what, RowArgs A, uint32_t rows, TopAr
     if constexpr (TOP) {
         constexpr auto S = k_select<T, CAP>;
         if (e == cudaSuccess && !P.fused) e = device_info<S>(&dev, false);
-        if (e == cudaSuccess && !P.fused) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(rows);
-            cfg.blockDim = dim3(THREADS);
-            cfg.dynamicSmemBytes = smem;
-            cfg.stream = st;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps k_stream's end
-            attr[0].val.programmaticStreamSerializationAllowed = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            e = cudaLaunchKernelEx(&cfg, S, A, P);
-        }
+        if (e == cudaSuccess && !P.fused) e = launch_after<S>(rows, THREADS, smem, st, A, P);   // (its launch overlaps k_stream's end)
     }
     return e == cudaSuccess ? BS_OK : failed(what, e);
 }
@@ -1940,8 +1946,8 @@ static RowArgs row_args(const bs_logits *x, const Scale &sc) {
 }
 
 static bs_status total_loss(const RowArgs &A, uint32_t rows, float *loss, cudaStream_t st) {
-    k_loss<<<1, 1024, 0, st>>>(A.row_loss, A.weights, A.w_all, rows, loss);
-    return launched("logit_ops loss");
+    cudaError_t e = launch_after<k_loss>(1, 1024, 0, st, (const float *)A.row_loss, A.weights, A.w_all, rows, loss);
+    return e == cudaSuccess ? BS_OK : failed("logit_ops loss", e);
 }
 
 static bs_status no_rows(float *d_loss, void *stream) {
