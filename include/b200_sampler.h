@@ -250,9 +250,10 @@ bs_status bs_sample_static(const bs_config *cfg, uint64_t *d_rng, const float *d
  * number of calls may run at once.  The sums are f32, in an order fixed by
  * the sizes and the alignment: the same call gives the same bits.
  *
- * Logits of -inf are masked tokens (p = 0, gradient 0 without a soft-cap); a
- * NaN or +inf logit makes its row NaN; a row all of -inf has no distribution
- * and is NaN too.  Gradients are of the logits' type, rounded once from f32;
+ * Logits of -inf are masked tokens (p = 0, gradient 0), a +inf logit makes its
+ * row NaN, a row all of -inf has no distribution and is NaN too (all three
+ * without a soft-cap, which makes +-cap of them); a NaN makes its row NaN.  So
+ * does a bounded device wait that gave up.  Gradients are of the logits' type, rounded once from f32;
  * d_grad may be the logits themselves (same pointer, ld_grad = ld) and must
  * not overlap them in any other way. */
 typedef enum bs_dtype { BS_F32 = 0, BS_BF16 = 1, BS_F16 = 2 } bs_dtype;

@@ -982,6 +982,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             bar_sync(BAR_Z + (i & 3), z_threads);
             if (i + 3 < n) copy(i + 3);
         }
+        // (S has seen every copy land; were it to have given up on one, it still lands before the CTA's memory goes)
+        for (uint32_t i = n > 3 ? n - 3 : 0; i < n; i++) bar_wait(&sh.full_bar[i % 3], i / 3 & 1);
     } else if constexpr (DIST) {
         // ---- warps B
         const uint32_t b = tid - COMPUTE - 96;

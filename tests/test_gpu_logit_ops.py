@@ -612,6 +612,47 @@ def test_refusals_on_device(gpu_pkg):
         gpu_pkg.policy_loss(x, t, f, f, clip_low=-1.0)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows,vocab,ld", [(4000, 1031, 1031), (2500, 4096, 4096), (700, 40003, 40003), (400, 128256, 128256),
+                                           (90, 256000, 256001)])
+def test_many_rows(gpu_pkg, dtype, rows, vocab, ld):
+    """Long runs of rows through the same thread blocks, left-out rows scattered and in runs among them."""
+    x, _ = make(rows, vocab, dtype, 131, ld, 1 if ld % 8 else 0)
+    g = torch.Generator(device="cuda").manual_seed(132)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda").int()
+    t[torch.rand(rows, generator=g, device="cuda") < 0.1] = -1
+    ref = Ref(x)
+    old, adv, rlp, w = policy_inputs(ref, t, 133)
+    w[torch.rand(rows, generator=g, device="cuda") < 0.2] = 0.0
+    w[rows // 3:rows // 3 + rows // 5] = 0.0
+    got = gpu_pkg.policy_loss(x, t, old, adv, rlp, w, clip_low=0.1, clip_high=0.3, kl_coef=0.1, entropy_coef=0.01)
+    want = policy_ref(ref, dtype, t, old, adv, rlp, w, 0.1, 0.3, 0.1, 0.01)
+    near(got.row_losses, want["L"], want["tol_L"], "rows")
+    near(got.loss, want["loss"], want["tol_loss"] + 2 * EPS * (want["L"].abs() * w.double()).sum(), "loss")
+    near(got.grad, want["grad"], want["tol_g"], "grad")
+    no = gpu_pkg.policy_loss(x, t, old, adv, rlp, w, clip_low=0.1, clip_high=0.3, kl_coef=0.1, entropy_coef=0.01, grad=False)
+    near(no.row_losses, want["L"], want["tol_L"], "rows without a gradient")
+    del got, no, want
+    r = gpu_pkg.token_logprobs(x, t)
+    live, lp, hot = ref.token(t)
+    near(r.logprobs, torch.where(live, lp, 0.0), ref.lp_tol(lp), "logprobs")
+    del hot
+    for K in (7, 150):
+        tl, ids, lse, _ = teacher_for(x, K, 134, 1.0)
+        ids[torch.rand(rows, generator=g, device="cuda") < 0.1] = -1      # no teacher
+        ids[::5, 1] = ids[::5, 0]                                         # an id twice
+        for s in (None, lse):
+            got = gpu_pkg.distill_loss(x, ids, tl, s, w)
+            want = distill_ref(ref, dtype, ids, tl, s, w, 1.0)
+            near(got.row_losses, want["L"], want["tol_L"], ("rows", K))
+            near(got.grad, want["grad"], want["tol_g"], ("grad", K))
+            no = gpu_pkg.distill_loss(x, ids, tl, s, w, grad=False)
+            near(no.row_losses, want["L"], want["tol_L"], ("rows without a gradient", K))
+    top = gpu_pkg.top_logits(x, 9)
+    at = torch.linspace(0, rows - 1, 20).long().cuda()
+    assert np.array_equal(top.ids[at].cpu().numpy(), top_ref(x[at], 9)[0])
+
+
 def run_all(pkg, x, t, old, adv, rlp, w, ids, tl, lse, stream=None):
     """The operators together, as an update uses them."""
     r = pkg.token_logprobs(x, t, stream=stream)
@@ -659,6 +700,62 @@ def test_streams_and_graphs(gpu_pkg):
     torch.cuda.synchronize()
     for outs in [o for _, o, _ in graphs] + [eager]:
         assert all(torch.equal(a, b) for a, b in zip(outs, want2))
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import __graft_entry__ as g
+pkg = g.load_package()
+x = torch.randn(40, 20000, device="cuda", dtype=torch.bfloat16)
+t = torch.arange(40, device="cuda", dtype=torch.int32)
+f = torch.full((40,), 0.02, device="cuda")
+ids = torch.arange(4, device="cuda", dtype=torch.int32).repeat(40, 1)
+tl = torch.randn(40, 4, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def run():
+    r = pkg.token_logprobs(x, t)
+    return [pkg.token_logprobs_grad(x, t, r, f, f), pkg.top_logits(x, 5).ids, pkg.policy_loss(x, t, f, f, f, f, kl_coef=0.1).grad,
+            pkg.distill_loss(x, ids, tl, None, f).grad]
+with torch.cuda.graph(graph):
+    outs = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(outs, run()))
+print("captured")
+"""
+
+
+def test_first_call_may_be_captured(gpu_pkg):
+    import subprocess
+    import sys
+    root = gpu_pkg.build.ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_from_two_threads(gpu_pkg):
+    import threading
+    ins = [all_inputs(30, 32003, "bf16", 141), all_inputs(30, 32003, "bf16", 151)]
+    want = [[v.clone() for v in run_all(gpu_pkg, *i)] for i in ins]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        s = torch.cuda.Stream()
+        for _ in range(20):
+            got = run_all(gpu_pkg, *ins[k], stream=s)
+            s.synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                bad.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_same_call_same_bits(gpu_pkg):
