@@ -422,11 +422,11 @@ template <bool ENT> struct GradRow {
 };
 
 // ---------------------------------------------------------------------------
-// The row kernel: statistics, results and (for the losses) the gradient of
-// whole rows, each logit read from memory once.
+// The losses' kernel: statistics, results and gradient of whole rows, each
+// logit read from memory once.
 //
-// What bounds it is HBM: V s bytes read and V s written a row, against some
-// ten issue slots and two ex2 a logit.  A row must be known whole before its
+// Its floor is HBM: V s bytes read and V s written a row, against some 14
+// issue slots and two ex2 a logit.  A row must be known whole before its
 // gradient starts, so it is kept on chip: a cluster of CTAs (one per SM) takes
 // a row, each CTA a slice of up to 1/3 of its shared memory, and the three
 // buffers hold the row whose gradient is being written, the row being summed
@@ -452,6 +452,19 @@ template <bool ENT> struct GradRow {
 // X (S -> A: row i summed), Y (A -> G: its coefficients), Z (-> C, B: done
 // with; from G, or without a gradient from S and A); and mbarriers: full_bar
 // (copy -> S), slots_bar (B -> S), mail_bar (A -> A of the other CTAs).
+//
+// Measured (policy loss and gradient, of the copy bandwidth for one read and
+// one write): 777 x 151936 f32 152 us, 95 %; 4096 x 128256 bf16 380 us, 79 %,
+// where the sums are what takes longest (4,500 cycles a slice of 32,000 logits
+// beside the gradient's 4,200; the copies take 4,900 a row on the 132 SMs that
+// clusters of four find, their own sum with nothing beside it 2,600).  Steps on
+// the way, 4096 x 128256 bf16: one CTA a row, read twice 523 us; clusters of
+// small CTAs that keep the row 543; this pipeline with one set of warps for
+// both passes and copies by the threads 488, with bulk copies 441 (the threads'
+// copies stalled on the memory system's queue), sums and gradient by different
+// warps 390, two exchange warps and more threads 380.  Two CTAs to an SM with
+// half the slice each: 504.  A quarter of the ex2 as polynomials on the FMA
+// pipe: 399.
 constexpr uint32_t COPY = 512;       // chunks of one copy
 constexpr int STEP = 4;              // chunks of a thread summed at a time
 constexpr int MAX_CWARPS = 24;       // most warps S and G together
@@ -483,8 +496,11 @@ struct Coef {
     uint32_t live;       // 0: the row is left out
 };
 // Threads of S and G, and of S alone where there is a gradient to write.  The
-// 16-bit types have twice the logits a byte and want more of both; f32 under a
-// soft-cap leaves most of the work to S (see LEAVE).
+// 16-bit types have twice the logits a byte and want more of both: 4096 x 128256
+// bf16 390 us with 512, 380 with 640, 389 with 768; 777 x 151936 f32 152 with
+// 512, 155 with 640.  Other shares than half: 394 with 352 of 640.  f32 under a
+// soft-cap leaves most of the work to S (see LEAVE): 512 x 256000 305 us with 384
+// of 512, 308 with 320.
 template <typename T> __host__ __device__ constexpr int compute_threads() { return sizeof(T) == 4 ? 512 : 640; }
 template <typename T, bool CAP> __host__ __device__ constexpr int sum_threads_of() {
     return CAP && sizeof(T) == 4 ? 384 : compute_threads<T>() / 2;
@@ -1141,7 +1157,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
 // The logits' gradient from those of log-probability and entropy, with the
 // forward pass's statistics:
 //   dv_j = m c'(v_j) [g (d_jt - p_j) - h p_j (log p_j + H)]
-// Grid: rows x slices of GRAD_SLICE chunks.
+// Grid: rows x slices of GRAD_SLICE chunks.  A pure stream, one read and one
+// write a logit: 2048 x 151936 bf16 (1792 rows read) 179 us, the copy bandwidth.
 constexpr int GRAD_BATCH = 4;
 constexpr uint32_t GRAD_SLICE = THREADS * GRAD_BATCH * 2;   // chunks of a CTA
 template <typename T, bool CAP, bool ENT>
@@ -1309,7 +1326,11 @@ template <typename T> __device__ __noinline__ void select_whole_row(const T *x, 
 // few bins), the tiles' loads are under way together, and the sort is one of
 // 64 elements in a warp's registers and a rank by binary searches in the other
 // warps' runs.  Where there are hardly more tiles than wanted logits (`each`),
-// the logits themselves are searched.
+// the logits themselves are searched.  A floor below very many equal values is
+// left where it is: the larger logits are taken and the rest filled up with the
+// lowest ids that have the value.  Measured, with k_stream before it: top 64 of
+// 256 x 128256 f32 38 us (10 of them here), top 256 of 1024 x 256000 bf16 133;
+// by a radix selection over the whole row 515 and 2015.
 struct TopArgs {
     uint32_t top;
     float out_scale;
@@ -1579,8 +1600,13 @@ __device__ __forceinline__ void select_top(const Row<T> &R, uint32_t row, const 
 // ---------------------------------------------------------------------------
 // One pass over the rows without a gradient: log-probability and entropy of
 // the rows' tokens, or (TOP) the rows' lse and the largest logit of each
-// 128-byte tile, from which CTA 0 of the row then selects.  Bound by HBM reads, so many small CTAs with
-// their loads under way at once; few rows are split over clusters of CTAs.
+// 128-byte tile, from which CTA 0 of the row then selects.  Bound by HBM reads,
+// so many small CTAs with their loads under way at once; few rows are split
+// over clusters of CTAs.  Measured: 1792 live rows of 151936 bf16 91 us, 91 % of
+// the copy bandwidth (the persistent form of the losses' kernel took 129: one
+// CTA an SM has too few warps for a pass that only reads); 256 x 128256 f32
+// 27 us, 74 %, two waves of CTAs with their start and end.  Three or five CTAs
+// an SM: 97 and 95 us.
 constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
 struct StreamShared {
     Stat warp[WARPS];
@@ -1895,7 +1921,9 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
         A.bit_words = is_distill(OP) ? (slice * E + 31) / 32 : 0;
         slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 48 + (size_t)A.bit_words * 16 : 0;
         room = slots < ROWS_SMEM ? (ROWS_SMEM - slots) / 48 : 0;
-        // enough CTAs to hold the row, and to use the GPU where the rows are few
+        // Enough CTAs to hold the row, and to use the GPU where the rows are few.  Sixteen only where eight cannot
+        // hold it (seven such clusters fit the GPU, 112 SMs): 512 x 256000 f32 424 us, with eight and the rest of
+        // the slices read again from L2 495.
         if (ranks == MAX_CLUSTER ||
             (slice <= room && !(ranks < 8 && (uint64_t)rows * ranks * 2 <= (uint64_t)dev->sms.load() && slice / 2 >= SLICE_MIN)))
             break;
