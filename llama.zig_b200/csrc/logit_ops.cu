@@ -281,27 +281,9 @@ template <typename T> struct Row {
 struct Stat {
     float m, s, u;
 };
-__device__ __forceinline__ void rebase(Stat &a, float m, float k) {
-    // factor 2^((a.m - m) k); fmaxf also turns -inf - -inf into "nothing there"
-    float d = fmaxf((a.m - m) * k, D_MIN);
-    float f = ex2(d);
-    a.u = f * fmaf(d, a.s, a.u);
-    a.s *= f;
-    a.m = m;
-}
 // A maximum of -inf (all of the set masked) is replaced by 0 in differences,
 // so that the masked logits give 2^-inf = 0.
 __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.0f : m; }
-
-__device__ __forceinline__ Stat merge(Stat a, const Stat &b, float k) {
-    float m = fmaxf(a.m, b.m);
-    Stat c = b;
-    rebase(a, m, k);
-    rebase(c, m, k);
-    a.s += c.s;
-    a.u += c.u;
-    return a;
-}
 
 // What a thread gathers of the logits it reads, on the scale of its running
 // maximum m: s = sum 2^d and u = sum 2^d d in pairs (even and odd logits).
@@ -312,7 +294,7 @@ template <typename T, bool CAP, bool ENT, bool TAIL> struct Gather {
     float m = -INFINITY, top = 0.0f;
     f2 s = {0.0f, 0.0f}, u = {0.0f, 0.0f};
     __device__ __forceinline__ void raise(float to, float k) {
-        if (to > m) {
+        if (to > m) {   // (fmaxf: from -inf there is nothing to rescale)
             const float d = fmaxf((m - to) * k, D_MIN), f = ex2(d);
             if (TAIL) top *= f;
             if (ENT) u = mul2(both(f), fma2(both(d), s, u));
@@ -367,11 +349,6 @@ template <typename T, bool CAP, bool ENT, bool TAIL> struct Gather {
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }

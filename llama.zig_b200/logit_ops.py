@@ -79,20 +79,19 @@ class PolicyLoss(NamedTuple):
     grad: Optional["torch.Tensor"]
 
 
-_dtypes = None
+torch = None      # imported by the first call: the rest of the package does without
+_dtypes = {}      # torch types -> bs_dtype
 
 
-def _codes():
-    global _dtypes
-    if _dtypes is None:
-        import torch
-        _dtypes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    return _dtypes
+def _import_torch():
+    global torch
+    import torch as t
+    _dtypes.update({t.float32: 0, t.bfloat16: 1, t.float16: 2})
+    torch = t
 
 
 def _raw_stream(index):
     """The current stream of a device, as a pointer."""
-    import torch
     fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return fast(index) if fast is not None else torch.cuda.current_stream(index).cuda_stream
 
@@ -101,9 +100,10 @@ class _Rows:
     """Checked logits of one call: the descriptor, and where to run."""
 
     def __init__(self, logits, temperature, softcap, logit_scale, stream):
-        import torch
+        if torch is None:
+            _import_torch()
         x = logits
-        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _codes():
+        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _dtypes:
             raise ValueError("logits must be a CUDA tensor of float32, bfloat16 or float16")
         if x.dim() == 1:
             x = x.unsqueeze(0)
@@ -116,14 +116,13 @@ class _Rows:
         if self.vocab > MAX_VOCAB:
             raise ValueError(f"vocab is at most {MAX_VOCAB}")
         self.x, self.ld, self.device = x, ld, x.device
-        self.desc = BsLogits(x.data_ptr(), ld, self.rows, self.vocab, _codes()[x.dtype], temperature, softcap,
+        self.desc = BsLogits(x.data_ptr(), ld, self.rows, self.vocab, _dtypes[x.dtype], temperature, softcap,
                              logit_scale)
         self._stream = stream
 
     def run(self, call):
         """``call(stream)`` with the logits' device and the caller's stream
         current: results are allocated on the stream that writes them."""
-        import torch
         s, index = self._stream, self.device.index
         if s is None:
             if torch.cuda.current_device() == index:
@@ -139,7 +138,6 @@ class _Rows:
 
     def floats(self, t, what, shape=None):
         """A float32 input on the logits' device, packed."""
-        import torch
         shape = (self.rows,) if shape is None else shape
         if isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.device == self.device and t.shape == shape \
                 and t.is_contiguous():
@@ -155,7 +153,6 @@ class _Rows:
     def ids(self, t, what, shape=None):
         """Token ids as packed int32; an id that int32 cannot hold is outside
         every vocabulary and becomes -1."""
-        import torch
         shape = (self.rows,) if shape is None else shape
         if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == self.device and t.shape == shape \
                 and t.is_contiguous():
@@ -173,7 +170,6 @@ class _Rows:
 
     def grad_out(self, out):
         """(tensor, row stride) of the gradient."""
-        import torch
         if out is None:
             if self.ld == self.vocab and self.rows > 1:
                 return torch.empty_like(self.x), self.vocab
@@ -195,9 +191,8 @@ class _Rows:
                 raise ValueError("out overlaps the logits without being them")
         return g, ld
 
-    def empty(self, *shape, dtype=None):
-        import torch
-        return torch.empty(shape, dtype=dtype or torch.float32, device=self.device)
+    def empty(self, *shape):
+        return torch.empty(*shape, dtype=torch.float32, device=self.device)
 
 
 def _ptr(t):
@@ -220,13 +215,11 @@ def token_logprobs(logits, tokens, *, temperature: float = 1.0, final_logit_soft
 
     def call(st):
         t = r.ids(tokens, "tokens")
-        n = r.rows
-        buf = r.empty(4 * n)
-        p = buf.data_ptr()
-        _s._check(_s.lib().bs_token_logprobs(ctypes.byref(r.desc), t.data_ptr(), p, p + 4 * n, p + 8 * n, st),
-                  "bs_token_logprobs")
-        lp, ent, stats = buf.split_with_sizes((n, n, 2 * n))
-        return TokenLogprobs(lp, ent, stats.view(n, 2))
+        lp = r.empty(r.rows)
+        ent, stats = torch.empty_like(lp), r.empty(r.rows, 2)
+        _s._check(_s.lib().bs_token_logprobs(ctypes.byref(r.desc), t.data_ptr(), lp.data_ptr(), ent.data_ptr(),
+                                             stats.data_ptr(), st), "bs_token_logprobs")
+        return TokenLogprobs(lp, ent, stats)
 
     return r.run(call)
 
@@ -262,10 +255,9 @@ def top_logits(logits, k: int, *, temperature: float = 1.0, final_logit_softcapp
     r = _Rows(logits, temperature, final_logit_softcapping, logit_scale, stream)
     if not 1 <= int(k) <= min(r.vocab, MAX_TOP):
         raise ValueError(f"k must be between 1 and the vocabulary (and {MAX_TOP})")
-    import torch
-
     def call(st):
-        values, ids, lse = r.empty(r.rows, k), r.empty(r.rows, k, dtype=torch.int32), r.empty(r.rows)
+        values, lse = r.empty(r.rows, k), r.empty(r.rows)
+        ids = torch.empty(r.rows, k, dtype=torch.int32, device=r.device)
         L, d = _s.lib(), ctypes.byref(r.desc)
         size = L.bs_top_logits_workspace(d)
         work = r.empty(size // 4)
@@ -301,7 +293,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
         lse = None if teacher_lse is None else r.floats(teacher_lse, "teacher_lse")
         w = None if weights is None else r.floats(weights, "weights")
         g, ld = r.grad_out(out) if grad else (None, 0)
-        loss, rows = r.empty(), r.empty(r.rows)
+        rows = r.empty(r.rows)
+        loss = rows.new_empty(())
         _s._check(_s.lib().bs_distill_loss(ctypes.byref(r.desc), ids.data_ptr(), tl.data_ptr(), _ptr(lse), shape[1],
                                            _ptr(w), loss.data_ptr(), rows.data_ptr(), _ptr(g), ld, st),
                   "bs_distill_loss")
