@@ -96,7 +96,8 @@ SHAPES = [  # rows, vocab, ld, offset in elements
     (2, 32003, 32003, 1), (6, 32000, 32768, 0), (150, 4099, 4100, 0), (1, 128256, 128256, 0), (3, 151936, 151936, 7),
     (2, 256000, 256000, 0), (1, 300001, 300001, 0), (9, 40000, 40000, 0), (17, 16385, 16385, 3),
 ]
-FACTORS = [dict(T=1.0, cap=0.0, scale=1.0), dict(T=0.7, cap=30.0, scale=2.0)]
+T07 = float(np.float32(0.7))   # the C ABI takes the temperature as f32
+FACTORS = [dict(T=1.0, cap=0.0, scale=1.0), dict(T=T07, cap=30.0, scale=2.0)]
 
 
 def how(f):
