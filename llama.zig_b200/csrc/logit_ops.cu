@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 if (wide) {
                     uint4 *o = reinterpret_cast<uint4 *>(out) + g;
 #pragma unroll 4
-                    for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT) 
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT)
                         *o = gr.template chunk<T, CAP, LEAVE>(*buf, A.sc);
                 } else {
                     for (uint32_t c = g; c < copied; c += GT, buf += GT)
