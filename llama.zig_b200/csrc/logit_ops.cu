@@ -40,6 +40,7 @@ struct Scale {
     float k;         // m log2(e)
     float m;         // 1 / (logit_scale T)
     float cap, icap; // soft-cap and its reciprocal
+    double md;       // m in 64 bits
     double inv_t;    // 1 / T
     double dk;       // what rounding left off k, relative
 };
@@ -62,7 +63,8 @@ struct RowArgs {
     const float *weights;       // null: 1 / rows each
     float w_all;
     const float *old_lp, *adv, *ref_lp;
-    float clip_lo, clip_hi, kl_coef, ent_coef;
+    double clip_lo, clip_hi;
+    float kl_coef, ent_coef;
     const int32_t *t_ids;       // rows x n_ids
     const float *t_logits, *t_lse;
     uint32_t n_ids;
@@ -467,9 +469,9 @@ __host__ __device__ constexpr int row_threads(int op, int compute) { return comp
 // Row i's results as the gradient needs them.
 struct Coef {
     float m, l2s;        // maximum, log2 S
-    float ca, cb, ct;    // dv_j = c'(v_j) p_j (ca + cb log2 p_j), + c'(v_t) ct at the token
+    float ca, cb;        // dv_j = c'(v_j) p_j (ca + cb log2 p_j)
+    float ct;            // the token's dv
     float q_all, wm;     // teacher's ids: c'(v_j) (p_j q_all - wm q_j)
-    float c_tok;         // the token's c(v)
     uint32_t live;       // 0: the row is left out
 };
 // Threads of S and G, and of S alone where there is a gradient to write.  The
@@ -544,46 +546,54 @@ __device__ __forceinline__ bool bar_wait(const uint64_t *bar, uint32_t parity) {
     return false;
 }
 
-// Results and coefficients of a row with a token.
+// Results and coefficients of a row with a token.  A few values a row, so all
+// in 64 bits from the f32 sums: a ratio near 1, a KL near 0 and a loss whose
+// terms cancel leave the sums' rounding and not their own.
 struct TokenIn {
     float w, adv, old_lp, ref_lp, c_tok;
+    float slope;         // the soft-cap's, at the token
 };
+// The gradient at the token itself, before the soft-cap's slope, from those of
+// log-probability and entropy: g (1 - p) - h p (log p + H).  1 - p is -expm1
+// of log p, whose bits a p near 1 in f32 has lost.
+__device__ __forceinline__ double token_slope(double lp, double H, double g, double h) {
+    return -g * expm1(lp) - (h != 0.0 ? h * exp(lp) * (fmax(lp, -1e4) + H) : 0.0);
+}
 template <int OP>
 __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const Stat &st, const TokenIn &in, bool write) {
-    const double m = st.m, ratio = (double)(st.u / st.s);
+    const double m = st.m, ratio = (double)st.u / (double)st.s;
     // k is m log2 e in f32: to first order, what its rounding did to the sum
-    const double l2s = log2_d(st.s) + A.sc.dk * ratio;
-    const double lp = LN2_D * (((double)in.c_tok - m) * ((double)A.sc.k * (1.0 + A.sc.dk)) - l2s);
-    const float H = (float)(LN2_D * (l2s - (1.0 + A.sc.dk) * ratio));
-    Coef c{st.m, (float)l2s, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, in.c_tok, 1u};
-    float kl = 0.0f, loss = 0.0f;
+    const double ln_s = log((double)st.s) + LN2_D * A.sc.dk * ratio;
+    const double lp = ((double)in.c_tok - m) * A.sc.md - ln_s;
+    const double H = ln_s - LN2_D * (1.0 + A.sc.dk) * ratio;
+    Coef c{st.m, (float)(ln_s / LN2_D), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 1u};
+    double kl = 0.0, loss = 0.0;
     if (is_policy(OP)) {
-        const float r = expf((float)(lp - (double)in.old_lp));
+        const double adv = in.adv, r = exp(lp - (double)in.old_lp);
         // min(r A, clip(r) A) is the clipped one only beyond the bound that A favours
-        const bool over = in.adv > 0.0f && r > A.clip_hi, under = in.adv < 0.0f && r < A.clip_lo;
-        loss = -in.adv * (over ? A.clip_hi : under ? A.clip_lo : r);
-        float g = over || under ? 0.0f : -r * in.adv;
+        const bool over = adv > 0.0 && r > A.clip_hi, under = adv < 0.0 && r < A.clip_lo;
+        loss = -adv * (over ? A.clip_hi : under ? A.clip_lo : r);
+        double g = over || under ? 0.0 : -r * adv;
         if (A.ref_lp) {
-            const float dr = (float)((double)in.ref_lp - lp);
-            const float x1 = expm1f(dr);
+            const double dr = (double)in.ref_lp - lp, x1 = expm1(dr);
             kl = x1 - dr;
             if (A.kl_coef != 0.0f) {
-                loss += A.kl_coef * kl;
-                g -= A.kl_coef * x1;
+                loss += (double)A.kl_coef * kl;
+                g -= (double)A.kl_coef * x1;
             }
         }
-        if (OP == OP_POLICY_ENT) loss -= A.ent_coef * H;
-        const float wm = in.w * A.sc.m;
-        c.ct = wm * g;
-        c.ca = wm * (OP == OP_POLICY_ENT ? A.ent_coef * H - g : -g);
-        c.cb = OP == OP_POLICY_ENT ? wm * A.ent_coef * LN2 : 0.0f;
+        const double ent = OP == OP_POLICY_ENT ? (double)A.ent_coef : 0.0, wm = (double)in.w * A.sc.md;
+        if (OP == OP_POLICY_ENT) loss -= ent * H;
+        c.ct = (float)(wm * token_slope(lp, H, g, -ent)) * in.slope;
+        c.ca = (float)(wm * (OP == OP_POLICY_ENT ? ent * H - g : -g));
+        c.cb = OP == OP_POLICY_ENT ? (float)(wm * ent * LN2_D) : 0.0f;
     }
     if (write) {
-        if (is_policy(OP)) A.row_loss[row] = loss;
+        if (is_policy(OP)) A.row_loss[row] = (float)loss;
         if (A.logprobs) A.logprobs[row] = (float)lp;
-        if (A.entropy) A.entropy[row] = H;
-        if (A.kl) A.kl[row] = kl;
-        if (A.stats) A.stats[row] = make_float2(st.m, (float)(LN2_D * l2s));
+        if (A.entropy) A.entropy[row] = (float)H;
+        if (A.kl) A.kl[row] = (float)kl;
+        if (A.stats) A.stats[row] = make_float2(st.m, (float)ln_s);
     }
     return c;
 }
@@ -628,7 +638,7 @@ __device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, cons
     }
     if (write) A.row_loss[row] = (float)(LN2_D * loss);
     const float wm = w * A.sc.m;
-    return Coef{st.m, (float)l2s, wm * ((float)mass - share), 0.0f, 0.0f, wm * (float)mass, wm, 0.0f, 1u};
+    return Coef{st.m, (float)l2s, wm * ((float)mass - share), 0.0f, 0.0f, wm * (float)mass, wm, 1u};
 }
 
 template <typename T, int OP, bool CAP>
@@ -827,8 +837,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     // is a single element, warp A has it)
                     const uint32_t t_at = (uint32_t)sh.code[i & 15] - R.lead - sl.c0 * E;
                     const uint32_t t = t_at / E, mine = t < copied ? t : t - copied;
-                    if (t < count && mine % GT == g)
-                        out[t_at] = from_f<T>((gr.one(cf.c_tok) + cf.ct) * slope<CAP>(cf.c_tok, A.sc));
+                    if (t < count && mine % GT == g) out[t_at] = from_f<T>(cf.ct);
                 }
             } else {   // the row is left out: zeros
                 for (uint32_t c = g; c < count; c += GT) store(c, make_uint4(0, 0, 0, 0));
@@ -935,6 +944,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 } else {
                     TokenIn in = cur.in;
                     in.c_tok = c_tok;
+                    in.slope = slope<CAP>(c_tok, A.sc);
                     cf = token_row<OP>(A, row, st, in, write);
                 }
             } else if (write) {
@@ -948,7 +958,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 float o = 0.0f;
                 if (live) {
                     const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
-                    o = (gr.one(c_edge) + (!DIST && edge == sh.code[i & 15] ? cf.ct : 0.0f)) * slope<CAP>(c_edge, A.sc);
+                    o = !DIST && edge == sh.code[i & 15] ? cf.ct : gr.one(c_edge) * slope<CAP>(c_edge, A.sc);
                 }
                 ((T *)A.grad)[(size_t)row * A.ld_grad + edge] = from_f<T>(o);
             }
@@ -1136,6 +1146,10 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
 //   dv_j = m c'(v_j) [g (d_jt - p_j) - h p_j (log p_j + H)]
 // Grid: rows x slices of GRAD_SLICE chunks.  A pure stream, one read and one
 // write a logit: 2048 x 151936 bf16 (1792 rows read) 179 us, the copy bandwidth.
+// The token's element is worked out again in 64 bits (token_slope).
+__device__ __noinline__ float token_grad(const Scale &sc, float c, float2 st, float H, float g, float h) {
+    return (float)(sc.md * token_slope(((double)c - (double)st.x) * sc.md - (double)st.y, H, g, h));
+}
 constexpr int GRAD_BATCH = 4;
 constexpr uint32_t GRAD_SLICE = THREADS * GRAD_BATCH * 2;   // chunks of a CTA
 template <typename T, bool CAP, bool ENT>
@@ -1152,14 +1166,14 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
     const bool live = (uint32_t)tok < V;
     const uint32_t t = ((uint32_t)tok - R.lead) / E;                          // the token's chunk,
     const bool own = live && t - c0 < c1 - c0 && (t - c0) % THREADS == tid;   // and whether this thread has it
-    float m = 0.0f, l2s = 0.0f, g = 0.0f, ca = 0.0f, cb = 0.0f, c_tok = 0.0f;
+    float m = 0.0f, l2s = 0.0f, ca = 0.0f, cb = 0.0f, v_tok = 0.0f;
     const float k = A.sc.k;
     if (live) {
-        if (own) c_tok = capped<CAP>(to_f(R.x[tok]), A.sc);
+        if (own) v_tok = to_f(R.x[tok]);
         const float2 st = stats[row];
         m = st.x;
         l2s = st.y * (float)(1.0 / LN2_D);
-        g = d_lp ? d_lp[row] * A.sc.m : 0.0f;
+        const float g = d_lp ? d_lp[row] * A.sc.m : 0.0f;
         const float h = ENT ? d_ent[row] * A.sc.m : 0.0f;
         ca = ENT ? -g - h * entropy[row] : -g;
         cb = ENT ? -h * LN2 : 0.0f;
@@ -1187,12 +1201,15 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
             if (cu < c1) store(cu, gr.template chunk<T, CAP>(q[u], A.sc));
         }
     }
+    auto at_token = [&](float c) {
+        return token_grad(A.sc, c, stats[row], ENT ? entropy[row] : 0.0f, d_lp ? d_lp[row] : 0.0f, ENT ? d_ent[row] : 0.0f) *
+               slope<CAP>(c, A.sc);
+    };
     // the token's own element, written again by the thread that wrote its chunk
-    if (own) gout[tok] = from_f<T>((gr.one(c_tok) + g) * slope<CAP>(c_tok, A.sc));
+    if (own) gout[tok] = from_f<T>(at_token(capped<CAP>(v_tok, A.sc)));
     if (edge >= 0) {
         const float cv = capped<CAP>(to_f(R.x[edge]), A.sc);
-        const float o = gr.one(cv) + (edge == tok ? g : 0.0f);
-        gout[edge] = from_f<T>(o * slope<CAP>(cv, A.sc));
+        gout[edge] = from_f<T>(edge == tok ? at_token(cv) : gr.one(cv) * slope<CAP>(cv, A.sc));
     }
 }
 
@@ -1695,7 +1712,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
         if (tid == 0) P.lse[row] = (float)((double)st.m * (double)A.sc.m + LN2_D * log2_d(st.s));
         if (P.fused) select_top<T, CAP>(R, row, A.sc, P, ts, keys);
     } else if (tid == 0) {
-        token_row<OP_LOGPROB>(A, row, st, TokenIn{1.0f, 0.0f, 0.0f, 0.0f, capped<CAP>(to_f(v_tok), A.sc)}, true);
+        token_row<OP_LOGPROB>(A, row, st, TokenIn{1.0f, 0.0f, 0.0f, 0.0f, capped<CAP>(to_f(v_tok), A.sc), 1.0f}, true);
     }
 }
 
@@ -1732,6 +1749,7 @@ static bs_status check_logits(const bs_logits *x, Scale *sc, float *out_scale, b
     const double k = m * 1.4426950408889634;
     if (!(k >= 1.2e-38) || !(k <= 3.0e38)) return BS_EINVAL;
     sc->m = (float)m;
+    sc->md = m;
     sc->k = (float)k;
     sc->dk = k / (double)sc->k - 1.0;
     sc->inv_t = 1.0 / (double)x->temperature;
@@ -2058,8 +2076,8 @@ extern "C" bs_status bs_policy_loss(const bs_logits *x, const int32_t *d_tokens,
     A.adv = d_advantages;
     A.ref_lp = d_ref_logprobs;
     A.weights = d_weights;
-    A.clip_lo = 1.0f - cfg->clip_low;
-    A.clip_hi = 1.0f + cfg->clip_high;
+    A.clip_lo = 1.0 - (double)cfg->clip_low;
+    A.clip_hi = 1.0 + (double)cfg->clip_high;
     A.kl_coef = cfg->kl_coef;
     A.ent_coef = cfg->entropy_coef;
     A.row_loss = d_row_loss;
