@@ -471,8 +471,14 @@ struct Coef {
     float m, l2s;        // maximum, log2 S
     float ca, cb;        // dv_j = c'(v_j) p_j (ca + cb log2 p_j)
     float ct;            // the token's dv
-    float q_all, wm;     // teacher's ids: c'(v_j) (p_j q_all - wm q_j)
     uint32_t live;       // 0: the row is left out
+    double lse, q_all, wm;   // teacher's ids: wm c'(v_j) (p_j q_all - q_j), log p_j = (c(v_j) - U) m - lse
+};
+// What the warps B sum of a row's slots, in 64 bits.
+struct Teacher {
+    double cross, mass;  // sum of q (log q - (c - U) m), sum of q
+    float u;             // U: the largest c(v) of the slots
+    uint32_t live;       // 0: no slot, or no share to give
 };
 // Threads of S and G, and of S alone where there is a gradient to write.  The
 // 16-bit types have twice the logits a byte and want more of both: 4096 x 128256
@@ -490,9 +496,10 @@ struct RowsShared {
     Coef coef[4];
     int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
     // B's
-    double scratch_d[BTHREADS / 32];
-    float scratch_f[BTHREADS / 32];
-    uint32_t slots_live[4], edge_marks[4], twice[4];   // twice: an id of the slice comes twice
+    double scratch_d[2][BTHREADS / 32];
+    float scratch_f[3][BTHREADS / 32];
+    Teacher teacher[4];
+    uint32_t edge_marks[4], twice[4];                  // twice: an id of the slice comes twice
     uint64_t mail_bar[4], full_bar[3], slots_bar[4];
 };
 
@@ -566,7 +573,7 @@ __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const 
     const double ln_s = log((double)st.s) + LN2_D * A.sc.dk * ratio;
     const double lp = ((double)in.c_tok - m) * A.sc.md - ln_s;
     const double H = ln_s - LN2_D * (1.0 + A.sc.dk) * ratio;
-    Coef c{st.m, (float)(ln_s / LN2_D), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 1u};
+    Coef c{st.m, (float)(ln_s / LN2_D), 0.0f, 0.0f, 0.0f, 1u, 0.0, 0.0, 0.0};
     double kl = 0.0, loss = 0.0;
     if (is_policy(OP)) {
         const double adv = in.adv, r = exp(lp - (double)in.old_lp);
@@ -600,45 +607,32 @@ __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const 
 
 // The teacher's slots of a row, in one of four sets.
 struct Slots {
+    double *q;        // the slot's share
     int32_t *id;      // -1: empty; padded to a multiple of 4 with empty ones
-    float *q;         // the slot's share
-    float *c;         // the student's c(v) there
+    float *v;         // the student's logit there
     uint32_t *bits;   // one bit per element of the CTA's slice: named by the teacher
 };
+constexpr uint32_t SLOT_BYTES = 16;
 __host__ __device__ __forceinline__ uint32_t slots_padded(uint32_t n_ids) { return (n_ids + 3u) & ~3u; }
 
-// Results and coefficients of a row with a teacher; one warp.
+// Results and coefficients of a row with a teacher, in 64 bits as those of a
+// row with a token: a student near its teacher has a loss near 0, and the rest
+// of the vocabulary the gradient p_j (1 - q_rest / p_rest).
 template <bool TAIL>
-__device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, const Slots &sl, float w, bool write) {
-    const float s = TAIL ? st.s + st.u : st.s;
-    const double l2s = log2_d(s), k_all = (double)A.sc.k * (1.0 + A.sc.dk);
-    // sum q (log q - log p) over the slots, and the rest as one outcome
-    double loss = 0.0, mass = 0.0;
-    for (uint32_t i = threadIdx.x & 31; i < A.n_ids; i += 32) {
-        const float q = sl.q[i];
-        if (sl.id[i] >= 0 && !(q <= 0.0f)) {
-            const double l2p = ((double)sl.c[i] - (double)st.m) * k_all - l2s;
-            loss += (double)q * (log2_d(q) - l2p);
-            mass += (double)q;
+__device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, const Teacher &t, float w, bool write) {
+    const double s = TAIL ? (double)st.s + (double)st.u : (double)st.s, wm = (double)w * A.sc.md;
+    const double ln_s = log(s), lse = ((double)st.m - (double)anchor(t.u)) * A.sc.md + ln_s;   // relative to U
+    double loss = t.cross + t.mass * lse, mass = t.mass, share = 0.0;
+    if (TAIL) {   // the rest as one outcome
+        const double qr = 1.0 - mass;
+        if (!(qr <= 0.0) && !(st.s == 0.0f)) {
+            loss += qr * (log(qr) - log((double)st.s) + ln_s);
+            mass += qr;
+            share = qr * s / (double)st.s;
         }
     }
-    for (int o = 16; o; o >>= 1) {
-        loss += __shfl_xor_sync(~0u, loss, o);
-        mass += __shfl_xor_sync(~0u, mass, o);
-    }
-    float share = 0.0f;
-    if (TAIL) {
-        const float qr = mass >= 1.0 ? 0.0f : (float)(1.0 - mass);
-        if (!(qr <= 0.0f) && !(st.s == 0.0f)) {
-            const double l2r = log2_d(st.s) - l2s;
-            loss += (double)qr * (log2_d(qr) - l2r);
-            mass += (double)qr;
-            share = (float)((double)qr * (double)s / (double)st.s);
-        }
-    }
-    if (write) A.row_loss[row] = (float)(LN2_D * loss);
-    const float wm = w * A.sc.m;
-    return Coef{st.m, (float)l2s, wm * ((float)mass - share), 0.0f, 0.0f, wm * (float)mass, wm, 1u};
+    if (write) A.row_loss[row] = (float)loss;
+    return Coef{st.m, (float)(ln_s / LN2_D), (float)(wm * (mass - share)), 0.0f, 0.0f, 1u, lse, mass, wm};
 }
 
 template <typename T, int OP, bool CAP>
@@ -677,10 +671,10 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         const uint32_t set = i & 3;
         char *base = (char *)(dyn + 3 * (size_t)A.keep);
         Slots s;
-        s.id = (int32_t *)base + set * pad;
-        s.q = (float *)base + (4 + set) * pad;
-        s.c = (float *)base + (8 + set) * pad;
-        s.bits = (uint32_t *)base + 12 * pad + set * A.bit_words;
+        s.q = (double *)base + set * pad;
+        s.id = (int32_t *)base + (8 + set) * pad;
+        s.v = (float *)base + (12 + set) * pad;
+        s.bits = (uint32_t *)base + 16 * pad + set * A.bit_words;
         return s;
     };
 
@@ -891,7 +885,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             load4(i + 2);
             bar_sync(BAR_X + (i & 3), x_threads);
             bool live = sh.code[i & 15] >= 0;
-            if (DIST && live) live = sh.slots_live[i & 3] != 0u;
+            if (DIST && live) live = sh.teacher[i & 3].live != 0u;
             const int32_t edge = edge_of(i);
             const float c_edge = capped<CAP>(to_f(cur.edge), A.sc);
             const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(cur.tok), A.sc);
@@ -940,7 +934,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             Coef cf{};
             if (live) {
                 if constexpr (DIST) {
-                    cf = teacher_row<TAIL>(A, row, st, slots(i), cur.in.w, write);
+                    cf = teacher_row<TAIL>(A, row, st, sh.teacher[i & 3], cur.in.w, write);
                 } else {
                     TokenIn in = cur.in;
                     in.c_tok = c_tok;
@@ -990,13 +984,33 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     } else if constexpr (DIST) {
         // ---- warps B
         const uint32_t b = tid - COMPUTE - 96;
-        auto b_max = [&](float v) {   // (a NaN stays)
-            for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+        // over the threads of B: the largest of three values each (a NaN stays), the sums of two
+        auto b_max = [&](float (&v)[3]) {
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                for (int o = 16; o; o >>= 1) v[e] = max_nan(v[e], __shfl_xor_sync(~0u, v[e], o));
             bar_sync(BAR_B, BTHREADS);
-            if (lane == 0) sh.scratch_f[b >> 5] = v;
+            if (lane == 0) {
+#pragma unroll
+                for (int e = 0; e < 3; e++) sh.scratch_f[e][b >> 5] = v[e];
+            }
             bar_sync(BAR_B, BTHREADS);
-            for (int i = 0; i < BTHREADS / 32; i++) v = max_nan(v, sh.scratch_f[i]);
-            return v;
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                for (int i = 0; i < BTHREADS / 32; i++) v[e] = max_nan(v[e], sh.scratch_f[e][i]);
+        };
+        auto b_sum = [&](double (&v)[2]) {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                for (int o = 16; o; o >>= 1) v[e] += __shfl_xor_sync(~0u, v[e], o);
+            bar_sync(BAR_B, BTHREADS);
+            if (lane == 0) sh.scratch_d[0][b >> 5] = v[0], sh.scratch_d[1][b >> 5] = v[1];
+            bar_sync(BAR_B, BTHREADS);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                v[e] = 0.0;
+                for (int i = 0; i < BTHREADS / 32; i++) v[e] += sh.scratch_d[e][i];
+            }
         };
         // Loads of a row ahead of their use: its weight, lse and (first of a thread) slot two iterations, the
         // student's logit there one.
@@ -1034,7 +1048,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             two = fetch(i + 2);
             fetch_logit(i + 1);
             const bool wanted = cur.w != 0.0f;
-            float umax = -INFINITY, any = 0.0f;
+            float most[3] = {0.0f, -INFINITY, -INFINITY};   // (whether there is a slot), teacher's logit, c(v)
             if (b == 0) sh.edge_marks[set] = sh.twice[set] = 0u;
             if (wanted) {
                 for (uint32_t j = b; j < pad; j += BTHREADS) {
@@ -1046,27 +1060,30 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     }
                     if ((uint32_t)id >= V) id = -1;
                     sl.id[j] = id;
-                    sl.q[j] = t;
+                    sl.q[j] = (double)t;
                     if (id >= 0) {
-                        sl.c[j] = capped<CAP>(to_f(j == b ? cur_logit : R.x[id]), A.sc);
-                        any = 1.0f;
-                        umax = max_nan(umax, t);
+                        const float v = to_f(j == b ? cur_logit : R.x[id]);
+                        sl.v[j] = v;
+                        most[0] = 1.0f;
+                        most[1] = max_nan(most[1], t);
+                        most[2] = max_nan(most[2], capped<CAP>(v, A.sc));
                     }
                 }
+                b_max(most);
             }
-            bool live = wanted && b_max(any) != 0.0f;   // (the same in all threads)
-            if (!TAIL && live) {
-                umax = b_max(umax);
-                live = live && umax != -INFINITY;   // no share to give: as without ids
-            }
+            // (the same in all threads; without a teacher's lse there may be no share to give: as without ids)
+            const bool live = wanted && most[0] != 0.0f && (TAIL || most[1] != -INFINITY);
             if (live) {
-                const double ref = TAIL ? (double)cur.lse : (double)umax * A.sc.inv_t;
-                double sum = 0.0;
+                const double ref = TAIL ? (double)cur.lse : (double)most[1] * A.sc.inv_t, u = (double)anchor(most[2]);
+                double sum[2] = {0.0, 0.0};   // of q, of q (log q - (c - U) m); q not yet divided by its sum
                 for (uint32_t j = b; j < pad; j += BTHREADS) {
                     const int32_t id = sl.id[j];
-                    const float q = id < 0 ? 0.0f : expf((float)((double)sl.q[j] * A.sc.inv_t - ref));
+                    const double a = sl.q[j] * A.sc.inv_t - ref, q = id < 0 ? 0.0 : exp(a);
                     sl.q[j] = q;
-                    sum += (double)q;
+                    if (!(q <= 0.0)) {
+                        sum[0] += q;
+                        sum[1] += q * (a - ((double)capped<CAP>(sl.v[j], A.sc) - u) * A.sc.md);
+                    }
                     if (id >= 0) {
                         const uint32_t e = (uint32_t)id - e0;
                         uint32_t *word = &sl.bits[e >> 5], bit = 1u << (e & 31);
@@ -1077,17 +1094,16 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                         if (bit && (atomicOr(word, bit) & bit)) sh.twice[set] = 1u;
                     }
                 }
+                b_sum(sum);
                 if (!TAIL) {
-                    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-                    bar_sync(BAR_B, BTHREADS);
-                    if (lane == 0) sh.scratch_d[b >> 5] = sum;
-                    bar_sync(BAR_B, BTHREADS);
-                    sum = 0.0;
-                    for (int j = 0; j < BTHREADS / 32; j++) sum += sh.scratch_d[j];
-                    for (uint32_t j = b; j < pad; j += BTHREADS) sl.q[j] /= (float)sum;
+                    for (uint32_t j = b; j < pad; j += BTHREADS) sl.q[j] /= sum[0];
+                    sum[1] = sum[1] / sum[0] - log(sum[0]);
+                    sum[0] /= sum[0];   // 1, or NaN
                 }
+                if (b == 0) sh.teacher[set] = Teacher{sum[1], sum[0], most[2], 1u};
+            } else if (b == 0) {
+                sh.teacher[set].live = 0u;
             }
-            if (b == 0) sh.slots_live[set] = live ? 1u : 0u;
         };
         auto finish = [&](uint32_t i) {
             const uint32_t row = row_of(i), set = i & 3;
@@ -1096,7 +1112,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             const Row<T> R(A.x, A.ld, row, V);
             const Slice part = slice_of(R);
             const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
-            if (!sh.slots_live[set]) return;
+            if (!sh.teacher[set].live) return;
+            const double u = (double)anchor(sh.teacher[set].u);
             const bool twice = sh.twice[set] != 0u;
             T *out = (T *)A.grad + (size_t)row * A.ld_grad;
             for (uint32_t j = b; j < A.n_ids; j += BTHREADS) {
@@ -1108,9 +1125,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 if (!single) sl.bits[e >> 5] = 0u;
                 if (!grad) continue;
                 // p Q - q, where q is the sum over the slots that hold the id (the first of them writes)
-                float q = sl.q[j];
+                double q = sl.q[j];
                 bool first = true;
-                if (twice) q = 0.0f;
+                if (twice) q = 0.0;
                 for (uint32_t o = 0; twice && o < pad; o += 4) {
                     const int4 v = *reinterpret_cast<const int4 *>(sl.id + o);
                     if (v.x == id) q += sl.q[o], first = first && o >= j;
@@ -1119,8 +1136,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     if (v.w == id) q += sl.q[o + 3], first = first && o + 3 >= j;
                 }
                 if (!first) continue;
-                const float p = ex2(fmaf(sl.c[j] - cf.m, k, -cf.l2s));
-                out[id] = from_f<T>((p * cf.q_all - cf.wm * q) * slope<CAP>(sl.c[j], A.sc));
+                const float c = capped<CAP>(sl.v[j], A.sc);
+                const double p = exp(((double)c - u) * A.sc.md - cf.lse);
+                out[id] = from_f<T>((float)(cf.wm * (p * cf.q_all - q)) * slope<CAP>(c, A.sc));
             }
         };
         one = fetch(0);
@@ -1919,7 +1937,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     for (;; ranks *= 2, log_ranks++) {
         slice = (chunks + ranks - 1) / ranks;
         A.bit_words = is_distill(OP) ? (slice * E + 31) / 32 : 0;
-        slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 48 + (size_t)A.bit_words * 16 : 0;
+        slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 4 * SLOT_BYTES + (size_t)A.bit_words * 16 : 0;
         room = slots < ROWS_SMEM ? (ROWS_SMEM - slots) / 48 : 0;
         // Enough CTAs to hold the row, and to use the GPU where the rows are few.  Sixteen only where eight cannot
         // hold it (seven such clusters fit the GPU, 112 SMs): 512 x 256000 f32 424 us, with eight and the rest of

@@ -70,3 +70,58 @@ def test_gradient_at_a_likely_token(gpu_pkg, gap, vocab):
     ratio = (-math.log1p(rest) - old.double().cpu()).exp()
     p = gpu_pkg.policy_loss(x, t, old, torch.ones(3, device="cuda"), None, w, temperature=T)
     relative(p.grad[:, 0], -ratio * w.double().cpu() * p_other / T, 3 * EPS, "gradient of the policy loss")
+
+
+def uniform_distill(vocab, ids, tl, lse, T, w):
+    """Loss and gradient of one equal-logits row, 64 bits, from the f32 inputs."""
+    logp = -math.log(vocab)
+    u = tl.double() / T
+    logq = u - torch.logsumexp(u, 0) if lse is None else u - float(lse)
+    q = logq.exp()
+    loss = (q * (logq - logp)).sum()
+    p = 1.0 / vocab
+    grad = torch.full((vocab,), p, dtype=torch.float64)
+    if lse is not None:
+        qr, pr = 1 - q.sum(), (vocab - len(ids)) / vocab
+        loss = loss + qr * (qr.log() - math.log(pr))
+        grad = grad - qr / pr * p
+        grad[ids.long()] = p
+    grad[ids.long()] -= q
+    return loss, w * grad / T
+
+
+@pytest.mark.parametrize("vocab,K", [(64, 64), (4096, 8), (4096, 130), (131072, 1024)])
+@pytest.mark.parametrize("tail", [False, True], ids=["slots", "tail"])
+@pytest.mark.parametrize("near", [1e-1, 1e-3])
+def test_student_near_its_teacher(gpu_pkg, vocab, K, tail, near):
+    # equal logits again, and a teacher whose shares differ from the student's by `near`.  With T = 1 and 2 nothing but
+    # the inputs is rounded before the results.  The loss is near^2 / 2 of the named mass in size, worked out from terms of
+    # q |log q|: some 2^-50 of their sum beside the rounding.
+    if tail and K == vocab:
+        pytest.skip("no rest")
+    g = torch.Generator().manual_seed(171)
+    for T in (1.0, 2.0):
+        x = torch.full((2, vocab), -0.75, device="cuda")
+        ids = torch.randperm(vocab, generator=g)[:K].int()
+        tl = near * torch.randn(K, generator=g)
+        lse = torch.tensor(math.log(vocab) + near).float() if tail else None
+        w = 0.5
+        want, grad = uniform_distill(vocab, ids, tl, lse, T, w)
+        both = lambda v: torch.stack([v, v]).cuda()  # noqa: E731
+        got = gpu_pkg.distill_loss(x, both(ids), both(tl), both(lse) if tail else None, torch.full((2,), w, device="cuda"),
+                                   temperature=T)
+        big = max(1.0, math.log(vocab))
+        relative(got.row_losses, [want] * 2, EPS + 2.0**-50 * big / float(want), "rows")
+        at = ids.long()
+        # p - q in 64 bits: one rounding, and 2^-50 of p over the difference
+        few = grad[at].abs() > 1e-9 / vocab
+        relative(got.grad[:, at.cuda()][0][few.cuda()], grad[at][few],
+                 1.01 * EPS + 2.0**-48 / vocab / float(grad[at][few].abs().min()), "named tokens")
+        rest = torch.ones(vocab, dtype=torch.bool)
+        rest[at] = False
+        if rest.any():
+            # 2^l of l = -log2 S: l rounded twice to f32 (2 |l| EPS ln 2), ex2 2^-22, the coefficient and the result; the
+            # coefficient's 64 bits lose 2^-50 over 1 - q_rest / p_rest
+            l2s = math.log2(vocab)
+            tol = EPS * (2 * l2s * math.log(2.0) + 4 + 2) + (2.0**-50 * vocab / float(grad[rest].abs().min()) / vocab if tail else 0)
+            relative(got.grad[:, rest.cuda()], grad[rest].expand(2, -1), tol, "rest")
