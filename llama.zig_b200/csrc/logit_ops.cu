@@ -420,14 +420,17 @@ template <bool ENT> struct GradRow {
 //                       before and behind the 16-byte chunks,
 //   warps G             write the gradient (without one, these sum too),
 //   warp C              starts the copy of row i + 3 into row i's buffer,
-//   warps B             losses with a teacher: prepare the slots of the rows
-//                       to come (shares q, the student's logits there), and
-//                       after row i's gradient write the tokens that its
-//                       teacher names.
+//   warps B             losses with a teacher (four, one for each set of slots,
+//                       with every fourth row): prepare a row's slots (shares
+//                       q, the student's logits there) and, after the row's
+//                       gradient, write the tokens that its teacher names.
 //
 // Summing and gradient each need one ex2 a logit, so half of the warps do
 // either, and the special-function unit always has work while a row's sums
-// travel.  Barriers, in as many copies as rows can be between the two sides:
+// travel.  A warp that shares the SM with these issues an instruction in some
+// ten cycles, so B's 64-bit work is spread over four rows and meets no barrier
+// of its own: with the four warps together on one row 512 x 256000 f32 with 128
+// ids took 262 us, so 208; 4000 x 8000 bf16 with 64 ids 71 and 75.  Barriers, in as many copies as rows can be between the two sides:
 // X (S -> A: row i summed), Y (A -> G: its coefficients), Z (-> C, B: done
 // with; from G, or without a gradient from S and A); and mbarriers: full_bar
 // (copy -> S), slots_bar (B -> S), mail_bar (A -> A of the other CTAs).
@@ -447,8 +450,9 @@ template <bool ENT> struct GradRow {
 constexpr uint32_t COPY = 512;       // chunks of one copy
 constexpr int STEP = 4;              // chunks of a thread summed at a time
 constexpr int MAX_CWARPS = 24;       // most warps S and G together
-constexpr int BTHREADS = 128;
-enum Bar { BAR_X = 1, BAR_Y = 5, BAR_Z = 9, BAR_B = 13 };
+constexpr int BTHREADS = 128;        // a warp for each of the four sets of slots
+constexpr int AHEAD = 4;             // slots of a lane that are loaded ahead
+enum Bar { BAR_X = 1, BAR_Y = 5, BAR_Z = 9 };
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -477,6 +481,7 @@ struct Coef {
 // What the warps B sum of a row's slots, in 64 bits.
 struct Teacher {
     double cross, mass;  // sum of q (log q - (c - U) m), sum of q
+    double scale;        // q = scale x what the slots hold
     float u;             // U: the largest c(v) of the slots
     uint32_t live;       // 0: no slot, or no share to give
 };
@@ -495,11 +500,8 @@ struct RowsShared {
     float4 mail[4][MAX_CLUSTER];     // and of the row's CTAs; two for each warp A
     Coef coef[4];
     int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
-    // B's
-    double scratch_d[2][BTHREADS / 32];
-    float scratch_f[3][BTHREADS / 32];
     Teacher teacher[4];
-    uint32_t edge_marks[4], twice[4];                  // twice: an id of the slice comes twice
+    uint32_t edge_marks[4];          // the teacher's ids among the row's single elements
     uint64_t mail_bar[4], full_bar[3], slots_bar[4];
 };
 
@@ -561,37 +563,52 @@ struct TokenIn {
     float slope;         // the soft-cap's, at the token
 };
 // The gradient at the token itself, before the soft-cap's slope, from those of
-// log-probability and entropy: g (1 - p) - h p (log p + H).  1 - p is -expm1
-// of log p, whose bits a p near 1 in f32 has lost.
-__device__ __forceinline__ double token_slope(double lp, double H, double g, double h) {
-    return -g * expm1(lp) - (h != 0.0 ? h * exp(lp) * (fmax(lp, -1e4) + H) : 0.0);
+// log-probability and entropy: g (1 - p) - h p (log p + H), with 1 - p as
+// -expm1(log p), whose bits a p near 1 in f32 has lost.
+__device__ __forceinline__ double token_slope(double lp, double pm1, double H, double g, double h) {
+    return -g * pm1 - (h != 0.0 ? h * (1.0 + pm1) * (fmax(lp, -1e4) + H) : 0.0);
+}
+// The exchange between a row's sums and its gradient waits for these few
+// values, so a warp works them out side by side: lane e has the function at the
+// e-th argument, and every lane gets all results.
+template <int N> __device__ __forceinline__ void by_lanes(double (&v)[N], double (*f)(double)) {
+    double mine = v[0];
+#pragma unroll
+    for (int e = 1; e < N; e++) mine = (threadIdx.x & 31) == e ? v[e] : mine;
+    mine = f(mine);
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e] = __shfl_sync(~0u, mine, e);
 }
 template <int OP>
 __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const Stat &st, const TokenIn &in, bool write) {
-    const double m = st.m, ratio = (double)st.u / (double)st.s;
+    // (u / s by one Newton step on the f32 reciprocal: 2^-46)
+    const double m = st.m, rs = (double)(1.0f / st.s), ratio = (double)st.u * (rs * (2.0 - (double)st.s * rs));
     // k is m log2 e in f32: to first order, what its rounding did to the sum
     const double ln_s = log((double)st.s) + LN2_D * A.sc.dk * ratio;
     const double lp = ((double)in.c_tok - m) * A.sc.md - ln_s;
     const double H = ln_s - LN2_D * (1.0 + A.sc.dk) * ratio;
-    Coef c{st.m, (float)(ln_s / LN2_D), 0.0f, 0.0f, 0.0f, 1u, 0.0, 0.0, 0.0};
+    Coef c{st.m, (float)(ln_s * (1.0 / LN2_D)), 0.0f, 0.0f, 0.0f, 1u, 0.0, 0.0, 0.0};
     double kl = 0.0, loss = 0.0;
     if (is_policy(OP)) {
-        const double adv = in.adv, r = exp(lp - (double)in.old_lp);
+        const double adv = in.adv, dr = (double)in.ref_lp - lp;
+        double x1[3] = {lp - (double)in.old_lp, dr, lp};
+        by_lanes(x1, [](double v) { return expm1(v); });
+        // (1 + expm1 has the exponential's bits but where it is small)
+        const double r = x1[0] < -0.5 ? exp(lp - (double)in.old_lp) : 1.0 + x1[0];
         // min(r A, clip(r) A) is the clipped one only beyond the bound that A favours
         const bool over = adv > 0.0 && r > A.clip_hi, under = adv < 0.0 && r < A.clip_lo;
         loss = -adv * (over ? A.clip_hi : under ? A.clip_lo : r);
         double g = over || under ? 0.0 : -r * adv;
         if (A.ref_lp) {
-            const double dr = (double)in.ref_lp - lp, x1 = expm1(dr);
-            kl = x1 - dr;
+            kl = x1[1] - dr;
             if (A.kl_coef != 0.0f) {
                 loss += (double)A.kl_coef * kl;
-                g -= (double)A.kl_coef * x1;
+                g -= (double)A.kl_coef * x1[1];
             }
         }
         const double ent = OP == OP_POLICY_ENT ? (double)A.ent_coef : 0.0, wm = (double)in.w * A.sc.md;
         if (OP == OP_POLICY_ENT) loss -= ent * H;
-        c.ct = (float)(wm * token_slope(lp, H, g, -ent)) * in.slope;
+        c.ct = (float)(wm * token_slope(lp, x1[2], H, g, -ent)) * in.slope;
         c.ca = (float)(wm * (OP == OP_POLICY_ENT ? ent * H - g : -g));
         c.cb = OP == OP_POLICY_ENT ? (float)(wm * ent * LN2_D) : 0.0f;
     }
@@ -607,7 +624,7 @@ __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const 
 
 // The teacher's slots of a row, in one of four sets.
 struct Slots {
-    double *q;        // the slot's share
+    double *q;        // the slot's share, but for the row's scale
     int32_t *id;      // -1: empty; padded to a multiple of 4 with empty ones
     float *v;         // the student's logit there
     uint32_t *bits;   // one bit per element of the CTA's slice: named by the teacher
@@ -621,18 +638,21 @@ __host__ __device__ __forceinline__ uint32_t slots_padded(uint32_t n_ids) { retu
 template <bool TAIL>
 __device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, const Teacher &t, float w, bool write) {
     const double s = TAIL ? (double)st.s + (double)st.u : (double)st.s, wm = (double)w * A.sc.md;
-    const double ln_s = log(s), lse = ((double)st.m - (double)anchor(t.u)) * A.sc.md + ln_s;   // relative to U
+    const double qr = 1.0 - t.mass;
+    double ln[3] = {s, (double)st.s, qr};
+    if (TAIL) by_lanes(ln, [](double v) { return log(v); });
+    else ln[0] = log(s);
+    const double ln_s = ln[0], lse = ((double)st.m - (double)anchor(t.u)) * A.sc.md + ln_s;   // relative to U
     double loss = t.cross + t.mass * lse, mass = t.mass, share = 0.0;
     if (TAIL) {   // the rest as one outcome
-        const double qr = 1.0 - mass;
         if (!(qr <= 0.0) && !(st.s == 0.0f)) {
-            loss += qr * (log(qr) - log((double)st.s) + ln_s);
+            loss += qr * (ln[2] - ln[1] + ln_s);
             mass += qr;
             share = qr * s / (double)st.s;
         }
     }
     if (write) A.row_loss[row] = (float)loss;
-    return Coef{st.m, (float)(ln_s / LN2_D), (float)(wm * (mass - share)), 0.0f, 0.0f, 1u, lse, mass, wm};
+    return Coef{st.m, (float)(ln_s * (1.0 / LN2_D)), (float)(wm * (mass - share)), 0.0f, 0.0f, 1u, lse, mass, wm};
 }
 
 template <typename T, int OP, bool CAP>
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     constexpr uint32_t ST = sum_threads_of<T, CAP>(), GT = COMPUTE - ST;
     const uint32_t sum_threads = grad ? ST : COMPUTE, x_threads = sum_threads + 32;
     const uint32_t y_threads = GT + 32;
-    const uint32_t z_threads = (grad ? GT : COMPUTE + 32) + 32 + (DIST ? BTHREADS : 0);
+    const uint32_t z_threads = (grad ? GT : COMPUTE + 32) + 32 + (DIST ? 32 : 0);
     // f32 logits under a soft-cap: S leaves c(v) in the buffer, so that G need not work it out again
     constexpr bool LEAVE = CAP && sizeof(T) == 4;
     auto row_of = [&](uint32_t i) { return cluster + i * clusters; };
@@ -982,141 +1002,130 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         // (S has seen every copy land; were it to have given up on one, it still lands before the CTA's memory goes)
         for (uint32_t i = n > 3 ? n - 3 : 0; i < n; i++) bar_wait(&sh.full_bar[i % 3], i / 3 & 1);
     } else if constexpr (DIST) {
-        // ---- warps B
-        const uint32_t b = tid - COMPUTE - 96;
-        // over the threads of B: the largest of three values each (a NaN stays), the sums of two
-        auto b_max = [&](float (&v)[3]) {
-#pragma unroll
-            for (int e = 0; e < 3; e++)
-                for (int o = 16; o; o >>= 1) v[e] = max_nan(v[e], __shfl_xor_sync(~0u, v[e], o));
-            bar_sync(BAR_B, BTHREADS);
-            if (lane == 0) {
-#pragma unroll
-                for (int e = 0; e < 3; e++) sh.scratch_f[e][b >> 5] = v[e];
-            }
-            bar_sync(BAR_B, BTHREADS);
-#pragma unroll
-            for (int e = 0; e < 3; e++)
-                for (int i = 0; i < BTHREADS / 32; i++) v[e] = max_nan(v[e], sh.scratch_f[e][i]);
+        // ---- warps B; warp w has the rows w, w + 4, ..., and the set w of slots
+        const uint32_t set = (tid - COMPUTE - 96) >> 5;
+        const Slots sl = slots(set);
+        // (f32 as a whole number of the same order; a NaN is the largest, 0 is below all)
+        auto order = [](float v) {
+            const uint32_t u = __float_as_uint(v);
+            return v != v ? ~0u : u & 0x80000000u ? ~u : u | 0x80000000u;
         };
-        auto b_sum = [&](double (&v)[2]) {
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                for (int o = 16; o; o >>= 1) v[e] += __shfl_xor_sync(~0u, v[e], o);
-            bar_sync(BAR_B, BTHREADS);
-            if (lane == 0) sh.scratch_d[0][b >> 5] = v[0], sh.scratch_d[1][b >> 5] = v[1];
-            bar_sync(BAR_B, BTHREADS);
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                v[e] = 0.0;
-                for (int i = 0; i < BTHREADS / 32; i++) v[e] += sh.scratch_d[e][i];
-            }
+        auto value = [](uint32_t key) {
+            return key == ~0u ? NAN : __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
         };
-        // Loads of a row ahead of their use: its weight, lse and (first of a thread) slot two iterations, the
-        // student's logit there one.
+        // A row's weight and lse and a lane's first slots, loaded while the row four before is worked on; the student's
+        // logits there once the ids have come.
         struct Ahead {
-            float w, lse, t;
-            int32_t id;
-        } one{}, two{};
-        T logit{};
-        auto fetch = [&](uint32_t i) {
-            Ahead f{0.0f, 0.0f, 0.0f, -1};
-            if (i < n) {
-                const uint32_t row = row_of(i);
-                f.w = weight(row);
-                if (TAIL) f.lse = A.t_lse[row];
-                if (b < A.n_ids) {
-                    f.id = A.t_ids[(size_t)row * A.n_ids + b];
-                    f.t = A.t_logits[(size_t)row * A.n_ids + b];
+            float w, lse, t[AHEAD];
+            int32_t id[AHEAD];
+            T x[AHEAD];
+        } f;
+        auto fetch_slots = [&](uint32_t row, uint32_t j0) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++) {
+                const uint32_t j = j0 + lane + 32 * a;
+                f.id[a] = -1;
+                if (j < A.n_ids) {
+                    f.id[a] = A.t_ids[(size_t)row * A.n_ids + j];
+                    f.t[a] = A.t_logits[(size_t)row * A.n_ids + j];
                 }
             }
-            return f;
         };
-        auto fetch_logit = [&](uint32_t i) {
-            if (i < n && one.w != 0.0f && (uint32_t)one.id < V) logit = ((const T *)A.x)[(size_t)row_of(i) * A.ld + one.id];
+        auto fetch_logits = [&](uint32_t row) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if ((uint32_t)f.id[a] < V) f.x[a] = ((const T *)A.x)[(size_t)row * A.ld + (uint32_t)f.id[a]];
         };
+        auto fetch = [&](uint32_t i) {
+            if (i < n) {
+                f.w = weight(row_of(i));
+                if (TAIL) f.lse = A.t_lse[row_of(i)];
+                fetch_slots(row_of(i), 0);
+            }
+        };
+        auto fetch_row_logits = [&](uint32_t i) {
+            if (i < n && f.w != 0.0f) fetch_logits(row_of(i));
+        };
+        bool twice = false;   // an id of the slice comes twice
         auto prepare = [&](uint32_t i) {
-            const uint32_t row = row_of(i), set = i & 3;
-            const size_t at = (size_t)row * A.n_ids;
-            const Slots sl = slots(i);
+            const uint32_t row = row_of(i);
             const Row<T> R(A.x, A.ld, row, V);
             const Slice part = slice_of(R);
             const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
-            const Ahead cur = one;
-            const T cur_logit = logit;
-            one = two;
-            two = fetch(i + 2);
-            fetch_logit(i + 1);
-            const bool wanted = cur.w != 0.0f;
-            float most[3] = {0.0f, -INFINITY, -INFINITY};   // (whether there is a slot), teacher's logit, c(v)
-            if (b == 0) sh.edge_marks[set] = sh.twice[set] = 0u;
+            const bool wanted = f.w != 0.0f;
+            uint32_t most_t = 0u, most_c = 0u;   // the largest of the teacher's logits and of c(v); 0 without a slot
+            if (lane == 0) sh.edge_marks[set] = 0u;
             if (wanted) {
-                for (uint32_t j = b; j < pad; j += BTHREADS) {
-                    int32_t id = -1;
-                    float t = 0.0f;
-                    if (j < A.n_ids) {
-                        id = j == b ? cur.id : A.t_ids[at + j];
-                        t = j == b ? cur.t : A.t_logits[at + j];
+                for (uint32_t j0 = 0; j0 < pad; j0 += 32 * AHEAD) {
+                    if (j0) {
+                        fetch_slots(row, j0);
+                        fetch_logits(row);
                     }
-                    if ((uint32_t)id >= V) id = -1;
-                    sl.id[j] = id;
-                    sl.q[j] = (double)t;
-                    if (id >= 0) {
-                        const float v = to_f(j == b ? cur_logit : R.x[id]);
-                        sl.v[j] = v;
-                        most[0] = 1.0f;
-                        most[1] = max_nan(most[1], t);
-                        most[2] = max_nan(most[2], capped<CAP>(v, A.sc));
+#pragma unroll
+                    for (int a = 0; a < AHEAD; a++) {
+                        const uint32_t j = j0 + lane + 32 * a;
+                        if (j >= pad) continue;
+                        const bool valid = (uint32_t)f.id[a] < V;
+                        sl.id[j] = valid ? f.id[a] : -1;
+                        if (valid) {
+                            const float v = to_f(f.x[a]);
+                            sl.q[j] = (double)f.t[a];
+                            sl.v[j] = v;
+                            most_t = max(most_t, order(f.t[a]));
+                            most_c = max(most_c, order(capped<CAP>(v, A.sc)));
+                        }
                     }
                 }
-                b_max(most);
+                most_t = __reduce_max_sync(~0u, most_t);
+                most_c = __reduce_max_sync(~0u, most_c);
             }
-            // (the same in all threads; without a teacher's lse there may be no share to give: as without ids)
-            const bool live = wanted && most[0] != 0.0f && (TAIL || most[1] != -INFINITY);
+            __syncwarp();
+            // (without a teacher's lse there may be no share to give: as without ids)
+            const bool live = wanted && most_c != 0u && (TAIL || most_t != order(-INFINITY));
             if (live) {
-                const double ref = TAIL ? (double)cur.lse : (double)most[1] * A.sc.inv_t, u = (double)anchor(most[2]);
-                double sum[2] = {0.0, 0.0};   // of q, of q (log q - (c - U) m); q not yet divided by its sum
-                for (uint32_t j = b; j < pad; j += BTHREADS) {
+                const double ref = TAIL ? (double)f.lse : (double)value(most_t) * A.sc.inv_t, u = (double)anchor(value(most_c));
+                double sum = 0.0, cross = 0.0;   // of q, of q (log q - (c - U) m); without an lse, q is not yet divided by its sum
+                bool again = false;
+                for (uint32_t j = lane; j < pad; j += 32) {
                     const int32_t id = sl.id[j];
-                    const double a = sl.q[j] * A.sc.inv_t - ref, q = id < 0 ? 0.0 : exp(a);
+                    if (id < 0) continue;
+                    const double a = sl.q[j] * A.sc.inv_t - ref, q = exp(a);
                     sl.q[j] = q;
                     if (!(q <= 0.0)) {
-                        sum[0] += q;
-                        sum[1] += q * (a - ((double)capped<CAP>(sl.v[j], A.sc) - u) * A.sc.md);
+                        sum += q;
+                        cross += q * (a - ((double)capped<CAP>(sl.v[j], A.sc) - u) * A.sc.md);
                     }
-                    if (id >= 0) {
-                        const uint32_t e = (uint32_t)id - e0;
-                        uint32_t *word = &sl.bits[e >> 5], bit = 1u << (e & 31);
-                        if (e >= span) {
-                            word = &sh.edge_marks[set];
-                            bit = (uint32_t)id < R.lead ? 1u << id : (uint32_t)id >= V - R.trail ? 256u << (id - (V - R.trail)) : 0u;
-                        }
-                        if (bit && (atomicOr(word, bit) & bit)) sh.twice[set] = 1u;
+                    const uint32_t e = (uint32_t)id - e0;
+                    uint32_t *word = &sl.bits[e >> 5], bit = 1u << (e & 31);
+                    if (e >= span) {
+                        word = &sh.edge_marks[set];
+                        bit = (uint32_t)id < R.lead ? 1u << id : (uint32_t)id >= V - R.trail ? 256u << (id - (V - R.trail)) : 0u;
                     }
+                    if (bit && (atomicOr(word, bit) & bit)) again = true;
                 }
-                b_sum(sum);
-                if (!TAIL) {
-                    for (uint32_t j = b; j < pad; j += BTHREADS) sl.q[j] /= sum[0];
-                    sum[1] = sum[1] / sum[0] - log(sum[0]);
-                    sum[0] /= sum[0];   // 1, or NaN
+                twice = __any_sync(~0u, again);
+                for (int o = 16; o; o >>= 1) {
+                    sum += __shfl_xor_sync(~0u, sum, o);
+                    cross += __shfl_xor_sync(~0u, cross, o);
                 }
-                if (b == 0) sh.teacher[set] = Teacher{sum[1], sum[0], most[2], 1u};
-            } else if (b == 0) {
+                const double scale = TAIL ? 1.0 : 1.0 / sum;
+                if (!TAIL) cross = cross * scale - log(sum);
+                if (lane == 0) sh.teacher[set] = Teacher{cross, sum * scale, scale, value(most_c), 1u};
+            } else if (lane == 0) {
                 sh.teacher[set].live = 0u;
             }
+            __syncwarp();
         };
         auto finish = [&](uint32_t i) {
-            const uint32_t row = row_of(i), set = i & 3;
-            const Slots sl = slots(i);
+            const uint32_t row = row_of(i);
             const Coef cf = sh.coef[set];
             const Row<T> R(A.x, A.ld, row, V);
             const Slice part = slice_of(R);
             const uint32_t e0 = R.lead + part.c0 * E, span = (part.c1 - part.c0) * E;
             if (!sh.teacher[set].live) return;
-            const double u = (double)anchor(sh.teacher[set].u);
-            const bool twice = sh.twice[set] != 0u;
+            const double u = (double)anchor(sh.teacher[set].u), scale = sh.teacher[set].scale;
             T *out = (T *)A.grad + (size_t)row * A.ld_grad;
-            for (uint32_t j = b; j < A.n_ids; j += BTHREADS) {
+            for (uint32_t j = lane; j < A.n_ids; j += 32) {
                 const int32_t id = sl.id[j];
                 if (id < 0) continue;
                 const uint32_t e = (uint32_t)id - e0;
@@ -1138,23 +1147,19 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 if (!first) continue;
                 const float c = capped<CAP>(sl.v[j], A.sc);
                 const double p = exp(((double)c - u) * A.sc.md - cf.lse);
-                out[id] = from_f<T>((float)(cf.wm * (p * cf.q_all - q)) * slope<CAP>(c, A.sc));
+                out[id] = from_f<T>((float)(cf.wm * (p * cf.q_all - q * scale)) * slope<CAP>(c, A.sc));
             }
         };
-        one = fetch(0);
-        two = fetch(1);
-        fetch_logit(0);
-        auto ready = [&](uint32_t i) {
+        fetch(set);
+        fetch_row_logits(set);
+        for (uint32_t i = set; i < n; i += 4) {
             prepare(i);
-            bar_sync(BAR_B, BTHREADS);
-            if (b == 0) bar_arrive_local(&sh.slots_bar[i & 3]);
-        };
-        for (uint32_t i = 0; i < 3 && i < n; i++) ready(i);
-        for (uint32_t i = 0; i < n; i++) {
-            if (i + 3 < n) ready(i + 3);               // (its set was row i - 1's)
-            bar_sync(BAR_Z + (i & 3), z_threads);      // row i's gradient is written
+            if (lane == 0) bar_arrive_local(&sh.slots_bar[set]);
+            fetch(i + 4);
+            bar_sync(BAR_Z + set, z_threads);          // row i's gradient is written
+            fetch_row_logits(i + 4);
             finish(i);
-            bar_sync(BAR_B, BTHREADS);
+            __syncwarp();
         }
     }
 }
@@ -1166,7 +1171,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
 // write a logit: 2048 x 151936 bf16 (1792 rows read) 179 us, the copy bandwidth.
 // The token's element is worked out again in 64 bits (token_slope).
 __device__ __noinline__ float token_grad(const Scale &sc, float c, float2 st, float H, float g, float h) {
-    return (float)(sc.md * token_slope(((double)c - (double)st.x) * sc.md - (double)st.y, H, g, h));
+    const double lp = ((double)c - (double)st.x) * sc.md - (double)st.y;
+    return (float)(sc.md * token_slope(lp, expm1(lp), H, g, h));
 }
 constexpr int GRAD_BATCH = 4;
 constexpr uint32_t GRAD_SLICE = THREADS * GRAD_BATCH * 2;   // chunks of a CTA
