@@ -298,11 +298,12 @@ bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t
  * over the row's teacher ids, loss = sum_i w_i L_i, and the loss's gradient.
  *   d_teacher_ids, d_teacher_logits : rows x n_ids (n_ids <= BS_MAX_TOP);
  *       an id outside the vocabulary is an empty slot; an id that comes
- *       twice has the sum of its shares
+ *       twice adds a term for each of its slots
  *   d_teacher_lse : NULL, and q is the softmax of teacher_logits / T over the
  *       row's slots; or rows values, and q_k = exp(t_k / T - lse) with the
  *       rest of the vocabulary as one more outcome (its share 1 - sum q_k,
- *       where positive; left out where the student gives the rest no mass)
+ *       where positive; left out where the teacher names all of the
+ *       vocabulary or the student's rest is all -inf)
  *   d_weights : rows, or NULL for 1 / rows each
  *   d_row_loss: the L_i;  d_grad: NULL, or d loss / d logits
  * A row of weight 0 or without a teacher id (or, where q is a softmax, all of

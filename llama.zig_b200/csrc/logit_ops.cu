@@ -254,6 +254,21 @@ template <typename T> __device__ __forceinline__ void store_each(T *g, const uin
     for (int i = 0; i < (int)(16 / sizeof(T)); i++) g[i] = e[i];
 }
 
+// Logits of a chunk that count for nothing: -inf in place of those in `marks`.
+template <typename T> __device__ __forceinline__ void mask_out(f2 (&v)[8 / sizeof(T)], uint32_t marks) {
+#pragma unroll
+    for (int i = 0; i < (int)(8 / sizeof(T)); i++) {
+        if (marks >> (2 * i) & 1u) v[i].x = -INFINITY;
+        if (marks >> (2 * i) & 2u) v[i].y = -INFINITY;
+    }
+}
+template <typename T> __device__ __forceinline__ void mask_out(uint4 &q, uint32_t marks) {
+    f2 v[8 / sizeof(T)];
+    unpack<T>(q, v);
+    mask_out<T>(v, marks);
+    q = pack<T>(v);
+}
+
 // A row as its body, the 16-byte aligned chunks that lie wholly inside it,
 // and at most E - 1 single elements before and behind the body.
 template <typename T> struct Row {
@@ -288,62 +303,50 @@ struct Stat {
 __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // What a thread gathers of the logits it reads, on the scale of its running
-// maximum m: s = sum 2^d and u = sum 2^d d in pairs (even and odd logits).
-// With TAIL, s is the sum over the tokens that are not the teacher's and
-// `top` that over those that are; u is then not kept.
-template <typename T, bool CAP, bool ENT, bool TAIL> struct Gather {
+// maximum m: s = sum 2^d and (ENT) u = sum 2^d d in pairs (even and odd logits).
+template <typename T, bool CAP, bool ENT> struct Gather {
     static constexpr int E = 16 / sizeof(T);
-    float m = -INFINITY, top = 0.0f;
+    float m = -INFINITY;
     f2 s = {0.0f, 0.0f}, u = {0.0f, 0.0f};
     __device__ __forceinline__ void raise(float to, float k) {
         if (to > m) {   // (fmaxf: from -inf there is nothing to rescale)
             const float d = fmaxf((m - to) * k, D_MIN), f = ex2(d);
-            if (TAIL) top *= f;
             if (ENT) u = mul2(both(f), fma2(both(d), s, u));
             s = mul2(s, both(f));
             m = to;
         }
     }
     // logits after the soft-cap, none above m (but for the soft-cap's rounding)
-    __device__ __forceinline__ void chunk(const f2 (&v)[E / 2], float k, uint32_t marks = 0) {
+    __device__ __forceinline__ void chunk(const f2 (&v)[E / 2], float k) {
         const f2 base = both(-anchor(m)), kk = both(k);
 #pragma unroll
         for (int i = 0; i < E / 2; i++) {
             const f2 d = mul2(add2(v[i], base), kk);
-            f2 e = ex2_2(d);
-            if (TAIL && marks) {
-                float a, b;
-                halves(e, a, b);
-                if (marks >> (2 * i) & 1u) top += a, a = 0.0f;
-                if (marks >> (2 * i) & 2u) top += b, b = 0.0f;
-                e = pair(a, b);
-            }
+            const f2 e = ex2_2(d);
             s = add2(s, e);
             if (ENT) u = fma2(e, floor2(d), u);
         }
     }
+    // (those in `marks` are left out)
     __device__ __forceinline__ void chunk(const uint4 &q, const Scale &sc, uint32_t marks = 0) {
         f2 v[E / 2];
         unpack<T>(q, v);
 #pragma unroll
         for (int i = 0; i < E / 2; i++) v[i] = capped2<CAP>(v[i], sc);
-        chunk(v, sc.k, marks);
+        if (CAP && marks) mask_out<T>(v, marks);
+        chunk(v, sc.k);
     }
-    __device__ __forceinline__ void one(float c, float k, bool marked) {   // a single logit
+    __device__ __forceinline__ void one(float c, float k) {   // a single logit
         raise(c, k);
         const float d = (c - anchor(m)) * k, e = ex2(d);
-        if (TAIL && marked) {
-            top += e;
-        } else {
-            s = add2(s, pair(e, 0.0f));
-            if (ENT) u = fma2(pair(e, 0.0f), both(max_nan(d, D_MIN)), u);
-        }
+        s = add2(s, pair(e, 0.0f));
+        if (ENT) u = fma2(pair(e, 0.0f), both(max_nan(d, D_MIN)), u);
     }
     __device__ __forceinline__ Stat stat() const {
         float a, b, c, d;
         halves(s, a, b);
         halves(u, c, d);
-        return Stat{m, a + b, TAIL ? top : c + d};
+        return Stat{m, a + b, c + d};
     }
 };
 
@@ -430,7 +433,7 @@ template <bool ENT> struct GradRow {
 // travel.  A warp that shares the SM with these issues an instruction in some
 // ten cycles, so B's 64-bit work is spread over four rows and meets no barrier
 // of its own: with the four warps together on one row 512 x 256000 f32 with 128
-// ids took 262 us, so 208; 4000 x 8000 bf16 with 64 ids 71 and 75.  Barriers, in as many copies as rows can be between the two sides:
+// ids took 262 us, so 210; 4000 x 8000 bf16 with 64 ids 71 and 83.  Barriers, in as many copies as rows can be between the two sides:
 // X (S -> A: row i summed), Y (A -> G: its coefficients), Z (-> C, B: done
 // with; from G, or without a gradient from S and A); and mbarriers: full_bar
 // (copy -> S), slots_bar (B -> S), mail_bar (A -> A of the other CTAs).
@@ -482,6 +485,7 @@ struct Coef {
 struct Teacher {
     double cross, mass;  // sum of q (log q - (c - U) m), sum of q
     double scale;        // q = scale x what the slots hold
+    double top;          // with a tail: sum of exp((c - U) m) over the CTA's own ids, each once
     float u;             // U: the largest c(v) of the slots
     uint32_t live;       // 0: no slot, or no share to give
 };
@@ -507,17 +511,17 @@ struct RowsShared {
 
 // The sum of a warp's (or of each group of W lanes') Stats, the same in all its
 // lanes: the largest maximum first, then every lane's sums on that scale.
-template <bool TAIL, int W> __device__ __forceinline__ Stat fold_lanes(Stat a, float k) {
+template <bool ENT, int W> __device__ __forceinline__ Stat fold_lanes(Stat a, float k) {
     float m = a.m;
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     const float d = fmaxf((a.m - m) * k, D_MIN), f = ex2(d);
-    a.u = f * (TAIL ? a.u : fmaf(d, a.s, a.u));   // (with TAIL, u is another sum, not one of 2^d d)
+    if (ENT) a.u = f * fmaf(d, a.s, a.u);
     a.s *= f;
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) {
         a.s += __shfl_xor_sync(~0u, a.s, o);
-        a.u += __shfl_xor_sync(~0u, a.u, o);
+        if (ENT) a.u += __shfl_xor_sync(~0u, a.u, o);
     }
     a.m = m;
     return a;
@@ -535,10 +539,10 @@ __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive_local(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ void mail_send(const float4 *slot, const uint64_t *bar, uint32_t rank, const Stat &a, float w) {
+__device__ __forceinline__ void mail_send(const float4 *slot, const uint64_t *bar, uint32_t rank, const float4 &v) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %5}, [%4];" ::"r"(
                      remote(slot, rank)),
-                 "r"(__float_as_uint(a.m)), "r"(__float_as_uint(a.s)), "r"(__float_as_uint(a.u)), "r"(remote(bar, rank)), "r"(__float_as_uint(w))
+                 "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(remote(bar, rank)), "r"(__float_as_uint(v.w))
                  : "memory");
 }
 // Waits for all bytes of a phase; false if it gave up (a second at the least).
@@ -567,6 +571,25 @@ struct TokenIn {
 // -expm1(log p), whose bits a p near 1 in f32 has lost.
 __device__ __forceinline__ double token_slope(double lp, double pm1, double H, double g, double h) {
     return -g * pm1 - (h != 0.0 ? h * (1.0 + pm1) * (fmax(lp, -1e4) + H) : 0.0);
+}
+// e^x to 2^-41: 2^n by the exponent's bits times the exponential series of the
+// rest, |r| <= ln 2 / 2, whose eleventh power over 11! is 2^-42.  0 below e^-700
+// (-inf too), +inf above e^700; a NaN stays.
+__device__ __forceinline__ double exp_d(double x) {
+    const double magic = 6755399441055744.0, n = fma(x, 1.0 / LN2_D, magic), r = fma(n - magic, -LN2_D, x);
+    double y = 1.0 / 3628800;
+    y = fma(y, r, 1.0 / 362880);
+    y = fma(y, r, 1.0 / 40320);
+    y = fma(y, r, 1.0 / 5040);
+    y = fma(y, r, 1.0 / 720);
+    y = fma(y, r, 1.0 / 120);
+    y = fma(y, r, 1.0 / 24);
+    y = fma(y, r, 1.0 / 6);
+    y = fma(y, r, 0.5);
+    y = fma(y, r, 1.0);
+    y = fma(y, r, 1.0);
+    y *= __hiloint2double((__double2loint(n) + 1023) << 20, 0);
+    return x < -700.0 ? 0.0 : x > 700.0 ? INFINITY : y;
 }
 // The exchange between a row's sums and its gradient waits for these few
 // values, so a warp works them out side by side: lane e has the function at the
@@ -626,33 +649,58 @@ __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const 
 struct Slots {
     double *q;        // the slot's share, but for the row's scale
     int32_t *id;      // -1: empty; padded to a multiple of 4 with empty ones
-    float *v;         // the student's logit there
+    float *c;         // the student's c(v) there
     uint32_t *bits;   // one bit per element of the CTA's slice: named by the teacher
 };
 constexpr uint32_t SLOT_BYTES = 16;
 __host__ __device__ __forceinline__ uint32_t slots_padded(uint32_t n_ids) { return (n_ids + 3u) & ~3u; }
 
 // Results and coefficients of a row with a teacher, in 64 bits as those of a
-// row with a token: a student near its teacher has a loss near 0, and the rest
-// of the vocabulary the gradient p_j (1 - q_rest / p_rest).
+// row with a token: a student near its teacher has a loss near 0.  With TAIL,
+// st is of the tokens that the teacher does not name, the rest R, on a scale of
+// its own: however far it lies below the others (or above), log p_R and the
+// shares p_j / p_R that its gradient goes by are finite,
+//     dv_j = w m c'(v_j) (p_j / p_R) (Q p_R - q_R)  in R,
+// and `top` is the sum of exp((c - U) m) over the named ones.
 template <bool TAIL>
-__device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, const Teacher &t, float w, bool write) {
-    const double s = TAIL ? (double)st.s + (double)st.u : (double)st.s, wm = (double)w * A.sc.md;
+__device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, double top, const Teacher &t, float w,
+                                            bool write) {
+    const double wm = (double)w * A.sc.md, u = (double)anchor(t.u);
+    double s = (double)st.s, big = (double)st.m, below = 1.0;
+    if (TAIL) {
+        const double d = ((double)st.m - (double)t.u) * A.sc.md, e = exp_d(-fabs(d));
+        if (d >= 0.0) {
+            s += top * e;
+        } else {
+            below = e;
+            s = s * e + top;
+            big = (double)t.u;
+        }
+    }
     const double qr = 1.0 - t.mass;
     double ln[3] = {s, (double)st.s, qr};
     if (TAIL) by_lanes(ln, [](double v) { return log(v); });
     else ln[0] = log(s);
-    const double ln_s = ln[0], lse = ((double)st.m - (double)anchor(t.u)) * A.sc.md + ln_s;   // relative to U
-    double loss = t.cross + t.mass * lse, mass = t.mass, share = 0.0;
+    const double lse = (big - u) * A.sc.md + ln[0];   // relative to U
+    double loss = t.cross + t.mass * lse, mass = t.mass;
+    Coef c{st.m, (float)(ln[TAIL ? 1 : 0] * (1.0 / LN2_D)), 0.0f, 0.0f, 0.0f, 1u, lse, 0.0, wm};
     if (TAIL) {   // the rest as one outcome
-        if (!(qr <= 0.0) && !(st.s == 0.0f)) {
-            loss += qr * (ln[2] - ln[1] + ln_s);
-            mass += qr;
-            share = qr * s / (double)st.s;
+        if (st.s == 0.0f) {
+            c.m = c.l2s = 0.0f;
+        } else {
+            const bool has = !(qr <= 0.0);
+            if (has) {
+                loss += qr * (ln[2] - (((double)st.m - big) * A.sc.md + ln[1] - ln[0]));
+                mass += qr;
+            }
+            c.ca = (float)(wm * (mass * ((double)st.s * below / s) - (has ? qr : 0.0)));
         }
+    } else {
+        c.ca = (float)(wm * mass);
     }
+    c.q_all = mass;
     if (write) A.row_loss[row] = (float)loss;
-    return Coef{st.m, (float)(ln_s * (1.0 / LN2_D)), (float)(wm * (mass - share)), 0.0f, 0.0f, 1u, lse, mass, wm};
+    return c;
 }
 
 template <typename T, int OP, bool CAP>
@@ -693,7 +741,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         Slots s;
         s.q = (double *)base + set * pad;
         s.id = (int32_t *)base + (8 + set) * pad;
-        s.v = (float *)base + (12 + set) * pad;
+        s.c = (float *)base + (12 + set) * pad;
         s.bits = (uint32_t *)base + 16 * pad + set * A.bit_words;
         return s;
     };
@@ -731,7 +779,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             there = bar_wait(&sh.full_bar[at], phase) && there;
             if (++at == 3) at = 0, phase ^= 1;
             if (DIST) there = bar_wait(&sh.slots_bar[i & 3], i >> 2 & 1) && there;
-            Gather<T, CAP, !DIST, TAIL> G;
+            Gather<T, CAP, !DIST> G;
             if (sh.code[i & 15] >= 0) {
                 const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
                 auto marks = [&](uint32_t c) -> uint32_t {
@@ -739,48 +787,51 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     const uint32_t b = c * E;
                     return bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
                 };
-                // several chunks at a time, for one comparison with the running maximum
-                uint32_t c = tid;
-                auto work = [&](const uint4 &q, uint4 *at, uint32_t cu) {
+                auto cap_chunk = [&](const uint4 &q) {
                     f2 v[E / 2];
                     unpack<T>(q, v);
 #pragma unroll
                     for (int e = 0; e < E / 2; e++) v[e] = capped2<CAP>(v[e], A.sc);
-                    if (LEAVE && grad) *at = pack<T>(v);
-                    G.chunk(v, k, marks(cu));
+                    return pack<T>(v);
                 };
+                // several chunks at a time, for one comparison with the running maximum
+                uint32_t c = tid;
                 for (; c + (STEP - 1) * sum_threads < copied; c += STEP * sum_threads, buf += STEP * sum_threads) {
                     uint4 q[STEP];
+                    uint32_t mk[STEP];
 #pragma unroll
-                    for (int u = 0; u < STEP; u++) q[u] = buf[u * sum_threads];
+                    for (int u = 0; u < STEP; u++) q[u] = buf[u * sum_threads], mk[u] = marks(c + u * sum_threads);
                     if constexpr (LEAVE) {
                         // (the soft-cap of all of them first: that of the largest alone would be waited for)
 #pragma unroll
                         for (int u = 0; u < STEP; u++) {
-                            f2 v[E / 2];
-                            unpack<T>(q[u], v);
-#pragma unroll
-                            for (int e = 0; e < E / 2; e++) v[e] = capped2<CAP>(v[e], A.sc);
-                            q[u] = pack<T>(v);
+                            q[u] = cap_chunk(q[u]);
                             if (grad) buf[u * sum_threads] = q[u];
+                            if (mk[u]) mask_out<T>(q[u], mk[u]);
                         }
                         G.raise(max_of<T>(q), k);
 #pragma unroll
                         for (int u = 0; u < STEP; u++) {
                             f2 v[E / 2];
                             unpack<T>(q[u], v);
-                            G.chunk(v, k, marks(c + u * sum_threads));
+                            G.chunk(v, k);
                         }
                     } else {
+#pragma unroll
+                        for (int u = 0; u < STEP; u++)
+                            if (mk[u]) mask_out<T>(q[u], mk[u]);
                         G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
 #pragma unroll
-                        for (int u = 0; u < STEP; u++) work(q[u], buf + u * sum_threads, c + u * sum_threads);
+                        for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, mk[u]);
                     }
                 }
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
-                    const uint4 q = buf[0];
+                    uint4 q = buf[0];
+                    const uint32_t mk = marks(c);
+                    if (LEAVE && grad) buf[0] = cap_chunk(q);
+                    if (mk) mask_out<T>(q, mk);
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
-                    work(q, buf, c);
+                    G.chunk(q, A.sc, mk);
                 }
                 // what did not fit
                 const T *x = R.at(sl.c0);
@@ -792,15 +843,17 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
 #pragma unroll
                     for (int u = 0; u < STEP; u++)
                         if (c + u * sum_threads < count) {
+                            const uint32_t mk = marks(c + u * sum_threads);
+                            if (mk) mask_out<T>(q[u], mk);
                             G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
-                            G.chunk(q[u], A.sc, marks(c + u * sum_threads));
+                            G.chunk(q[u], A.sc, mk);
                         }
                 }
             }
             // (the buffer is written by copies again)
             if (LEAVE && grad) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             Stat st{-INFINITY, 0.0f, 0.0f};
-            if (sh.code[i & 15] >= 0) st = fold_lanes<TAIL, 32>(G.stat(), k);
+            if (sh.code[i & 15] >= 0) st = fold_lanes<!DIST, 32>(G.stat(), k);
             // (a copy that never came: the row is NaN)
             if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
             bar_arrive(BAR_X + (i & 3), x_threads);
@@ -915,21 +968,15 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 st = Stat{f.x, f.y, f.z};
             }
             if (!grad && !DIST) bar_arrive(BAR_Z + (i & 3), z_threads);   // the sums are read: S may go on
-            if (live && edge >= 0) {
-                const bool marked = TAIL && (sh.edge_marks[i & 3] >> lane & 1u);
+            if (live && edge >= 0 && !(TAIL && (sh.edge_marks[i & 3] >> lane & 1u))) {
                 // one logit: 2^0 at itself, nothing where it is -inf (or a sum of NaN)
                 const float one = c_edge == -INFINITY ? 0.0f : c_edge - c_edge == 0.0f ? 1.0f : NAN;
-                const Stat e{c_edge, marked ? 0.0f : one, marked ? one : 0.0f};
                 const float m = c_edge != c_edge ? st.m : fmaxf(st.m, c_edge);
-                const float fa = ex2(fmaxf((st.m - m) * k, D_MIN)), fb = ex2(fmaxf((e.m - m) * k, D_MIN));
-                if (TAIL) {
-                    st = Stat{m, st.s * fa + e.s * fb, st.u * fa + e.u * fb};
-                } else {
-                    const float da = fmaxf((st.m - m) * k, D_MIN), db = fmaxf((e.m - m) * k, D_MIN);
-                    st = Stat{m, st.s * fa + e.s * fb, fa * fmaf(da, st.s, st.u) + fb * (db * e.s)};
-                }
+                const float da = fmaxf((st.m - m) * k, D_MIN), db = fmaxf((c_edge - m) * k, D_MIN), fa = ex2(da), fb = ex2(db);
+                st = Stat{m, st.s * fa + one * fb, fa * fmaf(da, st.s, st.u) + fb * (db * one)};
             }
-            st = fold_lanes<TAIL, 32>(st, k);
+            st = fold_lanes<!DIST, 32>(st, k);
+            double top = TAIL && live ? sh.teacher[i & 3].top : 0.0;
             if (ranks > 1 && sh.code[i & 15] >= 0) {
                 // The rows that take part in an exchange count the same in every CTA.  A warp's exchanges take turns
                 // with two boxes: a CTA sends into one only after all have sent into the other, so have read what
@@ -937,15 +984,23 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 // write the gradient over it.
                 const uint32_t box = which * 2 + (sent & 1), turn = sent >> 1 & 1;
                 sent++;
-                if (lane < ranks) mail_send(&sh.mail[box][rank], &sh.mail_bar[box], lane, st, c_tok);
+                float4 out = make_float4(st.m, st.s, st.u, c_tok);
+                if (TAIL) out.z = __int_as_float(__double2loint(top)), out.w = __int_as_float(__double2hiint(top));
+                if (lane < ranks) mail_send(&sh.mail[box][rank], &sh.mail_bar[box], lane, out);
                 if (lane == 0) bar_expect(&sh.mail_bar[box], ranks * 16);
                 const bool there = bar_wait(&sh.mail_bar[box], turn);
                 st = Stat{-INFINITY, 0.0f, 0.0f};
+                top = 0.0;
                 if (lane < ranks) {
                     const float4 f = sh.mail[box][lane];
                     st = Stat{f.x, there ? f.y : NAN, f.z};   // (a CTA that never sent: the row is NaN)
+                    if (TAIL) top = __hiloint2double(__float_as_int(f.w), __float_as_int(f.z));
                 }
-                st = fold_lanes<TAIL, MAX_CLUSTER>(st, k);
+                if (TAIL) {
+                    for (int o = MAX_CLUSTER / 2; o; o >>= 1) top += __shfl_xor_sync(~0u, top, o);
+                    top = __shfl_sync(~0u, top, 0);
+                }
+                st = fold_lanes<!DIST, MAX_CLUSTER>(st, k);
                 st.m = __shfl_sync(~0u, st.m, 0);
                 st.s = __shfl_sync(~0u, st.s, 0);
                 st.u = __shfl_sync(~0u, st.u, 0);
@@ -954,7 +1009,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             Coef cf{};
             if (live) {
                 if constexpr (DIST) {
-                    cf = teacher_row<TAIL>(A, row, st, sh.teacher[i & 3], cur.in.w, write);
+                    cf = teacher_row<TAIL>(A, row, st, top, sh.teacher[i & 3], cur.in.w, write);
                 } else {
                     TokenIn in = cur.in;
                     in.c_tok = c_tok;
@@ -1046,6 +1101,11 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         auto fetch_row_logits = [&](uint32_t i) {
             if (i < n && f.w != 0.0f) fetch_logits(row_of(i));
         };
+        // in the CTA's slice, or (rank 0) a single element
+        auto mine = [&](int32_t id, const Row<T> &R, uint32_t e0, uint32_t span) {
+            const bool single = (uint32_t)id < R.lead || (uint32_t)id >= V - R.trail;
+            return single ? rank == 0 : (uint32_t)id - e0 < span;
+        };
         bool twice = false;   // an id of the slice comes twice
         auto prepare = [&](uint32_t i) {
             const uint32_t row = row_of(i);
@@ -1068,11 +1128,11 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                         const bool valid = (uint32_t)f.id[a] < V;
                         sl.id[j] = valid ? f.id[a] : -1;
                         if (valid) {
-                            const float v = to_f(f.x[a]);
+                            const float c = capped<CAP>(to_f(f.x[a]), A.sc);
                             sl.q[j] = (double)f.t[a];
-                            sl.v[j] = v;
+                            sl.c[j] = c;
                             most_t = max(most_t, order(f.t[a]));
-                            most_c = max(most_c, order(capped<CAP>(v, A.sc)));
+                            most_c = max(most_c, order(c));
                         }
                     }
                 }
@@ -1089,11 +1149,11 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 for (uint32_t j = lane; j < pad; j += 32) {
                     const int32_t id = sl.id[j];
                     if (id < 0) continue;
-                    const double a = sl.q[j] * A.sc.inv_t - ref, q = exp(a);
+                    const double a = sl.q[j] * A.sc.inv_t - ref, q = exp_d(a);
                     sl.q[j] = q;
                     if (!(q <= 0.0)) {
                         sum += q;
-                        cross += q * (a - ((double)capped<CAP>(sl.v[j], A.sc) - u) * A.sc.md);
+                        cross += q * (a - ((double)sl.c[j] - u) * A.sc.md);
                     }
                     const uint32_t e = (uint32_t)id - e0;
                     uint32_t *word = &sl.bits[e >> 5], bit = 1u << (e & 31);
@@ -1104,13 +1164,25 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     if (bit && (atomicOr(word, bit) & bit)) again = true;
                 }
                 twice = __any_sync(~0u, again);
+                __syncwarp();   // all of sl.id is there
+                double top = 0.0;
+                if (TAIL) {
+                    for (uint32_t j = lane; j < pad; j += 32) {
+                        const int32_t id = sl.id[j];
+                        if (id < 0 || !mine(id, R, e0, span)) continue;
+                        bool first = true;
+                        for (uint32_t o = 0; twice && o < j; o++) first = first && sl.id[o] != id;
+                        if (first) top += exp_d(((double)sl.c[j] - u) * A.sc.md);
+                    }
+                }
                 for (int o = 16; o; o >>= 1) {
                     sum += __shfl_xor_sync(~0u, sum, o);
                     cross += __shfl_xor_sync(~0u, cross, o);
+                    if (TAIL) top += __shfl_xor_sync(~0u, top, o);
                 }
                 const double scale = TAIL ? 1.0 : 1.0 / sum;
                 if (!TAIL) cross = cross * scale - log(sum);
-                if (lane == 0) sh.teacher[set] = Teacher{cross, sum * scale, scale, value(most_c), 1u};
+                if (lane == 0) sh.teacher[set] = Teacher{cross, sum * scale, scale, top, value(most_c), 1u};
             } else if (lane == 0) {
                 sh.teacher[set].live = 0u;
             }
@@ -1129,9 +1201,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 const int32_t id = sl.id[j];
                 if (id < 0) continue;
                 const uint32_t e = (uint32_t)id - e0;
-                const bool single = (uint32_t)id < R.lead || (uint32_t)id >= V - R.trail;
-                if (single ? rank != 0 : e >= span) continue;
-                if (!single) sl.bits[e >> 5] = 0u;
+                if (!mine(id, R, e0, span)) continue;
+                if (e < span) sl.bits[e >> 5] = 0u;
                 if (!grad) continue;
                 // p Q - q, where q is the sum over the slots that hold the id (the first of them writes)
                 double q = sl.q[j];
@@ -1145,8 +1216,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     if (v.w == id) q += sl.q[o + 3], first = first && o + 3 >= j;
                 }
                 if (!first) continue;
-                const float c = capped<CAP>(sl.v[j], A.sc);
-                const double p = exp(((double)c - u) * A.sc.md - cf.lse);
+                const float c = sl.c[j];
+                const double p = exp_d(((double)c - u) * A.sc.md - cf.lse);
                 out[id] = from_f<T>((float)(cf.wm * (p * cf.q_all - q * scale)) * slope<CAP>(c, A.sc));
             }
         };
@@ -1659,7 +1730,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
     const float v_edge = edge >= 0 ? to_f(R.x[edge]) : -INFINITY;
     const T v_tok = !TOP && rank == 0 && tid == 0 ? R.x[tok] : from_f<T>(0.0f);
     float *tile_max = TOP ? P.maxima + (size_t)row * P.max_ld : nullptr;
-    Gather<T, CAP, !TOP, false> G;
+    Gather<T, CAP, !TOP> G;
 
     // whole batches of the CTA, so that a warp's lanes stay together
     for (uint32_t b = c0; b < c1; b += BATCH * THREADS) {
@@ -1705,18 +1776,18 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
             if (first < c1) tile_max[first / TOP_TILE] = mx[0];
         }
     }
-    if (edge >= 0) G.one(capped<CAP>(v_edge, A.sc), k, false);
+    if (edge >= 0) G.one(capped<CAP>(v_edge, A.sc), k);
     if (TOP && rank == 0 && tid < 32) {          // the single elements as one more tile
         float m = v_edge;
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         if (tid == 0) tile_max[tiles] = m;
     }
-    Stat st = fold_lanes<false, 32>(G.stat(), k);
+    Stat st = fold_lanes<!TOP, 32>(G.stat(), k);
     if (lane == 0) sh.warp[tid >> 5] = st;
     __syncthreads();
     if (tid < 32) {
         st = lane < WARPS ? sh.warp[lane] : Stat{-INFINITY, 0.0f, 0.0f};
-        st = fold_lanes<false, 32>(st, k);
+        st = fold_lanes<!TOP, 32>(st, k);
     }
     if (ranks > 1) {
         cluster_wait();
@@ -1726,7 +1797,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
         cluster_wait();
         if (tid < 32) {
             const float4 f = lane < ranks ? sh.cta[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-            st = fold_lanes<false, 32>(Stat{f.x, f.y, f.z}, k);
+            st = fold_lanes<!TOP, 32>(Stat{f.x, f.y, f.z}, k);
         }
     }
     if (rank != 0) return;

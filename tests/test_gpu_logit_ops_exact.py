@@ -125,3 +125,68 @@ def test_student_near_its_teacher(gpu_pkg, vocab, K, tail, near):
             l2s = math.log2(vocab)
             tol = EPS * (2 * l2s * math.log(2.0) + 4 + 2) + (2.0**-50 * vocab / float(grad[rest].abs().min()) / vocab if tail else 0)
             relative(got.grad[:, rest.cuda()], grad[rest].expand(2, -1), tol, "rest")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("gap", [60.0, 90.0, 104.0, 200.0, 2000.0, -200.0])
+@pytest.mark.parametrize("vocab,off", [(40, 0), (5001, 1), (128256, 3)])
+def test_rest_far_below_the_teacher(gpu_pkg, dtype, gap, vocab, off):
+    """The tail's outcome where the student gives it e^-gap of a named token (or, below zero, the named ones that)."""
+    g = torch.Generator(device="cuda").manual_seed(181)
+    rows, K = 3, 7
+    x = torch.zeros(off + rows * vocab, dtype=dtype, device="cuda")[off:].view(rows, vocab)
+    x.copy_(torch.randn(rows, vocab, generator=g, device="cuda"))
+    ids = torch.stack([torch.randperm(vocab, generator=g, device="cuda")[:K] for _ in range(rows)]).int()
+    ids[0, 0], ids[0, 1] = 0, vocab - 1        # (single elements before and behind the 16-byte chunks, where there are)
+    for i in range(rows):
+        x[i, ids[i].long()] = (gap + 3.0 * torch.randn(K, generator=g, device="cuda")).to(dtype)
+    ids[1, 3] = ids[1, 2]                      # one twice
+    ids[2, 5] = -1
+    tl = torch.randn(rows, K, generator=g, device="cuda")
+    lse = torch.logsumexp(tl, 1) + 0.5
+    w = torch.tensor([1.0, 0.5, 0.25], device="cuda")
+    got = gpu_pkg.distill_loss(x, ids, tl, lse, w)
+    v = x.double().requires_grad_()
+    valid = ids >= 0
+    at = ids.long().clamp_min(0)
+    q = torch.where(valid, (tl.double() - lse.double()[:, None]).exp(), 0.0)
+    logp = torch.log_softmax(v, 1)
+    inside = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda")
+    for i in range(rows):
+        inside[i, at[i][valid[i]]] = True
+    qr = 1 - q.sum(1)
+    lr = torch.logsumexp(logp.masked_fill(inside, -math.inf), 1)
+    L = torch.where(valid, q * (q.clamp_min(1e-300).log() - logp.gather(1, at)), 0.0).sum(1) + qr * (qr.log() - lr)
+    (L * w).sum().backward()
+    # logits of one side differ by at most R; a term of its sum carries 3 R ln 2 EPS and 4 EPS, is rescaled at most 8 times,
+    # and is one of vocab / 128 + 32 a thread and its fold adds
+    R = 12.0 * 1.4427
+    delta = EPS * (9 * (3 * R + 4) + vocab / 128 + 32)
+    tol_L = delta + 2 * EPS * L.abs()
+    assert bool(((got.row_losses.double() - L).abs() <= tol_L).all()), (got.row_losses, L)
+    size = w[:, None] * torch.where(inside, (logp.exp() + q.sum(1, keepdim=True)), (logp - lr[:, None]).exp())
+    half = torch.finfo(dtype).eps / 2
+    # (2^l is 0 below 2^-126: a named token that takes another's place leaves its logit in the rest, and the others there
+    # have shares near e^-gap; half of f16's least step is 2^-25)
+    tol = 3 * delta * size + 1.01 * half * v.grad.abs() + (2.0**-25 if dtype == torch.float16 else 2.0**-126)
+    bad = (got.grad.double() - v.grad).abs() > tol
+    assert not bool(bad.any()), (int(bad.sum()), got.grad.double()[bad][:5], v.grad[bad][:5])
+
+
+def test_no_rest_is_left_out(gpu_pkg):
+    # all of the rest masked: the outcome that the student cannot give is left out, whatever share the teacher gives it
+    x = torch.full((2, 300), -math.inf, device="cuda")
+    ids = torch.tensor([[3, 299, 150], [0, 1, 2]], dtype=torch.int32, device="cuda")
+    x[0, ids[0].long()] = torch.tensor([1.0, 2.0, -1.0], device="cuda")
+    x[1, ids[1].long()] = torch.tensor([500.0, 2.0, -1.0], device="cuda")
+    tl = torch.tensor([[0.5, 0.0, 0.25], [0.5, 0.0, 0.25]], device="cuda")
+    lse = torch.logsumexp(tl, 1) + 0.5
+    got = gpu_pkg.distill_loss(x, ids, tl, lse, torch.ones(2, device="cuda"))
+    q = (tl - lse[:, None]).double().exp()
+    logp = torch.log_softmax(x.double(), 1).gather(1, ids.long())
+    want = (q * (q.log() - logp)).sum(1)
+    assert bool(((got.row_losses - want).abs() <= 8 * EPS * (1 + want.abs())).all())
+    grad = (logp.exp() * q.sum(1, keepdim=True) - q)
+    assert bool(((got.grad.gather(1, ids.long()) - grad).abs() <= 8 * EPS).all())
+    rest = got.grad.scatter(1, ids.long(), 0.0)
+    assert not bool(rest.any()) and bool(torch.isfinite(rest).all())
