@@ -40,6 +40,8 @@ struct Scale {
     float k;         // m log2(e)
     float m;         // 1 / (logit_scale T)
     float cap, icap; // soft-cap and its reciprocal
+    float k2, k2_lo; // -2 log2(e) / cap, and what f32 leaves off it
+    float most;      // c(v) is +-cap from here on
     double md;       // m in 64 bits
     double inv_t;    // 1 / T
     double dk;       // what rounding left off k, relative
@@ -109,45 +111,40 @@ __device__ __forceinline__ f2 floor2(f2 v) {   // at least D_MIN; a NaN stays
     return pair(max_nan(a, D_MIN), max_nan(b, D_MIN));
 }
 
-// The soft-cap c(v) = cap tanh(v / cap).  tanh(x) is x P(x^2) / Q(x^2) for
-// |x| <= 9, where 1 - tanh is below half a step: a least-squares fit of the
-// relative error over [0, 9], reweighted towards its maximum, 2.1e-8.  All
-// coefficients are positive, so the two sums lose nothing; at most 12 half
-// steps off with the products and the approximate reciprocal.  Two FMA-pipe
-// slots a term for two logits and one reciprocal each, where the form with an
-// exponential needs two of the scarce special functions.
-__constant__ const float TANH_P[5] = {0.9999999794944238f, 0.13381039141757592f, 0.0034956033997520213f,
-                                      2.0609303648709823e-05f, 1.3354913460618338e-08f};
-__constant__ const float TANH_Q[4] = {0.46714354763692456f, 0.025877042277977037f, 0.0003285658489434587f,
-                                      7.776672917322147e-07f};
+// The soft-cap c(v) = cap tanh(v / cap).  Up to |v| = cap, where nearly all
+// logits are, c = v + v y W(y) with y = (v / cap)^2 and W a polynomial: the least
+// largest relative error of c over y in [0, 1] with f32 coefficients, 4.7e-9.
+// The last fused step rounds once, what comes before it is at most 0.31 of c: at
+// most 3.3 half steps in all, 0.75 root mean square, as cap * tanhf(v / cap) has.
+// Ten FMA-pipe slots for two logits.  Beyond, c = cap - cap 2 e / (1 + e) with
+// e = exp(-2 |v| / cap), the exponent with what its two roundings left off: at
+// most 3.7 half steps.
+__constant__ const float TANH_W[7] = {-0.33333295583724976f, 0.13332347571849823f, -0.0538799911737442f, 0.021487198770046234f,
+                                      -0.007946893572807312f, 0.0023019297514110804f, -0.00035861122887581587f};
 __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float within(float x) {   // [-9, 9]; a NaN stays
-    float y;
-    asm("min.NaN.f32 %0, %1, 0f41100000;" : "=f"(y) : "f"(max_nan(x, -9.0f)));
-    return y;
+__device__ __forceinline__ f2 cap_near(f2 v, const Scale &sc) {
+    const f2 x = mul2(v, both(sc.icap)), y = mul2(x, x);
+    f2 w = both(TANH_W[6]);
+#pragma unroll
+    for (int i = 5; i >= 0; i--) w = fma2(w, y, both(TANH_W[i]));
+    return fma2(mul2(v, y), w, v);
 }
-template <bool CAP> __device__ __forceinline__ f2 capped2(f2 v, const Scale &sc) {
-    if (!CAP) return v;
-    float a, b;
-    halves(mul2(v, both(sc.icap)), a, b);
-    const f2 x = pair(within(a), within(b)), y = mul2(x, x);
-    f2 p = both(TANH_P[4]), q = both(TANH_Q[3]);
-#pragma unroll
-    for (int i = 3; i >= 0; i--) p = fma2(p, y, both(TANH_P[i]));
-#pragma unroll
-    for (int i = 2; i >= 0; i--) q = fma2(q, y, both(TANH_Q[i]));
-    halves(fma2(q, y, both(1.0f)), a, b);
-    return mul2(mul2(mul2(x, p), pair(rcp(a), rcp(b))), both(sc.cap));
+__device__ __forceinline__ float cap_far(float v, const Scale &sc) {
+    const float a = fminf(fabsf(v), sc.most), t = a * sc.k2;
+    const float e = ex2(t) * fmaf(LN2, fmaf(a, sc.k2, -t) + a * sc.k2_lo, 1.0f);
+    const float q = 2.0f * e * rcp(1.0f + e);
+    return copysignf(fmaf(-sc.cap, q, sc.cap), v);
 }
 template <bool CAP> __device__ __forceinline__ float capped(float v, const Scale &sc) {
-    float a, b;
-    halves(capped2<CAP>(both(v), sc), a, b);
-    return a;
+    if (!CAP) return v;
+    if (fabsf(v) > sc.cap) return cap_far(v, sc);
+    return cap_near(both(v), sc).x;
 }
+
 // The soft-cap's slope 1 - (c / cap)^2.
 template <bool CAP> __device__ __forceinline__ f2 slope2(f2 c, const Scale &sc) {
     const f2 t = mul2(c, both(sc.icap));
@@ -247,6 +244,34 @@ template <typename T, int N> __device__ __forceinline__ float max_of(const uint4
     }
     return max_of<T>(m);
 }
+// The largest |logit| of a chunk (a NaN is passed over).
+template <typename T> __device__ __forceinline__ float max_abs(uint4 q) {
+    if constexpr (sizeof(T) == 4) {
+        return fmaxf(fmaxf(fabsf(__uint_as_float(q.x)), fabsf(__uint_as_float(q.y))),
+                     fmaxf(fabsf(__uint_as_float(q.z)), fabsf(__uint_as_float(q.w))));
+    } else {
+        const uint32_t m = 0x7FFF7FFFu;
+        return max_of<T>(make_uint4(q.x & m, q.y & m, q.z & m, q.w & m));
+    }
+}
+// A chunk's logits after the soft-cap.
+template <typename T, bool CAP> __device__ __forceinline__ void cap_chunk(const uint4 &q, f2 (&v)[8 / sizeof(T)], const Scale &sc) {
+    unpack<T>(q, v);
+    if (!CAP) return;
+    constexpr int N = 8 / sizeof(T);
+    const bool far = max_abs<T>(q) > sc.cap;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = cap_near(v[i], sc);
+    if (far) {
+        f2 raw[N];
+        unpack<T>(q, raw);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (fabsf(raw[i].x) > sc.cap) v[i].x = cap_far(raw[i].x, sc);
+            if (fabsf(raw[i].y) > sc.cap) v[i].y = cap_far(raw[i].y, sc);
+        }
+    }
+}
 // What a thread writes of a chunk where 16-byte stores do not fit.
 template <typename T> __device__ __forceinline__ void store_each(T *g, const uint4 &q) {
     const T *e = reinterpret_cast<const T *>(&q);
@@ -330,9 +355,7 @@ template <typename T, bool CAP, bool ENT> struct Gather {
     // (those in `marks` are left out)
     __device__ __forceinline__ void chunk(const uint4 &q, const Scale &sc, uint32_t marks = 0) {
         f2 v[E / 2];
-        unpack<T>(q, v);
-#pragma unroll
-        for (int i = 0; i < E / 2; i++) v[i] = capped2<CAP>(v[i], sc);
+        cap_chunk<T, CAP>(q, v, sc);
         if (CAP && marks) mask_out<T>(v, marks);
         chunk(v, sc.k);
     }
@@ -388,10 +411,9 @@ template <bool ENT> struct GradRow {
     __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
         constexpr int N = 8 / sizeof(T);
         f2 v[N], o[N];
-        unpack<T>(q, v);
+        cap_chunk<T, CAP && !DONE>(q, v, sc);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (!DONE) v[i] = capped2<CAP>(v[i], sc);
             const f2 l = fma2(add2(v[i], both(-m)), both(k), both(-l2s));
             o[i] = mul2(ex2_2(l), ENT ? fma2(both(cb), floor2(l), both(ca)) : both(ca));
         }
@@ -787,11 +809,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     const uint32_t b = c * E;
                     return bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
                 };
-                auto cap_chunk = [&](const uint4 &q) {
+                auto capped_chunk = [&](const uint4 &q) {
                     f2 v[E / 2];
-                    unpack<T>(q, v);
-#pragma unroll
-                    for (int e = 0; e < E / 2; e++) v[e] = capped2<CAP>(v[e], A.sc);
+                    cap_chunk<T, CAP>(q, v, A.sc);
                     return pack<T>(v);
                 };
                 // several chunks at a time, for one comparison with the running maximum
@@ -805,7 +825,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                         // (the soft-cap of all of them first: that of the largest alone would be waited for)
 #pragma unroll
                         for (int u = 0; u < STEP; u++) {
-                            q[u] = cap_chunk(q[u]);
+                            q[u] = capped_chunk(q[u]);
                             if (grad) buf[u * sum_threads] = q[u];
                             if (mk[u]) mask_out<T>(q[u], mk[u]);
                         }
@@ -828,7 +848,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
                     uint4 q = buf[0];
                     const uint32_t mk = marks(c);
-                    if (LEAVE && grad) buf[0] = cap_chunk(q);
+                    if (LEAVE && grad) buf[0] = capped_chunk(q);
                     if (mk) mask_out<T>(q, mk);
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
                     G.chunk(q, A.sc, mk);
@@ -1851,6 +1871,10 @@ static bs_status check_logits(const bs_logits *x, Scale *sc, float *out_scale, b
     *cap = x->final_logit_softcapping > 0.0f;
     sc->cap = *cap ? x->final_logit_softcapping : 1.0f;
     sc->icap = 1.0f / sc->cap;
+    const double k2 = -2.0 * 1.4426950408889634 / (double)sc->cap;
+    sc->k2 = (float)k2;
+    sc->k2_lo = (float)(k2 - (double)sc->k2);
+    sc->most = (float)fmin(64.0 * (double)sc->cap, 3.4e38);
     *out_scale = (float)(1.0 / scale);
     return BS_OK;
 }

@@ -190,3 +190,30 @@ def test_no_rest_is_left_out(gpu_pkg):
     assert bool(((got.grad.gather(1, ids.long()) - grad).abs() <= 8 * EPS).all())
     rest = got.grad.scatter(1, ids.long(), 0.0)
     assert not bool(rest.any()) and bool(torch.isfinite(rest).all())
+
+
+@pytest.mark.parametrize("cap", [30.0, 20.0, 50.0, 0.37, 1000.0])
+def test_soft_cap_is_as_exact_as_tanh(gpu_pkg, cap):
+    """c(v) is within 4 half steps of cap tanh(v / cap), 0.8 of one in the mean, and off to no side, as cap * tanhf(v / cap) is."""
+    # top_logits returns c(v) itself.  Half steps, |v| <= cap: the argument's product and 1 / cap 2, squared 5, felt by c at
+    # 0.23 at most; v y and the polynomial 3, on 0.31 of c; the last step 1: 3.3.  Beyond: the exponential 5 and its
+    # quotient 4, on 0.31 of c; the last step 1: 3.8.
+    cap32 = float(np.float32(cap))
+    g = torch.Generator(device="cuda").manual_seed(191)
+    for lo, hi, dtype in ((0.0, 0.5, torch.float32), (0.0, 1.0, torch.float32), (0.9, 1.5, torch.float32), (1.0, 9.0, torch.float32),
+                          (0.0, 1.0, torch.bfloat16)):
+        v = (lo + (hi - lo) * torch.rand(64, 1024, generator=g, device="cuda")) * cap32
+        v = (v * torch.where(torch.rand(v.shape, generator=g, device="cuda") < 0.5, -1.0, 1.0)).to(dtype)
+        got = gpu_pkg.top_logits(v, 1024, final_logit_softcapping=cap)
+        c = got.logits.double()
+        want = cap32 * torch.tanh(v.double().gather(1, got.ids.long()) / cap32)
+        some = want != 0
+        off = ((c - want) / want)[some] / EPS
+        f32 = (cap32 * torch.tanh(v.float().gather(1, got.ids.long()) / cap32)).double()
+        plain = ((f32 - want) / want)[some] / EPS
+        assert float(off.abs().max()) <= 4.0, (lo, hi, float(off.abs().max()))
+        assert float(off.square().mean().sqrt()) <= 1.15 * float(plain.square().mean().sqrt()), (lo, hi)
+        if dtype == torch.float32 and hi <= 1.0:
+            assert abs(float(off.mean())) <= 0.3, (lo, hi, float(off.mean()))
+        x = torch.tensor([[math.inf, -math.inf, 0.0, 1e30, -1e30]], device="cuda")
+        assert gpu_pkg.top_logits(x, 5, final_logit_softcapping=cap).logits.tolist() == [[cap32, cap32, 0.0, -cap32, -cap32]]
