@@ -133,10 +133,11 @@ __device__ __forceinline__ f2 cap_near(f2 v, const Scale &sc) {
     for (int i = 5; i >= 0; i--) w = fma2(w, y, both(TANH_W[i]));
     return fma2(mul2(v, y), w, v);
 }
-__device__ __forceinline__ float cap_far(float v, const Scale &sc) {
+__device__ __forceinline__ float cap_far(float v, const Scale &sc, float *slope = nullptr) {
     const float a = fminf(fabsf(v), sc.most), t = a * sc.k2;
     const float e = ex2(t) * fmaf(LN2, fmaf(a, sc.k2, -t) + a * sc.k2_lo, 1.0f);
-    const float q = 2.0f * e * rcp(1.0f + e);
+    const float r = rcp(1.0f + e), q = 2.0f * e * r;
+    if (slope) *slope = 2.0f * q * r;
     return copysignf(fmaf(-sc.cap, q, sc.cap), v);
 }
 template <bool CAP> __device__ __forceinline__ float capped(float v, const Scale &sc) {
@@ -145,15 +146,24 @@ template <bool CAP> __device__ __forceinline__ float capped(float v, const Scale
     return cap_near(both(v), sc).x;
 }
 
-// The soft-cap's slope 1 - (c / cap)^2.
-template <bool CAP> __device__ __forceinline__ f2 slope2(f2 c, const Scale &sc) {
+// The soft-cap's slope: 1 - (c / cap)^2 up to |v| = cap, where at least 0.42 is
+// left of it; beyond, where less and less would be, 4 e / (1 + e)^2.
+__device__ __forceinline__ f2 slope2(f2 c, const Scale &sc) {
     const f2 t = mul2(c, both(sc.icap));
     return fma2(mul2(t, both(-1.0f)), t, both(1.0f));
 }
-template <bool CAP> __device__ __forceinline__ float slope(float c, const Scale &sc) {
-    if (!CAP) return 1.0f;
-    float t = c * sc.icap;
-    return fmaf(-t, t, 1.0f);
+// The slope at one logit, and c(v) with it.
+__device__ __forceinline__ float cap_slope(float c, float v, const Scale &sc) {
+    float slope = slope2(both(c), sc).x;
+    if (fabsf(v) > sc.cap) cap_far(v, sc, &slope);
+    return slope;
+}
+template <bool CAP> __device__ __forceinline__ float2 cap_both(float v, const Scale &sc) {
+    if (!CAP) return make_float2(v, 1.0f);
+    float2 r = make_float2(cap_near(both(v), sc).x, 0.0f);
+    r.y = slope2(both(r.x), sc).x;
+    if (fabsf(v) > sc.cap) r.x = cap_far(v, sc, &r.y);
+    return r;
 }
 
 // A streaming read: the line is the first to leave L2 (and L1) again.
@@ -254,8 +264,17 @@ template <typename T> __device__ __forceinline__ float max_abs(uint4 q) {
         return max_of<T>(make_uint4(q.x & m, q.y & m, q.z & m, q.w & m));
     }
 }
+// Who wants to know of a logit above the soft-cap: `stamp` goes to *at.
+struct Note {
+    uint32_t *at;
+    uint32_t stamp;
+    __device__ __forceinline__ void put() const {
+        if (at) *at = stamp;
+    }
+};
 // A chunk's logits after the soft-cap.
-template <typename T, bool CAP> __device__ __forceinline__ void cap_chunk(const uint4 &q, f2 (&v)[8 / sizeof(T)], const Scale &sc) {
+template <typename T, bool CAP>
+__device__ __forceinline__ void cap_chunk(const uint4 &q, f2 (&v)[8 / sizeof(T)], const Scale &sc, const Note &note) {
     unpack<T>(q, v);
     if (!CAP) return;
     constexpr int N = 8 / sizeof(T);
@@ -263,6 +282,7 @@ template <typename T, bool CAP> __device__ __forceinline__ void cap_chunk(const 
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = cap_near(v[i], sc);
     if (far) {
+        note.put();
         f2 raw[N];
         unpack<T>(q, raw);
 #pragma unroll
@@ -271,6 +291,27 @@ template <typename T, bool CAP> __device__ __forceinline__ void cap_chunk(const 
             if (fabsf(raw[i].y) > sc.cap) v[i].y = cap_far(raw[i].y, sc);
         }
     }
+}
+// A chunk's elements one after the other through f: little code and few
+// registers, for what is rare.
+template <typename T, typename F> __device__ __forceinline__ uint4 each_of(uint4 q, F f) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll 1
+    for (int e = 0; e < (int)(16 / sizeof(T)); e++) {
+        // (the lowest element out, the result in at the top)
+        uint32_t in;
+        if constexpr (sizeof(T) == 4) {
+            in = __float_as_uint(f(__uint_as_float(w[0])));
+            w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = in;
+        } else {
+            float a, b;
+            halves(widen(w[0], T()), a, b);
+            in = narrow(pair(f(a), 0.0f), T());
+            w[0] = __funnelshift_r(w[0], w[1], 16), w[1] = __funnelshift_r(w[1], w[2], 16), w[2] = __funnelshift_r(w[2], w[3], 16);
+            w[3] = w[3] >> 16 | in << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // What a thread writes of a chunk where 16-byte stores do not fit.
 template <typename T> __device__ __forceinline__ void store_each(T *g, const uint4 &q) {
@@ -353,9 +394,9 @@ template <typename T, bool CAP, bool ENT> struct Gather {
         }
     }
     // (those in `marks` are left out)
-    __device__ __forceinline__ void chunk(const uint4 &q, const Scale &sc, uint32_t marks = 0) {
+    __device__ __forceinline__ void chunk(const uint4 &q, const Scale &sc, uint32_t marks = 0, Note note = {}) {
         f2 v[E / 2];
-        cap_chunk<T, CAP>(q, v, sc);
+        cap_chunk<T, CAP>(q, v, sc, note);
         if (CAP && marks) mask_out<T>(v, marks);
         chunk(v, sc.k);
     }
@@ -406,20 +447,30 @@ template <bool ENT> struct GradRow {
         const float l = fmaf(c - m, k, -l2s), p = ex2(l);
         return ENT ? p * fmaf(cb, max_nan(l, D_MIN), ca) : p * ca;
     }
-    // a chunk of it (DONE: q holds c(v) already)
+    // A chunk of it.
+    template <typename T, bool CAP> __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
+        if (CAP && max_abs<T>(q) > sc.cap)
+            return each_of<T>(q, [&](float v) {
+                const float2 c = cap_both<CAP>(v, sc);
+                return one(c.x) * c.y;
+            });
+        return near<T, CAP>(q, sc);
+    }
+    // The same where no logit lies above the soft-cap; DONE: q holds c(v) already.
     template <typename T, bool CAP, bool DONE = false>
-    __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
+    __device__ __forceinline__ uint4 near(const uint4 &q, const Scale &sc) const {
         constexpr int N = 8 / sizeof(T);
         f2 v[N], o[N];
-        cap_chunk<T, CAP && !DONE>(q, v, sc);
+        unpack<T>(q, v);
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            if (CAP && !DONE) v[i] = cap_near(v[i], sc);
             const f2 l = fma2(add2(v[i], both(-m)), both(k), both(-l2s));
             o[i] = mul2(ex2_2(l), ENT ? fma2(both(cb), floor2(l), both(ca)) : both(ca));
         }
         if (CAP) {
 #pragma unroll
-            for (int i = 0; i < N; i++) o[i] = mul2(o[i], slope2<CAP>(v[i], sc));
+            for (int i = 0; i < N; i++) o[i] = mul2(o[i], slope2(v[i], sc));
         }
         return pack<T>(o);
     }
@@ -473,7 +524,6 @@ template <bool ENT> struct GradRow {
 // half the slice each: 504.  A quarter of the ex2 as polynomials on the FMA
 // pipe: 399.
 constexpr uint32_t COPY = 512;       // chunks of one copy
-constexpr int STEP = 4;              // chunks of a thread summed at a time
 constexpr int MAX_CWARPS = 24;       // most warps S and G together
 constexpr int BTHREADS = 128;        // a warp for each of the four sets of slots
 constexpr int AHEAD = 4;             // slots of a lane that are loaded ahead
@@ -515,8 +565,8 @@ struct Teacher {
 // 16-bit types have twice the logits a byte and want more of both: 4096 x 128256
 // bf16 390 us with 512, 380 with 640, 389 with 768; 777 x 151936 f32 152 with
 // 512, 155 with 640.  Other shares than half: 394 with 352 of 640.  f32 under a
-// soft-cap leaves most of the work to S (see LEAVE): 512 x 256000 305 us with 384
-// of 512, 308 with 320.
+// soft-cap leaves most of the work to S (see LEAVE): policy loss 777 x 151936
+// 197 us with 384 of 512, 208 with 352, 249 with 416.
 template <typename T> __host__ __device__ constexpr int compute_threads() { return sizeof(T) == 4 ? 512 : 640; }
 template <typename T, bool CAP> __host__ __device__ constexpr int sum_threads_of() {
     return CAP && sizeof(T) == 4 ? 384 : compute_threads<T>() / 2;
@@ -525,6 +575,7 @@ struct RowsShared {
     float4 part[4][MAX_CWARPS];          // (m, s, u) of the warps S
     float4 mail[4][MAX_CLUSTER];     // and of the row's CTAs; two for each warp A
     Coef coef[4];
+    uint32_t far[4];                 // i + 1: row i has a logit above the soft-cap in the slice
     int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
     Teacher teacher[4];
     uint32_t edge_marks[4];          // the teacher's ids among the row's single elements
@@ -671,10 +722,10 @@ __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const 
 struct Slots {
     double *q;        // the slot's share, but for the row's scale
     int32_t *id;      // -1: empty; padded to a multiple of 4 with empty ones
-    float *c;         // the student's c(v) there
+    float *c, *v;     // the student's c(v) there and (under a soft-cap) v
     uint32_t *bits;   // one bit per element of the CTA's slice: named by the teacher
 };
-constexpr uint32_t SLOT_BYTES = 16;
+template <bool CAP> __host__ __device__ constexpr uint32_t slot_words() { return CAP ? 5 : 4; }
 __host__ __device__ __forceinline__ uint32_t slots_padded(uint32_t n_ids) { return (n_ids + 3u) & ~3u; }
 
 // Results and coefficients of a row with a teacher, in 64 bits as those of a
@@ -744,6 +795,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     const uint32_t z_threads = (grad ? GT : COMPUTE + 32) + 32 + (DIST ? 32 : 0);
     // f32 logits under a soft-cap: S leaves c(v) in the buffer, so that G need not work it out again
     constexpr bool LEAVE = CAP && sizeof(T) == 4;
+    // Chunks of a thread summed at a time.  Under a soft-cap, with 4 and 2: distillation 512 x 256000 f32 326 and 291 us,
+    // 2048 x 128256 bf16 409 and 387; policy loss 777 x 151936 f32 197 and 195, 2048 x 128256 bf16 388 and 398.
+    constexpr int STEP = CAP && (DIST || sizeof(T) == 4) ? 2 : 4;
     auto row_of = [&](uint32_t i) { return cluster + i * clusters; };
     auto weight = [&](uint32_t row) {
         return OP == OP_LOGPROB ? 1.0f : A.weights ? A.weights[row] : A.w_all;
@@ -764,7 +818,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         s.q = (double *)base + set * pad;
         s.id = (int32_t *)base + (8 + set) * pad;
         s.c = (float *)base + (12 + set) * pad;
-        s.bits = (uint32_t *)base + 16 * pad + set * A.bit_words;
+        s.v = (float *)base + (16 + set) * pad;
+        s.bits = (uint32_t *)base + 4 * slot_words<CAP>() * pad + set * A.bit_words;
         return s;
     };
 
@@ -781,6 +836,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     if (tid == 0) {
         for (int i = 0; i < 4; i++) bar_init(&sh.mail_bar[i]), bar_init(&sh.slots_bar[i]);
         for (int i = 0; i < 3; i++) bar_init(&sh.full_bar[i]);
+        for (int i = 0; i < 4; i++) sh.far[i] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -802,6 +858,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             if (++at == 3) at = 0, phase ^= 1;
             if (DIST) there = bar_wait(&sh.slots_bar[i & 3], i >> 2 & 1) && there;
             Gather<T, CAP, !DIST> G;
+            const Note note{CAP && grad ? &sh.far[i & 3] : nullptr, i + 1}, none{};
             if (sh.code[i & 15] >= 0) {
                 const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
                 auto marks = [&](uint32_t c) -> uint32_t {
@@ -811,8 +868,13 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 };
                 auto capped_chunk = [&](const uint4 &q) {
                     f2 v[E / 2];
-                    cap_chunk<T, CAP>(q, v, A.sc);
+                    cap_chunk<T, CAP>(q, v, A.sc, note);
                     return pack<T>(v);
+                };
+                // (a chunk's named tokens left out)
+                auto leave_out = [&](uint4 &q, uint32_t mk) {
+                    if (CAP && max_abs<T>(q) > A.sc.cap) note.put();
+                    mask_out<T>(q, mk);
                 };
                 // several chunks at a time, for one comparison with the running maximum
                 uint32_t c = tid;
@@ -839,19 +901,19 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     } else {
 #pragma unroll
                         for (int u = 0; u < STEP; u++)
-                            if (mk[u]) mask_out<T>(q[u], mk[u]);
+                            if (mk[u]) leave_out(q[u], mk[u]);
                         G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
 #pragma unroll
-                        for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, mk[u]);
+                        for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, mk[u], mk[u] ? none : note);
                     }
                 }
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
                     uint4 q = buf[0];
                     const uint32_t mk = marks(c);
                     if (LEAVE && grad) buf[0] = capped_chunk(q);
-                    if (mk) mask_out<T>(q, mk);
+                    if (mk) leave_out(q, mk);
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
-                    G.chunk(q, A.sc, mk);
+                    G.chunk(q, A.sc, mk, mk ? none : note);
                 }
                 // what did not fit
                 const T *x = R.at(sl.c0);
@@ -864,9 +926,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     for (int u = 0; u < STEP; u++)
                         if (c + u * sum_threads < count) {
                             const uint32_t mk = marks(c + u * sum_threads);
-                            if (mk) mask_out<T>(q[u], mk);
+                            if (mk) leave_out(q[u], mk);
                             G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
-                            G.chunk(q[u], A.sc, mk);
+                            G.chunk(q[u], A.sc, mk, mk ? none : note);
                         }
                 }
             }
@@ -900,24 +962,33 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             const Coef cf = sh.coef[i & 3];
             if (cf.live) {
                 const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
-                if (wide) {
-                    uint4 *o = reinterpret_cast<uint4 *>(out) + g;
-#pragma unroll 4
-                    for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT)
-                        *o = gr.template chunk<T, CAP, LEAVE>(*buf, A.sc);
-                } else {
-                    for (uint32_t c = g; c < copied; c += GT, buf += GT)
-                        store(c, gr.template chunk<T, CAP, LEAVE>(*buf, A.sc));
-                }
                 const T *x = R.at(sl.c0);
-                for (uint32_t c = copied + g; c < count; c += STEP * GT) {
-                    uint4 q[STEP];
+                if (CAP && __builtin_expect(sh.far[i & 3] == i + 1, 0)) {
+                    // (under LEAVE the logits themselves are needed: no other thread writes over this one's chunks)
+#pragma unroll 1
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT)
+                        store(c, gr.template chunk<T, CAP>(LEAVE ? ld_stream(x + (size_t)c * E) : *buf, A.sc));
+#pragma unroll 1
+                    for (uint32_t c = copied + g; c < count; c += GT) store(c, gr.template chunk<T, CAP>(ld_stream(x + (size_t)c * E), A.sc));
+                } else {
+                    if (wide) {
+                        uint4 *o = reinterpret_cast<uint4 *>(out) + g;
+#pragma unroll 4
+                        for (uint32_t c = g; c < copied; c += GT, buf += GT, o += GT)
+                            *o = gr.template near<T, CAP, LEAVE>(*buf, A.sc);
+                    } else {
+                        for (uint32_t c = g; c < copied; c += GT, buf += GT)
+                            store(c, gr.template near<T, CAP, LEAVE>(*buf, A.sc));
+                    }
+                    for (uint32_t c = copied + g; c < count; c += STEP * GT) {
+                        uint4 q[STEP];
 #pragma unroll
-                    for (int u = 0; u < STEP; u++)
-                        if (c + u * GT < count) q[u] = ld_stream(x + (size_t)(c + u * GT) * E);
+                        for (int u = 0; u < STEP; u++)
+                            if (c + u * GT < count) q[u] = ld_stream(x + (size_t)(c + u * GT) * E);
 #pragma unroll
-                    for (int u = 0; u < STEP; u++)
-                        if (c + u * GT < count) store(c + u * GT, gr.template chunk<T, CAP>(q[u], A.sc));
+                        for (int u = 0; u < STEP; u++)
+                            if (c + u * GT < count) store(c + u * GT, gr.template near<T, CAP>(q[u], A.sc));
+                    }
                 }
                 if (!DIST) {
                     // the token's own element, written again by the thread that wrote its chunk (where the token
@@ -1033,7 +1104,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 } else {
                     TokenIn in = cur.in;
                     in.c_tok = c_tok;
-                    in.slope = slope<CAP>(c_tok, A.sc);
+                    in.slope = cap_both<CAP>(to_f(cur.tok), A.sc).y;
                     cf = token_row<OP>(A, row, st, in, write);
                 }
             } else if (write) {
@@ -1047,7 +1118,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 float o = 0.0f;
                 if (live) {
                     const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
-                    o = !DIST && edge == sh.code[i & 15] ? cf.ct : gr.one(c_edge) * slope<CAP>(c_edge, A.sc);
+                    o = !DIST && edge == sh.code[i & 15] ? cf.ct : gr.one(c_edge) * cap_both<CAP>(to_f(cur.edge), A.sc).y;
                 }
                 ((T *)A.grad)[(size_t)row * A.ld_grad + edge] = from_f<T>(o);
             }
@@ -1151,6 +1222,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                             const float c = capped<CAP>(to_f(f.x[a]), A.sc);
                             sl.q[j] = (double)f.t[a];
                             sl.c[j] = c;
+                            if (CAP) sl.v[j] = to_f(f.x[a]);
                             most_t = max(most_t, order(f.t[a]));
                             most_c = max(most_c, order(c));
                         }
@@ -1236,9 +1308,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     if (v.w == id) q += sl.q[o + 3], first = first && o + 3 >= j;
                 }
                 if (!first) continue;
-                const float c = sl.c[j];
+                const float c = sl.c[j], slope = CAP ? cap_slope(c, sl.v[j], A.sc) : 1.0f;
                 const double p = exp_d(((double)c - u) * A.sc.md - cf.lse);
-                out[id] = from_f<T>((float)(cf.wm * (p * cf.q_all - q * scale)) * slope<CAP>(c, A.sc));
+                out[id] = from_f<T>((float)(cf.wm * (p * cf.q_all - q * scale)) * slope);
             }
         };
         fetch(set);
@@ -1316,15 +1388,14 @@ __global__ void __launch_bounds__(THREADS) k_logprob_grad(RowArgs A, uint32_t sl
             if (cu < c1) store(cu, gr.template chunk<T, CAP>(q[u], A.sc));
         }
     }
-    auto at_token = [&](float c) {
-        return token_grad(A.sc, c, stats[row], ENT ? entropy[row] : 0.0f, d_lp ? d_lp[row] : 0.0f, ENT ? d_ent[row] : 0.0f) *
-               slope<CAP>(c, A.sc);
+    auto at_token = [&](float2 c) {
+        return token_grad(A.sc, c.x, stats[row], ENT ? entropy[row] : 0.0f, d_lp ? d_lp[row] : 0.0f, ENT ? d_ent[row] : 0.0f) * c.y;
     };
     // the token's own element, written again by the thread that wrote its chunk
-    if (own) gout[tok] = from_f<T>(at_token(capped<CAP>(v_tok, A.sc)));
+    if (own) gout[tok] = from_f<T>(at_token(cap_both<CAP>(v_tok, A.sc)));
     if (edge >= 0) {
-        const float cv = capped<CAP>(to_f(R.x[edge]), A.sc);
-        gout[edge] = from_f<T>(edge == tok ? at_token(cv) : gr.one(cv) * slope<CAP>(cv, A.sc));
+        const float2 c = cap_both<CAP>(to_f(R.x[edge]), A.sc);
+        gout[edge] = from_f<T>(edge == tok ? at_token(c) : gr.one(c.x) * c.y);
     }
 }
 
@@ -2038,7 +2109,7 @@ static bs_status launch_row(RowArgs A, uint32_t rows, cudaStream_t st) {
     for (;; ranks *= 2, log_ranks++) {
         slice = (chunks + ranks - 1) / ranks;
         A.bit_words = is_distill(OP) ? (slice * E + 31) / 32 : 0;
-        slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 4 * SLOT_BYTES + (size_t)A.bit_words * 16 : 0;
+        slots = is_distill(OP) ? (size_t)slots_padded(A.n_ids) * 16 * slot_words<CAP>() + (size_t)A.bit_words * 16 : 0;
         room = slots < ROWS_SMEM ? (ROWS_SMEM - slots) / 48 : 0;
         // Enough CTAs to hold the row, and to use the GPU where the rows are few.  Sixteen only where eight cannot
         // hold it (seven such clusters fit the GPU, 112 SMs): 512 x 256000 f32 424 us, with eight and the rest of

@@ -217,3 +217,63 @@ def test_soft_cap_is_as_exact_as_tanh(gpu_pkg, cap):
             assert abs(float(off.mean())) <= 0.3, (lo, hi, float(off.mean()))
         x = torch.tensor([[math.inf, -math.inf, 0.0, 1e30, -1e30]], device="cuda")
         assert gpu_pkg.top_logits(x, 5, final_logit_softcapping=cap).logits.tolist() == [[cap32, cap32, 0.0, -cap32, -cap32]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("vocab,off", [(64, 0), (1003, 1), (40000, 3)])
+def test_gradient_where_the_soft_cap_saturates(gpu_pkg, dtype, vocab, off):
+    """Each gradient element holds its own bits where the slope 1 / cosh^2(v / cap) is small, up to 8 cap."""
+    cap, rows = 4.0, 4
+    g = torch.Generator(device="cuda").manual_seed(201)
+    x = torch.zeros(off + rows * vocab, dtype=dtype, device="cuda")[off:].view(rows, vocab)
+    x.copy_(cap * 16.0 * (torch.rand(rows, vocab, generator=g, device="cuda") - 0.5))
+    t = torch.tensor([0, vocab - 1, vocab // 2, 3], dtype=torch.int32, device="cuda")
+    x[0, 0], x[1, vocab - 1], x[2, vocab // 2], x[3, 3] = 7.5 * cap, -7.5 * cap, 0.99 * cap, 4.0 * cap
+    v = x.double()
+    slope = 1 / torch.cosh(v / cap) ** 2
+    z = cap * torch.tanh(v / cap)
+    logp = torch.log_softmax(z, 1)
+    p, H = logp.exp(), -(logp.exp() * logp).sum(1, keepdim=True)
+    hot = torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0)
+    # a term of the sum: d up to 8 log2(e) = 11.6, 3 R EPS; ex2 4; c off by 4 half steps of cap at most, twice; 8 rescalings
+    delta = EPS * (9 * (3 * 11.6 + 4 + 8 * cap) + vocab / 128 + 32)
+    w = torch.tensor([1.0, 0.5, -2.0, 1.0], device="cuda")
+    wd = w.double()[:, None]
+    half, tiny = torch.finfo(dtype).eps / 2, (2.0**-25 if dtype == torch.float16 else 2.0**-126)
+
+    def check(got, pre, size, what):
+        # the slope: t twice (4 half steps each) on at most 0.58 of it, over 0.42; beyond, the exponential's 5 and the
+        # quotient's 4, twice: 20 half steps with the products
+        out = pre * slope
+        tol = slope * (delta * size + 40 * EPS * size) + 1.01 * half * out.abs() + tiny
+        bad = (got.double() - out).abs() > tol
+        assert not bool(bad.any()), (what, int(bad.sum()), got.double()[bad][:4], out[bad][:4])
+
+    r = gpu_pkg.token_logprobs(x, t, final_logit_softcapping=cap)
+    got = gpu_pkg.token_logprobs_grad(x, t, r, w, 0.25 * w, final_logit_softcapping=cap)
+    size = wd.abs() * (hot + p + 0.25 * p * (3 * logp.abs() + 3 * H + 3))
+    check(got, wd * (hot - p) - 0.25 * wd * p * (logp + H), size, "log-probabilities")
+    lp = (hot * logp).sum(1)
+    got = gpu_pkg.policy_loss(x, t, lp.float(), torch.ones(rows, device="cuda"), None, w, final_logit_softcapping=cap).grad
+    ratio = (lp - lp.float().double()).exp()[:, None]
+    check(got, -wd * ratio * (hot - p), 3 * wd.abs() * (hot + p), "policy")
+    ids = torch.stack([torch.randperm(vocab, generator=g, device="cuda")[:9] for _ in range(rows)]).int()
+    ids[0, 0], ids[1, 0] = 0, vocab - 1
+    ids[0, 1:][ids[0, 1:] == 0] = -1
+    ids[1, 1:][ids[1, 1:] == vocab - 1] = -1
+    tl = torch.randn(rows, 9, generator=g, device="cuda")
+    lse = torch.logsumexp(tl, 1) + 0.7
+    valid = ids >= 0
+    for tail in (None, lse):
+        got = gpu_pkg.distill_loss(x, ids, tl, tail, w, final_logit_softcapping=cap).grad
+        u = torch.where(valid, tl.double(), -math.inf)
+        q = torch.softmax(u, 1) if tail is None else torch.where(valid, (u - tail.double()[:, None]).exp(), 0.0)
+        spread = torch.zeros_like(p).scatter_add_(1, ids.long().clamp_min(0), torch.where(valid, q, 0.0))
+        factor, big = torch.ones_like(p), torch.ones_like(p)
+        if tail is not None:
+            inside = torch.zeros_like(p).scatter_add_(1, ids.long().clamp_min(0), valid.double()) > 0
+            qr = 1 - q.sum(1, keepdim=True)
+            pr = torch.where(inside, 0.0, p).sum(1, keepdim=True)
+            factor = torch.where(inside, 1.0, 1 - qr / pr)
+            big = torch.where(inside, 1.0, 1 + qr / pr)
+        check(got, wd * (p * factor - spread), 3 * wd.abs() * (p * big + spread), ("distillation", tail is not None))
