@@ -370,10 +370,17 @@ __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.0f 
 
 // What a thread gathers of the logits it reads, on the scale of its running
 // maximum m: s = sum 2^d and (ENT) u = sum 2^d d in pairs (even and odd logits).
+// Terms are added up by chunks and steps of chunks (`part`) before they meet s:
+// once the row's largest logit is in s, every addition to it rounds off half a
+// step of 1, however small the term.
 template <typename T, bool CAP, bool ENT> struct Gather {
     static constexpr int E = 16 / sizeof(T);
     float m = -INFINITY;
-    f2 s = {0.0f, 0.0f}, u = {0.0f, 0.0f};
+    f2 s = {0.0f, 0.0f}, u = {0.0f, 0.0f}, part = {0.0f, 0.0f};
+    __device__ __forceinline__ void step() {
+        s = add2(s, part);
+        part = both(0.0f);
+    }
     __device__ __forceinline__ void raise(float to, float k) {
         if (to > m) {   // (fmaxf: from -inf there is nothing to rescale)
             const float d = fmaxf((m - to) * k, D_MIN), f = ex2(d);
@@ -385,13 +392,15 @@ template <typename T, bool CAP, bool ENT> struct Gather {
     // logits after the soft-cap, none above m (but for the soft-cap's rounding)
     __device__ __forceinline__ void chunk(const f2 (&v)[E / 2], float k) {
         const f2 base = both(-anchor(m)), kk = both(k);
+        f2 sum;
 #pragma unroll
         for (int i = 0; i < E / 2; i++) {
             const f2 d = mul2(add2(v[i], base), kk);
             const f2 e = ex2_2(d);
-            s = add2(s, e);
+            sum = i ? add2(sum, e) : e;
             if (ENT) u = fma2(e, floor2(d), u);
         }
+        part = add2(part, sum);
     }
     // (those in `marks` are left out)
     __device__ __forceinline__ void chunk(const uint4 &q, const Scale &sc, uint32_t marks = 0, Note note = {}) {
@@ -898,6 +907,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                             unpack<T>(q[u], v);
                             G.chunk(v, k);
                         }
+                        G.step();
                     } else {
 #pragma unroll
                         for (int u = 0; u < STEP; u++)
@@ -905,6 +915,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                         G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
 #pragma unroll
                         for (int u = 0; u < STEP; u++) G.chunk(q[u], A.sc, mk[u], mk[u] ? none : note);
+                        G.step();
                     }
                 }
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
@@ -914,6 +925,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     if (mk) leave_out(q, mk);
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
                     G.chunk(q, A.sc, mk, mk ? none : note);
+                    G.step();
                 }
                 // what did not fit
                 const T *x = R.at(sl.c0);
@@ -929,6 +941,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                             if (mk) leave_out(q[u], mk);
                             G.raise(capped<CAP>(max_of<T>(q[u]), A.sc), k);
                             G.chunk(q[u], A.sc, mk, mk ? none : note);
+                            G.step();
                         }
                 }
             }
@@ -1832,7 +1845,11 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
             if (!TOP) {
                 G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
 #pragma unroll
-                for (int u = 0; u < BATCH; u++) G.chunk(q[u], A.sc);
+                for (int u = 0; u < BATCH; u++) {
+                    G.chunk(q[u], A.sc);
+                    if (u == BATCH / 2 - 1) G.step();
+                }
+                G.step();
                 continue;
             }
         } else {
@@ -1840,16 +1857,19 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
             for (int u = 0; u < BATCH; u++)
                 if (b + u * THREADS + tid < c1) q[u] = ld_stream(body + (size_t)(b + u * THREADS + tid) * E);
         }
-        float mx[BATCH];
+        float mx[BATCH], big = -INFINITY;
 #pragma unroll
         for (int u = 0; u < BATCH; u++) {
-            mx[u] = -INFINITY;
-            if (b + u * THREADS + tid < c1) {
-                mx[u] = max_of<T>(q[u]);
-                G.raise(capped<CAP>(mx[u], A.sc), k);
-                G.chunk(q[u], A.sc);
-            }
+            mx[u] = b + u * THREADS + tid < c1 ? max_of<T>(q[u]) : -INFINITY;
+            big = fmaxf(big, mx[u]);
         }
+        G.raise(capped<CAP>(big, A.sc), k);
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            if (b + u * THREADS + tid < c1) G.chunk(q[u], A.sc);
+            if (u == BATCH / 2 - 1) G.step();
+        }
+        G.step();
         if (TOP) {
             // 8 x 8 transposing maximum: lane l of an 8-lane group ends up with
             // the maximum of batch step l & 7 over the group, one tile

@@ -277,3 +277,24 @@ def test_gradient_where_the_soft_cap_saturates(gpu_pkg, dtype, vocab, off):
             factor = torch.where(inside, 1.0, 1 - qr / pr)
             big = torch.where(inside, 1.0, 1 + qr / pr)
         check(got, wd * (p * factor - spread), 3 * wd.abs() * (p * big + spread), ("distillation", tail is not None))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows", [1, 600])
+def test_small_terms_beside_a_large_one(gpu_pkg, dtype, rows):
+    # one term of 1 and 131071 of 2^-25, which one by one round away against it (the row holds 3.9e-3 of them)
+    vocab, T = 131072, float(np.float32(1.0 / math.log(2.0)))
+    x = torch.full((rows, vocab), -25.0, dtype=dtype, device="cuda")
+    at = torch.arange(rows, device="cuda") * 211 % vocab
+    x[torch.arange(rows, device="cuda"), at] = 0.0
+    want = -math.log1p((vocab - 1) * math.exp(-25.0 / T))
+    # at most 16 terms that share a step with the large one are lost; then one rounding for each of the sum's folds: 5
+    # between a warp's lanes, 4 between warps, 3 between blocks, and the last chunk steps
+    tol = 16 * 2.0**-25 + 16 * EPS
+    r = gpu_pkg.token_logprobs(x, at.int(), temperature=T)
+    assert float((r.logprobs.double() - want).abs().max()) <= tol
+    top = gpu_pkg.top_logits(x, 3, temperature=T)
+    assert float((top.lse.double() + want).abs().max()) <= tol
+    one = torch.ones(rows, device="cuda")
+    p = gpu_pkg.policy_loss(x, at.int(), 0 * one, one, None, one, temperature=T)
+    assert float((p.logprobs.double() - want).abs().max()) <= tol
