@@ -203,6 +203,14 @@ def _like(logits, grad):
     return grad[0] if grad is not None and logits.dim() == 1 else grad
 
 
+def _written(out):
+    """Tells autograd that the kernel wrote over the caller's tensor, as an
+    in-place operation of torch's does: a backward that saved its old values
+    raises, and does not go by the new ones."""
+    if out is not None and not out.is_inference():   # (these have no version)
+        torch.autograd.graph.increment_version(out)
+
+
 def token_logprobs(logits, tokens, *, temperature: float = 1.0, final_logit_softcapping: float = 0.0,
                    logit_scale: float = 1.0, stream=None) -> TokenLogprobs:
     """Log-probability of each row's token and the row's entropy (bs_token_logprobs).
@@ -242,6 +250,7 @@ def token_logprobs_grad(logits, tokens, fwd: TokenLogprobs, grad_logprobs=None, 
         g, ld = r.grad_out(out)
         _s._check(_s.lib().bs_token_logprobs_grad(ctypes.byref(r.desc), t.data_ptr(), stats.data_ptr(), ent.data_ptr(),
                                                   _ptr(gl), _ptr(gh), g.data_ptr(), ld, st), "bs_token_logprobs_grad")
+        _written(out)
         return _like(logits, g)
 
     return r.run(call)
@@ -298,6 +307,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
         _s._check(_s.lib().bs_distill_loss(ctypes.byref(r.desc), ids.data_ptr(), tl.data_ptr(), _ptr(lse), shape[1],
                                            _ptr(w), loss.data_ptr(), rows.data_ptr(), _ptr(g), ld, st),
                   "bs_distill_loss")
+        if grad:
+            _written(out)
         return DistillLoss(loss, rows, _like(logits, g))
 
     return r.run(call)
@@ -335,6 +346,8 @@ def policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs=None, wei
         _s._check(_s.lib().bs_policy_loss(ctypes.byref(r.desc), t.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref),
                                           _ptr(w), ctypes.byref(cfg), p + 16 * n, p, p + 4 * n, p + 8 * n, p + 12 * n,
                                           _ptr(g), ld, st), "bs_policy_loss")
+        if grad:
+            _written(out)
         rows, lp, ent, kl, loss = buf.split_with_sizes((n, n, n, n, 1))
         return PolicyLoss(loss.squeeze(0), rows, lp, ent, kl, _like(logits, g))
 

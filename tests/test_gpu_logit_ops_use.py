@@ -1,0 +1,50 @@
+"""The vocabulary-row operators as parts of a user's program: autograd around them, ids of every type, streams of other
+devices, batches that go through the same blocks in place."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("call", ["logprobs", "policy", "distill"])
+def test_a_gradient_over_logits_that_autograd_saved(gpu_pkg, call):
+    # a z-loss saves the logits; with the gradient written over them its backward has to raise, not to go by the gradient
+    head = torch.randn(64, 4, device="cuda", requires_grad=True)
+    logits = torch.randn(3, 4, device="cuda") @ head.t()
+    z_loss = logits.logsumexp(-1).square().mean()
+    x = logits.detach()
+    t = torch.arange(3, dtype=torch.int32, device="cuda")
+    one = torch.ones(3, device="cuda")
+    before = logits._version
+    if call == "logprobs":
+        gpu_pkg.token_logprobs_grad(x, t, gpu_pkg.token_logprobs(x, t), one, out=x)
+    elif call == "policy":
+        gpu_pkg.policy_loss(x, t, -one, one, out=x)
+    else:
+        gpu_pkg.distill_loss(x, t[:, None], one[:, None], out=x)
+    assert logits._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z_loss.backward()
+    # without a gradient nothing is written, and a buffer of one's own is no concern of the logits
+    logits = torch.randn(3, 4, device="cuda") @ head.t()
+    z_loss = logits.logsumexp(-1).square().mean()
+    x = logits.detach()
+    gpu_pkg.policy_loss(x, t, -one, one, grad=False, out=x)
+    gpu_pkg.policy_loss(x, t, -one, one, out=torch.empty_like(x))
+    z_loss.backward()
+    assert head.grad is not None and bool(torch.isfinite(head.grad).all())
+    # one row, 1-D
+    row = torch.randn(40, device="cuda")
+    v = row._version
+    gpu_pkg.policy_loss(row, t[:1], -one[:1], one[:1], out=row)
+    assert row._version == v + 1
+
+
+def test_a_gradient_over_inference_tensors(gpu_pkg):
+    with torch.inference_mode():
+        x = torch.randn(3, 40, device="cuda")
+    t, one = torch.arange(3, dtype=torch.int32, device="cuda"), torch.ones(3, device="cuda")
+    want = gpu_pkg.policy_loss(x, t, -one, one).grad
+    assert torch.equal(gpu_pkg.policy_loss(x, t, -one, one, out=x).grad, want)
