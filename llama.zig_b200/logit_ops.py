@@ -162,6 +162,8 @@ class _Rows:
             raise ValueError(f"{what} must be an integer tensor on the logits' device")
         if tuple(t.shape) != shape and not (shape == (1,) and t.dim() == 0):
             raise ValueError(f"{what} must have shape {shape}")
+        if t.dtype == torch.uint64:
+            t = t.to(torch.int64)   # (2^63 and above become negative)
         if t.dtype == torch.int64:
             t = torch.where((t >= 0) & (t < 2**31), t, -1)
         if t.dtype not in (torch.int32, torch.uint32):

@@ -48,3 +48,15 @@ def test_a_gradient_over_inference_tensors(gpu_pkg):
     t, one = torch.arange(3, dtype=torch.int32, device="cuda"), torch.ones(3, device="cuda")
     want = gpu_pkg.policy_loss(x, t, -one, one).grad
     assert torch.equal(gpu_pkg.policy_loss(x, t, -one, one, out=x).grad, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.uint16, torch.int64, torch.uint32, torch.uint64], ids=str)
+def test_ids_of_every_type(gpu_pkg, dtype):
+    x = torch.randn(4, 100, device="cuda")
+    want = gpu_pkg.token_logprobs(x, torch.tensor([5, 99, 0, -1], dtype=torch.int32, device="cuda")).logprobs
+    # an id that no vocabulary holds leaves its row out, and is not cut down to one that it holds
+    far = {torch.int8: -1, torch.uint8: 200, torch.int16: -1, torch.uint16: 65535, torch.int64: 2**32 + 5, torch.uint32: 2**32 - 1,
+           torch.uint64: 2**32 + 5}[dtype]
+    for other in (far, 2**63 + 7) if dtype == torch.uint64 else (far,):
+        ids = torch.tensor([5, 99, 0, other], dtype=dtype).cuda()
+        assert torch.equal(gpu_pkg.token_logprobs(x, ids).logprobs, want), other
