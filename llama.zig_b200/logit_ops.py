@@ -130,7 +130,10 @@ class _Rows:
             with torch.cuda.device(index):
                 return call(_raw_stream(index))
         with torch.cuda.device(index):
-            if not isinstance(s, torch.cuda.Stream):
+            if isinstance(s, torch.cuda.Stream):
+                if s.device != self.device:
+                    raise ValueError("stream must be of the logits' device")
+            else:
                 ptr = int(getattr(s, "cuda_stream", s))
                 s = torch.cuda.ExternalStream(ptr, device=self.device) if ptr else torch.cuda.default_stream()
             with torch.cuda.stream(s):

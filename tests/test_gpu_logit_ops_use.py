@@ -60,3 +60,15 @@ def test_ids_of_every_type(gpu_pkg, dtype):
     for other in (far, 2**63 + 7) if dtype == torch.uint64 else (far,):
         ids = torch.tensor([5, 99, 0, other], dtype=dtype).cuda()
         assert torch.equal(gpu_pkg.token_logprobs(x, ids).logprobs, want), other
+
+
+def test_a_stream_of_another_device_is_refused(gpu_pkg):
+    class Elsewhere(torch.cuda.Stream):
+        device = property(lambda self: torch.device("cuda", 1))
+
+    x, t, one = torch.randn(3, 40, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda"), torch.ones(3, device="cuda")
+    s = Elsewhere()
+    for call in (lambda: gpu_pkg.token_logprobs(x, t, stream=s), lambda: gpu_pkg.top_logits(x, 2, stream=s),
+                 lambda: gpu_pkg.policy_loss(x, t, one, one, stream=s), lambda: gpu_pkg.distill_loss(x, t[:, None], one[:, None], stream=s)):
+        with pytest.raises(ValueError, match="device"):
+            call()
