@@ -251,9 +251,10 @@ bs_status bs_sample_static(const bs_config *cfg, uint64_t *d_rng, const float *d
  * the sizes and the alignment: the same call gives the same bits.
  *
  * Logits of -inf are masked tokens (p = 0, gradient 0), a +inf logit makes its
- * row NaN, a row all of -inf has no distribution and is NaN too (all three
- * without a soft-cap, which makes +-cap of them); a NaN makes its row NaN.  So
- * does a bounded device wait that gave up.  Gradients are of the logits' type, rounded once from f32;
+ * row NaN, a row all of -inf has no distribution and is NaN too, with an lse of
+ * -inf (all three without a soft-cap, which makes +-cap of them); a NaN makes
+ * its row NaN.  So does a bounded device wait that gave up.  Gradients are of
+ * the logits' type, rounded once from f32;
  * d_grad may be the logits themselves (same pointer, ld_grad = ld) and must
  * not overlap them in any other way. */
 typedef enum bs_dtype { BS_F32 = 0, BS_BF16 = 1, BS_F16 = 2 } bs_dtype;
@@ -307,7 +308,8 @@ bs_status bs_top_logits(const bs_logits *x, uint32_t k, float *d_values, int32_t
  *   d_weights : rows, or NULL for 1 / rows each
  *   d_row_loss: the L_i;  d_grad: NULL, or d loss / d logits
  * A row of weight 0 or without a teacher id (or, where q is a softmax, all of
- * whose teacher logits are -inf) is left out: zeros. */
+ * whose teacher logits are -inf) is left out: zeros.  A teacher's lse of -inf
+ * says that its row has no distribution: the row is NaN. */
 bs_status bs_distill_loss(const bs_logits *x, const int32_t *d_teacher_ids, const float *d_teacher_logits,
                           const float *d_teacher_lse, uint32_t n_ids, const float *d_weights, float *d_loss,
                           float *d_row_loss, void *d_grad, size_t ld_grad, void *stream);

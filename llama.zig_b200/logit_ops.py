@@ -265,7 +265,8 @@ def top_logits(logits, k: int, *, temperature: float = 1.0, final_logit_softcapp
                logit_scale: float = 1.0, stream=None) -> TopLogits:
     """The k largest logits of each row in falling order (the lowest id first
     among equals) with their ids, and the row's normaliser (bs_top_logits).
-    ``logits / temperature - lse[:, None]`` are their log-probabilities."""
+    ``logits / temperature - lse[:, None]`` are their log-probabilities.  A row
+    all of -inf has an lse of -inf."""
     r = _Rows(logits, temperature, final_logit_softcapping, logit_scale, stream)
     if not 1 <= int(k) <= min(r.vocab, MAX_TOP):
         raise ValueError(f"k must be between 1 and the vocabulary (and {MAX_TOP})")

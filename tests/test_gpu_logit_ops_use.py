@@ -72,3 +72,25 @@ def test_a_stream_of_another_device_is_refused(gpu_pkg):
                  lambda: gpu_pkg.policy_loss(x, t, one, one, stream=s), lambda: gpu_pkg.distill_loss(x, t[:, None], one[:, None], stream=s)):
         with pytest.raises(ValueError, match="device"):
             call()
+
+
+@pytest.mark.parametrize("vocab", [7, 5000, 128256])
+def test_a_row_without_a_distribution(gpu_pkg, vocab):
+    # all masked: lse is -inf as a logsumexp, and whoever takes the row for a teacher with a tail gets NaN, not zeros
+    x = torch.randn(3, vocab, device="cuda")
+    x[1] = -math.inf
+    top = gpu_pkg.top_logits(x, 5)
+    assert torch.equal(top.lse == -math.inf, torch.tensor([False, True, False], device="cuda"))
+    assert top.ids[1].tolist() == [0, 1, 2, 3, 4] and bool((top.logits[1] == -math.inf).all())
+    t = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    lp = gpu_pkg.token_logprobs(x, t)
+    assert lp.logprobs.isnan().tolist() == [False, True, False] and lp.entropy.isnan().tolist() == [False, True, False]
+    y = torch.randn(3, vocab, device="cuda")
+    w = torch.ones(3, device="cuda")
+    r = gpu_pkg.distill_loss(y, top.ids, top.logits, top.lse, w)
+    assert r.row_losses.isnan().tolist() == [False, True, False] and bool(r.grad[1].isnan().all())
+    assert not bool(r.grad[0].isnan().any()) and not bool(r.grad[2].isnan().any())
+    assert float(gpu_pkg.distill_loss(y, top.ids, top.logits, None, w).row_losses[1]) == 0.0
+    w[1] = 0.0
+    r = gpu_pkg.distill_loss(y, top.ids, top.logits, top.lse, w)
+    assert bool(torch.isfinite(r.loss)) and not bool(r.grad[1].any()) and float(r.row_losses[1]) == 0.0
