@@ -134,8 +134,8 @@ __device__ __forceinline__ f2 cap_near(f2 v, const Scale &sc) {
     return fma2(mul2(v, y), w, v);
 }
 __device__ __forceinline__ float cap_far(float v, const Scale &sc, float *slope = nullptr) {
-    const float a = fminf(fabsf(v), sc.most), t = a * sc.k2;
-    const float e = ex2(t) * fmaf(LN2, fmaf(a, sc.k2, -t) + a * sc.k2_lo, 1.0f);
+    const float a = fabsf(v), t = a * sc.k2;
+    const float e = a >= sc.most ? 0.0f : ex2(t) * fmaf(LN2, fmaf(a, sc.k2, -t) + a * sc.k2_lo, 1.0f);
     const float r = rcp(1.0f + e), q = 2.0f * e * r;
     if (slope) *slope = 2.0f * q * r;
     return copysignf(fmaf(-sc.cap, q, sc.cap), v);
@@ -1961,11 +1961,12 @@ static bs_status check_logits(const bs_logits *x, Scale *sc, float *out_scale, b
     sc->inv_t = 1.0 / (double)x->temperature;
     *cap = x->final_logit_softcapping > 0.0f;
     sc->cap = *cap ? x->final_logit_softcapping : 1.0f;
-    sc->icap = 1.0f / sc->cap;
-    const double k2 = -2.0 * 1.4426950408889634 / (double)sc->cap;
+    // (a cap below 2^-126 has reciprocals past f32)
+    sc->icap = (float)fmin(1.0 / (double)sc->cap, 3.4e38);
+    const double k2 = fmax(-2.0 * 1.4426950408889634 / (double)sc->cap, -3.4e38);
     sc->k2 = (float)k2;
     sc->k2_lo = (float)(k2 - (double)sc->k2);
-    sc->most = (float)fmin(64.0 * (double)sc->cap, 3.4e38);
+    sc->most = 64.0f * sc->cap;
     *out_scale = (float)(1.0 / scale);
     return BS_OK;
 }

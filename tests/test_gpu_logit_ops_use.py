@@ -94,3 +94,21 @@ def test_a_row_without_a_distribution(gpu_pkg, vocab):
     w[1] = 0.0
     r = gpu_pkg.distill_loss(y, top.ids, top.logits, top.lse, w)
     assert bool(torch.isfinite(r.loss)) and not bool(r.grad[1].any()) and float(r.row_losses[1]) == 0.0
+
+
+def test_soft_caps_at_the_ends_of_f32(gpu_pkg):
+    # no cap is refused but NaN and infinity; 1 / cap is past f32 for the smallest
+    x = torch.tensor([[0.0, 1.0, -1.0, 30.0, math.inf, -math.inf, 1e-42, -0.0]], device="cuda")
+    one = torch.ones(1, device="cuda")
+    for cap in (1e-45, 1e-40, 1.5e-38, 1e-30, 1e30, 3e38):
+        top = gpu_pkg.top_logits(x, 8, final_logit_softcapping=cap)
+        c = float(torch.tensor(cap, dtype=torch.float32))
+        want = c * torch.tanh(x.double() / c).gather(1, top.ids.long())
+        want = torch.where(x.gather(1, top.ids.long()).isinf(), torch.sign(want) * c, want)
+        assert bool(((top.logits.double() - want).abs() <= 4 * 2.0**-24 * want.abs() + 2.0**-148).all()), (cap, top.logits, want)
+        t = torch.zeros(1, dtype=torch.int32, device="cuda")
+        r = gpu_pkg.token_logprobs(x, t, final_logit_softcapping=cap)
+        if cap < 1.0:      # eight equal ones, as far as exp can tell
+            assert abs(float(r.logprobs) + math.log(8.0)) <= 8 * 2.0**-24
+            g = gpu_pkg.token_logprobs_grad(x, t, r, one, final_logit_softcapping=cap)
+            assert bool(torch.isfinite(g).all()) and abs(float(g[0, 0]) - 0.875) <= 8 * 2.0**-24
