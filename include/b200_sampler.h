@@ -333,6 +333,11 @@ bs_status bs_policy_loss(const bs_logits *x, const int32_t *d_tokens, const floa
                          const bs_policy_config *cfg, float *d_loss, float *d_row_loss, float *d_logprobs,
                          float *d_entropy, float *d_kl, void *d_grad, size_t ld_grad, void *stream);
 
+/* BS_ETIMEOUT if a bounded device wait of one of these operators gave up on the
+ * current device since the last such call (its rows are NaN from there on, those
+ * of one thread block in part), BS_OK if none did.  Waits for the device. */
+bs_status bs_logit_ops_status(void);
+
 void bs_destroy(bs_sampler *s);
 
 const char *bs_status_string(bs_status st);

@@ -18,8 +18,8 @@ The directory name contains a dot, so it is loaded by path, e.g.::
 """
 from . import build, sharding, workloads  # noqa: F401
 from .logit_ops import (  # noqa: F401
-    DistillLoss, PolicyLoss, TokenLogprobs, TopLogits, distill_loss, policy_loss, token_logprobs, token_logprobs_grad,
-    top_logits,
+    DistillLoss, PolicyLoss, TokenLogprobs, TopLogits, distill_loss, logit_ops_status, policy_loss, token_logprobs,
+    token_logprobs_grad, top_logits,
 )
 from .sampler import (  # noqa: F401
     EXPORTS, Sampler, SamplerConfig, SamplerError, lib, sample_argmax, status_string,

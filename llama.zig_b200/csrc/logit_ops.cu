@@ -56,6 +56,8 @@ struct RowArgs {
     uint32_t bit_words;         // with a teacher: words of one bit per element of a slice
     Scale sc;
     const int32_t *tokens;
+    long long wait_limit;       // clock cycles
+    uint32_t gone_rank, gone_row;   // (for tests) the CTA of a row whose waits give up, from a cluster's i-th row on
     // outputs (null where not asked for)
     float *logprobs, *entropy, *kl, *row_loss;
     float2 *stats;
@@ -559,7 +561,7 @@ struct Coef {
     float m, l2s;        // maximum, log2 S
     float ca, cb;        // dv_j = c'(v_j) p_j (ca + cb log2 p_j)
     float ct;            // the token's dv
-    uint32_t live;       // 0: the row is left out
+    uint32_t live;       // 0: the row is left out; 2: lost, a wait gave up
     double lse, q_all, wm;   // teacher's ids: wm c'(v_j) (p_j q_all - q_j), log p_j = (c(v_j) - U) m - lse
 };
 // What the warps B sum of a row's slots, in 64 bits.
@@ -585,6 +587,10 @@ struct RowsShared {
     float4 mail[4][MAX_CLUSTER];     // and of the row's CTAs; two for each warp A
     Coef coef[4];
     uint32_t far[4];                 // i + 1: row i has a logit above the soft-cap in the slice
+    uint32_t gone;                   // a wait of this CTA gave up
+    uint32_t passed;                 // rows that C has seen through Z
+    uint32_t sent[2][MAX_CLUSTER];   // at the end: exchanges that the CTAs' warps A have sent into,
+    uint32_t failed[2];              // and whether this CTA's gave up on its last
     int32_t code[16];                // the row's token (0 for a teacher's row); -1: left out
     Teacher teacher[4];
     uint32_t edge_marks[4];          // the teacher's ids among the row's single elements
@@ -627,9 +633,15 @@ __device__ __forceinline__ void mail_send(const float4 *slot, const uint64_t *ba
                  "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(remote(bar, rank)), "r"(__float_as_uint(v.w))
                  : "memory");
 }
-// Waits for all bytes of a phase; false if it gave up (a second at the least).
-__device__ __forceinline__ bool bar_wait(const uint64_t *bar, uint32_t parity) {
-    for (uint32_t tries = 0; tries < (1u << 24); tries++) {
+// Takes bytes off what a phase waits for: those that nobody will send.
+__device__ __forceinline__ void bar_forgo(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+// Waits for a phase; false if it gave up, after `limit` clock cycles or because
+// another wait of the CTA had (`gone`).
+__device__ __forceinline__ bool bar_wait(const uint64_t *bar, uint32_t parity, long long limit, const volatile uint32_t *gone) {
+    long long start = 0;
+    for (uint32_t tries = 0;; tries++) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -637,9 +649,14 @@ __device__ __forceinline__ bool bar_wait(const uint64_t *bar, uint32_t parity) {
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
         if (done) return true;
+        const long long now = clock64();
+        if (tries == 0) start = now;
+        if (now - start > limit || (gone && *gone)) return false;
     }
-    return false;
 }
+constexpr long long WAIT_LIMIT = 1ll << 32;   // two seconds
+// Set by a wait that gave up, until the host asks (bs_logit_ops_status).
+__device__ uint32_t wait_gave_up;
 
 // Results and coefficients of a row with a token.  A few values a row, so all
 // in 64 bits from the f32 sums: a ratio near 1, a KL near 0 and a loss whose
@@ -845,6 +862,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     if (tid == 0) {
         for (int i = 0; i < 4; i++) bar_init(&sh.mail_bar[i]), bar_init(&sh.slots_bar[i]);
         for (int i = 0; i < 3; i++) bar_init(&sh.full_bar[i]);
+        sh.gone = sh.passed = 0u;
         for (int i = 0; i < 4; i++) sh.far[i] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -853,6 +871,18 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         cluster_arrive();
         cluster_wait();
     }
+
+    // A wait that gives up is the CTA's last: from there on it starts no copies and no exchanges, and its rows are NaN.
+    // (The other CTAs of the row then miss its mail, and give up too.)  All warps still go through all rows and meet at
+    // the barriers, so that none is left waiting.
+    const volatile uint32_t *const gone = &sh.gone;
+    const uint32_t give_up = rank == A.gone_rank ? A.gone_row : 0xFFFFFFFFu;
+    auto wait = [&](const uint64_t *bar, uint32_t parity, uint32_t i) {
+        if (i < give_up && bar_wait(bar, parity, A.wait_limit, gone)) return true;
+        *const_cast<volatile uint32_t *>(gone) = 1u;
+        *const_cast<volatile uint32_t *>(&wait_gave_up) = 1u;
+        return false;
+    };
 
     if (tid < sum_threads) {
         // ---- warps S; thread tid has the chunks tid, tid + sum_threads, ... of the slice
@@ -863,12 +893,19 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             const Slice sl = slice_of(R);
             const uint32_t count = sl.c1 - sl.c0, copied = min(count, A.keep);
             uint4 *buf = dyn + at * A.keep + tid;
-            there = bar_wait(&sh.full_bar[at], phase) && there;
+            there = there && wait(&sh.full_bar[at], phase, i);
             if (++at == 3) at = 0, phase ^= 1;
-            if (DIST) there = bar_wait(&sh.slots_bar[i & 3], i >> 2 & 1) && there;
+            if (DIST) there = there && wait(&sh.slots_bar[i & 3], i >> 2 & 1, i);
+            if (!there) {
+                // without copies to wait for: not further ahead of the other warps than with them
+                const volatile uint32_t *const passed = &sh.passed;
+                const long long start = clock64();
+                while (*passed + 2 < i && clock64() - start < WAIT_LIMIT) __nanosleep(200);
+            }
+            there = __all_sync(~0u, there);
             Gather<T, CAP, !DIST> G;
             const Note note{CAP && grad ? &sh.far[i & 3] : nullptr, i + 1}, none{};
-            if (sh.code[i & 15] >= 0) {
+            if (there && sh.code[i & 15] >= 0) {
                 const uint32_t *bits = TAIL ? slots(i).bits : nullptr;
                 auto marks = [&](uint32_t c) -> uint32_t {
                     if (!TAIL) return 0u;
@@ -948,9 +985,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             // (the buffer is written by copies again)
             if (LEAVE && grad) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             Stat st{-INFINITY, 0.0f, 0.0f};
-            if (sh.code[i & 15] >= 0) st = fold_lanes<!DIST, 32>(G.stat(), k);
-            // (a copy that never came: the row is NaN)
-            if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, there ? st.s : NAN, st.u, 0.0f);
+            if (there && sh.code[i & 15] >= 0) st = fold_lanes<!DIST, 32>(G.stat(), k);
+            if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, st.s, st.u, there ? 0.0f : 1.0f);
             bar_arrive(BAR_X + (i & 3), x_threads);
             if (!grad) bar_arrive(BAR_Z + (i & 3), z_threads);
         }
@@ -973,7 +1009,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             };
             bar_sync(BAR_Y + (i & 3), y_threads);
             const Coef cf = sh.coef[i & 3];
-            if (cf.live) {
+            if (cf.live == 1u) {
                 const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
                 const T *x = R.at(sl.c0);
                 if (CAP && __builtin_expect(sh.far[i & 3] == i + 1, 0)) {
@@ -1010,8 +1046,11 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     const uint32_t t = t_at / E, mine = t < copied ? t : t - copied;
                     if (t < count && mine % GT == g) out[t_at] = from_f<T>(cf.ct);
                 }
-            } else {   // the row is left out: zeros
-                for (uint32_t c = g; c < count; c += GT) store(c, make_uint4(0, 0, 0, 0));
+            } else {   // the row is left out: zeros; or lost: NaN
+                f2 v[E / 2];
+                for (int e = 0; e < E / 2; e++) v[e] = both(cf.live ? NAN : 0.0f);
+                const uint4 fill = pack<T>(v);
+                for (uint32_t c = g; c < count; c += GT) store(c, fill);
             }
             bar_arrive(BAR_Z + (i & 3), z_threads);
         }
@@ -1054,6 +1093,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
         };
         load4(which);
         uint32_t sent = 0;        // exchanges of this warp so far
+        bool failed = false, stopped = false;   // its last one gave up; or what S waited for did
         for (uint32_t i = which; i < n; i += 2) {
             const Params cur = next;
             const uint32_t row = row_of(i);
@@ -1061,16 +1101,20 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             if (lane == 0 && i + 4 < n) sh.code[(i + 4) & 15] = w4 != 0.0f && (uint32_t)t4 < V ? t4 : -1;
             load4(i + 2);
             bar_sync(BAR_X + (i & 3), x_threads);
-            bool live = sh.code[i & 15] >= 0;
-            if (DIST && live) live = sh.teacher[i & 3].live != 0u;
             const int32_t edge = edge_of(i);
             const float c_edge = capped<CAP>(to_f(cur.edge), A.sc);
             const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(cur.tok), A.sc);
             Stat st{-INFINITY, 0.0f, 0.0f};
+            bool gave_up = false;
             if (lane < sum_threads / 32) {
                 const float4 f = sh.part[i & 3][lane];
                 st = Stat{f.x, f.y, f.z};
+                gave_up = f.w != 0.0f;
             }
+            stopped = __any_sync(~0u, gave_up || stopped);
+            const bool wanted = sh.code[i & 15] >= 0;
+            bool lost = wanted && stopped, live = wanted && !lost;
+            if (DIST && live) live = sh.teacher[i & 3].live != 0u;
             if (!grad && !DIST) bar_arrive(BAR_Z + (i & 3), z_threads);   // the sums are read: S may go on
             if (live && edge >= 0 && !(TAIL && (sh.edge_marks[i & 3] >> lane & 1u))) {
                 // one logit: 2^0 at itself, nothing where it is -inf (or a sum of NaN)
@@ -1081,7 +1125,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             }
             st = fold_lanes<!DIST, 32>(st, k);
             double top = TAIL && live ? sh.teacher[i & 3].top : 0.0;
-            if (ranks > 1 && sh.code[i & 15] >= 0) {
+            if (ranks > 1 && wanted && !lost) {
                 // The rows that take part in an exchange count the same in every CTA.  A warp's exchanges take turns
                 // with two boxes: a CTA sends into one only after all have sent into the other, so have read what
                 // was in this one.  The token's logit goes along so that it has been read before another CTA may
@@ -1092,12 +1136,14 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 if (TAIL) out.z = __int_as_float(__double2loint(top)), out.w = __int_as_float(__double2hiint(top));
                 if (lane < ranks) mail_send(&sh.mail[box][rank], &sh.mail_bar[box], lane, out);
                 if (lane == 0) bar_expect(&sh.mail_bar[box], ranks * 16);
-                const bool there = bar_wait(&sh.mail_bar[box], turn);
+                lost = !__all_sync(~0u, wait(&sh.mail_bar[box], turn, i));
+                live = live && !lost;
+                failed = stopped = lost;
                 st = Stat{-INFINITY, 0.0f, 0.0f};
                 top = 0.0;
                 if (lane < ranks) {
                     const float4 f = sh.mail[box][lane];
-                    st = Stat{f.x, there ? f.y : NAN, f.z};   // (a CTA that never sent: the row is NaN)
+                    st = Stat{f.x, f.y, f.z};
                     if (TAIL) top = __hiloint2double(__float_as_int(f.w), __float_as_int(f.z));
                 }
                 if (TAIL) {
@@ -1120,15 +1166,18 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     in.slope = cap_both<CAP>(to_f(cur.tok), A.sc).y;
                     cf = token_row<OP>(A, row, st, in, write);
                 }
-            } else if (write) {
-                if (A.logprobs) A.logprobs[row] = 0.0f;
-                if (A.entropy) A.entropy[row] = 0.0f;
-                if (A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
-                if (A.kl) A.kl[row] = 0.0f;
-                if (A.row_loss) A.row_loss[row] = 0.0f;
+            } else {
+                const float none = lost ? NAN : 0.0f;
+                if (write) {
+                    if (A.logprobs) A.logprobs[row] = none;
+                    if (A.entropy) A.entropy[row] = none;
+                    if (A.kl) A.kl[row] = none;
+                    A.row_loss[row] = none;
+                }
+                if (lost) cf.live = 2u;
             }
             if (grad && edge >= 0) {
-                float o = 0.0f;
+                float o = lost ? NAN : 0.0f;
                 if (live) {
                     const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
                     o = !DIST && edge == sh.code[i & 15] ? cf.ct : gr.one(c_edge) * cap_both<CAP>(to_f(cur.edge), A.sc).y;
@@ -1140,6 +1189,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             if (grad) bar_arrive(BAR_Y + (i & 3), y_threads);
             else if (DIST) bar_arrive(BAR_Z + (i & 3), z_threads);   // (done with the slots)
         }
+        if (lane < ranks)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(&sh.sent[which][rank], lane)), "r"(sent) : "memory");
+        if (lane == 0) sh.failed[which] = failed;
     } else if (tid < COMPUTE + 96) {
         // ---- warp C: row i + 3 into row i's buffer
         auto copy = [&](uint32_t i) {
@@ -1153,13 +1205,15 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             for (uint32_t c = lane * COPY; c < copied; c += 32 * COPY)
                 copy_bulk(buf + c, R.at(sl.c0 + c), min(copied - c, COPY) * 16, bar);
         };
-        for (uint32_t i = 0; i < 3 && i < n; i++) copy(i);
+        uint32_t started = 0;
+        for (; started < 3 && started < n; started++) copy(started);
         for (uint32_t i = 0; i < n; i++) {
             bar_sync(BAR_Z + (i & 3), z_threads);
-            if (i + 3 < n) copy(i + 3);
+            if (lane == 0) *const_cast<volatile uint32_t *>(&sh.passed) = i + 1;
+            if (i + 3 < n && !__any_sync(~0u, *gone != 0u)) copy(started++);
         }
         // (S has seen every copy land; were it to have given up on one, it still lands before the CTA's memory goes)
-        for (uint32_t i = n > 3 ? n - 3 : 0; i < n; i++) bar_wait(&sh.full_bar[i % 3], i / 3 & 1);
+        for (uint32_t i = started > 3 ? started - 3 : 0; i < started; i++) bar_wait(&sh.full_bar[i % 3], i / 3 & 1, WAIT_LIMIT, nullptr);
     } else if constexpr (DIST) {
         // ---- warps B; warp w has the rows w, w + 4, ..., and the set w of slots
         const uint32_t set = (tid - COMPUTE - 96) >> 5;
@@ -1308,7 +1362,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 const uint32_t e = (uint32_t)id - e0;
                 if (!mine(id, R, e0, span)) continue;
                 if (e < span) sl.bits[e >> 5] = 0u;
-                if (!grad) continue;
+                if (!grad || cf.live != 1u) continue;
                 // p Q - q, where q is the sum over the slots that hold the id (the first of them writes)
                 double q = sl.q[j];
                 bool first = true;
@@ -1336,6 +1390,25 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             fetch_row_logits(i + 4);
             finish(i);
             __syncwarp();
+        }
+    }
+    // No CTA's memory goes while another's mail may be on its way: all have sent what they will, and who gave up waits for
+    // what was sent all the same (who did not has seen it).
+    if (ranks > 1) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (tid >= COMPUTE && tid < COMPUTE + 4 && *gone) {
+            const uint32_t box = tid - COMPUTE, which = box >> 1, odd = box & 1;
+            auto into = [&](uint32_t sent) { return (sent + 1 - odd) / 2; };   // of a warp's exchanges, those in this box
+            const uint32_t mine = sh.sent[which][rank];
+            const bool armed = sh.failed[which] && ((mine - 1) & 1) == odd;    // the one it gave up on
+            const uint32_t seen = into(mine) - (armed ? 1 : 0);
+            uint32_t left = 0;
+            for (uint32_t r = 0; r < ranks; r++) left += (into(sh.sent[which][r]) - seen) * 16;
+            if (armed && left < ranks * 16) bar_forgo(&sh.mail_bar[box], ranks * 16 - left);
+            if (!armed && left) bar_expect(&sh.mail_bar[box], left);
+            if (armed || left) bar_wait(&sh.mail_bar[box], seen & 1, WAIT_LIMIT, nullptr);
         }
     }
 }
@@ -2176,8 +2249,14 @@ static bs_status launch_row_typed(const bs_logits *x, const RowArgs &A, bool cap
     }
 }
 
+static std::atomic<long long> wait_limit{WAIT_LIMIT};
+static std::atomic<uint32_t> gone_rank{0xFFFFFFFFu}, gone_row{0};
+
 static RowArgs row_args(const bs_logits *x, const Scale &sc) {
     RowArgs A = {};
+    A.wait_limit = wait_limit.load(std::memory_order_relaxed);
+    A.gone_rank = gone_rank.load(std::memory_order_relaxed);
+    A.gone_row = gone_row.load(std::memory_order_relaxed);
     A.x = x->data;
     A.ld = x->ld;
     A.vocab = x->vocab;
@@ -2203,6 +2282,26 @@ static bs_status no_rows(float *d_loss, void *stream) {
 }  // namespace bs
 
 using namespace bs::ops;
+
+extern "C" bs_status bs_logit_ops_status(void) {
+    uint32_t gave_up = 0;
+    const uint32_t zero = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&gave_up, wait_gave_up, sizeof(gave_up)) != cudaSuccess ||
+        (gave_up && cudaMemcpyToSymbol(wait_gave_up, &zero, sizeof(zero)) != cudaSuccess)) {
+        cudaGetLastError();
+        return BS_ECUDA;
+    }
+    return gave_up ? BS_ETIMEOUT : BS_OK;
+}
+
+// For tests of what follows a wait that gives up: the waits' limit in clock
+// cycles (0: as it is without this call), and a CTA of the clusters whose waits
+// give up at once from its row-th row on (rank 0xFFFFFFFF: none).
+extern "C" void bs_debug_logit_ops_waits(uint64_t cycles, uint32_t rank, uint32_t row) {
+    wait_limit.store(cycles && cycles < (uint64_t)WAIT_LIMIT ? (long long)cycles : WAIT_LIMIT);
+    gone_rank.store(rank);
+    gone_row.store(row);
+}
 
 extern "C" bs_status bs_token_logprobs(const bs_logits *x, const int32_t *d_tokens, float *d_logprobs, float *d_entropy,
                                        float *d_stats, void *stream) {

@@ -216,6 +216,16 @@ def _written(out):
         torch.autograd.graph.increment_version(out)
 
 
+def logit_ops_status(device=None) -> int:
+    """BS_ETIMEOUT if a bounded device wait of one of these operators gave up on
+    the device since the last such call, else BS_OK (bs_logit_ops_status).
+    Waits for the device."""
+    if torch is None:
+        _import_torch()
+    with torch.cuda.device(device):
+        return _s.lib().bs_logit_ops_status()
+
+
 def token_logprobs(logits, tokens, *, temperature: float = 1.0, final_logit_softcapping: float = 0.0,
                    logit_scale: float = 1.0, stream=None) -> TokenLogprobs:
     """Log-probability of each row's token and the row's entropy (bs_token_logprobs).

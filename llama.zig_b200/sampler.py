@@ -36,7 +36,7 @@ EXPORTS = [
     "bs_status_string", "bs_profile_enable", "bs_profile_read", "bs_argmax_ex", "bs_set_logit_prologue",
     "bs_sample_static", "bs_seed_state",
     "bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_top_logits_workspace",
-    "bs_distill_loss", "bs_policy_loss",
+    "bs_distill_loss", "bs_policy_loss", "bs_logit_ops_status",
 ]
 
 
@@ -152,8 +152,11 @@ def lib() -> ctypes.CDLL:
         L.bs_top_logits_workspace.restype = sz
         L.bs_distill_loss.argtypes = [vp, vp, f32p, f32p, u32, f32p, f32p, f32p, vp, sz, vp]
         L.bs_policy_loss.argtypes = [vp, vp, f32p, f32p, f32p, f32p, vp, f32p, f32p, f32p, f32p, f32p, vp, sz, vp]
+        L.bs_logit_ops_status.argtypes = []
+        L.bs_debug_logit_ops_waits.argtypes = [ctypes.c_uint64, u32, u32]
+        L.bs_debug_logit_ops_waits.restype = None
         for name in ("bs_token_logprobs", "bs_token_logprobs_grad", "bs_top_logits", "bs_distill_loss",
-                     "bs_policy_loss"):
+                     "bs_policy_loss", "bs_logit_ops_status"):
             getattr(L, name).restype = ctypes.c_int
         for name in ("bs_create", "bs_sample", "bs_sample_host", "bs_argmax", "bs_argmax_ex",
                      "bs_set_logit_prologue", "bs_get_rng_state",
