@@ -112,3 +112,53 @@ def test_soft_caps_at_the_ends_of_f32(gpu_pkg):
             assert abs(float(r.logprobs) + math.log(8.0)) <= 8 * 2.0**-24
             g = gpu_pkg.token_logprobs_grad(x, t, r, one, final_logit_softcapping=cap)
             assert bool(torch.isfinite(g).all()) and abs(float(g[0, 0]) - 0.875) <= 8 * 2.0**-24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("rows,vocab,ld,cap", [(1500, 1031, 1031, 0.0), (900, 8192, 8192, 0.0), (500, 40003, 40003, 0.0), (300, 128256, 128256, 0.0),
+                                               (60, 256000, 256001, 0.0), (20, 600000, 600000, 0.0), (300, 40003, 40003, 2.0),
+                                               (20, 600000, 600000, 2.0)])
+def test_gradients_over_the_logits_of_many_rows(gpu_pkg, dtype, rows, vocab, ld, cap):
+    """The gradient in place, rows going one after the other through the same blocks: what is loaded ahead (rows, tokens,
+    single elements, a teacher's logits) is read before another block writes over it, rows that do not fit on chip and
+    logits above a soft-cap are read again by whoever writes there.  The same bits as into a buffer of its own."""
+    off = 1 if ld % 8 else 0
+    g = torch.Generator(device="cuda").manual_seed(221)
+    base = torch.zeros(off + rows * ld, dtype=dtype, device="cuda")
+    src = 3.0 * torch.randn(rows, vocab, generator=g, device="cuda")
+
+    def fresh():
+        x = base[off:].view(rows, ld)[:, :vocab]
+        x.copy_(src)
+        return x
+
+    x = fresh()
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda").int()
+    t[::11] = 0                                    # single elements before and behind the chunks
+    t[5::11] = vocab - 1
+    t[torch.rand(rows, generator=g, device="cuda") < 0.1] = -1
+    w = torch.rand(rows, generator=g, device="cuda") + 0.5
+    w[torch.rand(rows, generator=g, device="cuda") < 0.2] = 0.0
+    w[rows // 3:rows // 2] = 0.0
+    one = torch.ones(rows, device="cuda")
+    tl, ids = torch.topk(src + torch.randn(rows, vocab, generator=g, device="cuda"), 40, dim=1)
+    ids = ids.int()
+    ids[::5, 1] = ids[::5, 0]                      # an id twice
+    ids[3::7] = -1                                 # no teacher
+    ids[2::9, 4] = vocab - 1
+    lse = torch.logsumexp(src, 1) + 0.1
+    calls = {
+        "policy": lambda x, out: gpu_pkg.policy_loss(x, t, -9 * one, one, -9 * one, w, kl_coef=0.01, entropy_coef=0.01,
+                                                     final_logit_softcapping=cap, out=out),
+        "slots": lambda x, out: gpu_pkg.distill_loss(x, ids, tl, None, w, final_logit_softcapping=cap, out=out),
+        "tail": lambda x, out: gpu_pkg.distill_loss(x, ids, tl, lse, w, final_logit_softcapping=cap, out=out),
+    }
+    for name, call in calls.items():
+        # (a buffer whose rows are aligned like the logits': a kernel's writes do not depend on it, its sums on the logits)
+        want = call(x, None)
+        for _ in range(2):
+            y = fresh()
+            got = call(y, y)
+            assert torch.equal(got.row_losses, want.row_losses), name
+            assert torch.equal(y, want.grad), (name, int((y != want.grad).sum()))
+        x = fresh()
