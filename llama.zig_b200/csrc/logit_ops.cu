@@ -168,7 +168,7 @@ template <bool CAP> __device__ __forceinline__ float2 cap_both(float v, const Sc
     return r;
 }
 
-// A streaming read: the line is the first to leave L2 (and L1) again.
+// A streaming read: not kept in L1.
 __device__ __forceinline__ uint4 ld_stream(const void *p) {
     uint4 q;
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -517,17 +517,19 @@ template <bool ENT> struct GradRow {
 // travel.  A warp that shares the SM with these issues an instruction in some
 // ten cycles, so B's 64-bit work is spread over four rows and meets no barrier
 // of its own: with the four warps together on one row 512 x 256000 f32 with 128
-// ids took 262 us, so 210; 4000 x 8000 bf16 with 64 ids 71 and 83.  Barriers, in as many copies as rows can be between the two sides:
+// ids took 262 us, so 214; 4000 x 8000 bf16 with 64 ids, where a row is short,
+// 71 and 88.  Barriers, in as many copies as rows can be between the two sides:
 // X (S -> A: row i summed), Y (A -> G: its coefficients), Z (-> C, B: done
 // with; from G, or without a gradient from S and A); and mbarriers: full_bar
 // (copy -> S), slots_bar (B -> S), mail_bar (A -> A of the other CTAs).
 //
 // Measured (policy loss and gradient, of the copy bandwidth for one read and
-// one write): 777 x 151936 f32 152 us, 95 %; 4096 x 128256 bf16 380 us, 79 %,
-// where the sums are what takes longest (4,500 cycles a slice of 32,000 logits
+// one write): 777 x 151936 f32 155 us, 93 %; 2048 x 128256 bf16 212 us, 76 %,
+// where the sums are what takes longest (4,700 cycles a slice of 32,000 logits
 // beside the gradient's 4,200; the copies take 4,900 a row on the 132 SMs that
-// clusters of four find, their own sum with nothing beside it 2,600).  Steps on
-// the way, 4096 x 128256 bf16: one CTA a row, read twice 523 us; clusters of
+// clusters of four find, their own sum with nothing beside it 2,600).  The 64-bit
+// scalars of a row, its lost-wait checks and sums by steps are 4 % of that: 205
+// us without.  Steps on the way, 4096 x 128256 bf16: one CTA a row, read twice 523 us; clusters of
 // small CTAs that keep the row 543; this pipeline with one set of warps for
 // both passes and copies by the threads 488, with bulk copies 441 (the threads'
 // copies stalled on the memory system's queue), sums and gradient by different
@@ -825,9 +827,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     // 2048 x 128256 bf16 409 and 387; policy loss 777 x 151936 f32 197 and 195, 2048 x 128256 bf16 388 and 398.
     constexpr int STEP = CAP && (DIST || sizeof(T) == 4) ? 2 : 4;
     auto row_of = [&](uint32_t i) { return cluster + i * clusters; };
-    auto weight = [&](uint32_t row) {
-        return OP == OP_LOGPROB ? 1.0f : A.weights ? A.weights[row] : A.w_all;
-    };
+    auto weight = [&](uint32_t row) { return A.weights ? A.weights[row] : A.w_all; };
     // the slice [c0, c1) of a row's chunks
     struct Slice {
         uint32_t c0, c1;
@@ -1417,7 +1417,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
 // forward pass's statistics:
 //   dv_j = m c'(v_j) [g (d_jt - p_j) - h p_j (log p_j + H)]
 // Grid: rows x slices of GRAD_SLICE chunks.  A pure stream, one read and one
-// write a logit: 2048 x 151936 bf16 (1792 rows read) 179 us, the copy bandwidth.
+// write a logit: 1024 x 151936 bf16 98 us, 97 % of the copy bandwidth; under a
+// soft-cap 124.
 // The token's element is worked out again in 64 bits (token_slope).
 __device__ __noinline__ float token_grad(const Scale &sc, float c, float2 st, float H, float g, float h) {
     const double lp = ((double)c - (double)st.x) * sc.md - (double)st.y;
@@ -1595,7 +1596,7 @@ template <typename T> __device__ __noinline__ void select_whole_row(const T *x, 
 // the logits themselves are searched.  A floor below very many equal values is
 // left where it is: the larger logits are taken and the rest filled up with the
 // lowest ids that have the value.  Measured, with k_stream before it: top 64 of
-// 256 x 128256 f32 38 us (10 of them here), top 256 of 1024 x 256000 bf16 133;
+// 256 x 128256 f32 38 us (10 of them here), top 256 of 1024 x 256000 bf16 136;
 // by a radix selection over the whole row 515 and 2015.
 struct TopArgs {
     uint32_t top;
@@ -1868,7 +1869,7 @@ __device__ __forceinline__ void select_top(const Row<T> &R, uint32_t row, const 
 // the rows' tokens, or (TOP) the rows' lse and the largest logit of each
 // 128-byte tile, from which CTA 0 of the row then selects.  Bound by HBM reads,
 // so many small CTAs with their loads under way at once; few rows are split
-// over clusters of CTAs.  Measured: 1792 live rows of 151936 bf16 91 us, 91 % of
+// over clusters of CTAs.  Measured: 1792 rows of 151936 bf16 94 us, 89 % of
 // the copy bandwidth (the persistent form of the losses' kernel took 129: one
 // CTA an SM has too few warps for a pass that only reads); 256 x 128256 f32
 // 27 us, 74 %, two waves of CTAs with their start and end.  Three or five CTAs
@@ -2130,7 +2131,7 @@ constexpr uint32_t STREAM_CTAS = 148 * 4;   // of k_stream that run at once
 // CTAs per row of k_stream: few rows still fill the GPU (four to an SM), no CTA
 // has less than two chunks a thread.  Measured, split against one CTA a row:
 // 1 x 128256 f32 6.2 and 12.8 us (the first is the launch), 64 rows 11.1 and
-// 20.6, 256 rows 27.2 and 26.7.
+// 20.6; at 256 rows it no longer matters (27.2 and 26.7).
 static uint32_t stream_log_ranks(uint32_t rows, uint32_t chunks) {
     uint32_t l = 0;
     while (l < 3 && ((uint64_t)rows << l) < STREAM_CTAS && (chunks >> (l + 1)) >= 2 * THREADS) l++;
