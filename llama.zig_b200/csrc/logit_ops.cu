@@ -119,8 +119,7 @@ __device__ __forceinline__ f2 floor2(f2 v) {   // at least D_MIN; a NaN stays
 // The last fused step rounds once, what comes before it is at most 0.31 of c: at
 // most 3.3 half steps in all, 0.75 root mean square, as cap * tanhf(v / cap) has.
 // Ten FMA-pipe slots for two logits.  Beyond, c = cap - cap 2 e / (1 + e) with
-// e = exp(-2 |v| / cap), the exponent with what its two roundings left off: at
-// most 3.7 half steps.
+// e = exp(-2 |v| / cap), the exponent rounded once: at most 3.9 half steps.
 __constant__ const float TANH_W[7] = {-0.33333295583724976f, 0.13332347571849823f, -0.0538799911737442f, 0.021487198770046234f,
                                       -0.007946893572807312f, 0.0023019297514110804f, -0.00035861122887581587f};
 __device__ __forceinline__ float rcp(float x) {
@@ -136,8 +135,8 @@ __device__ __forceinline__ f2 cap_near(f2 v, const Scale &sc) {
     return fma2(mul2(v, y), w, v);
 }
 __device__ __forceinline__ float cap_far(float v, const Scale &sc, float *slope = nullptr) {
-    const float a = fabsf(v), t = a * sc.k2;
-    const float e = a >= sc.most ? 0.0f : ex2(t) * fmaf(LN2, fmaf(a, sc.k2, -t) + a * sc.k2_lo, 1.0f);
+    const float a = fminf(fabsf(v), sc.most);
+    const float e = isinf(v) ? 0.0f : ex2(fmaf(a, sc.k2, a * sc.k2_lo));
     const float r = rcp(1.0f + e), q = 2.0f * e * r;
     if (slope) *slope = 2.0f * q * r;
     return copysignf(fmaf(-sc.cap, q, sc.cap), v);
@@ -166,6 +165,16 @@ template <bool CAP> __device__ __forceinline__ float2 cap_both(float v, const Sc
     r.y = slope2(both(r.x), sc).x;
     if (fabsf(v) > sc.cap) r.x = cap_far(v, sc, &r.y);
     return r;
+}
+
+// Two at once, the same operations.
+template <bool SLOPE> __device__ __forceinline__ f2 cap_far2(f2 v, const Scale &sc, f2 &slope) {
+    const f2 a = pair(fminf(fabsf(v.x), sc.most), fminf(fabsf(v.y), sc.most));
+    const f2 e = ex2_2(fma2(a, both(sc.k2), mul2(a, both(sc.k2_lo))));
+    const f2 n = add2(e, both(1.0f)), r = pair(rcp(n.x), rcp(n.y)), q = mul2(add2(e, e), r);
+    if (SLOPE) slope = mul2(add2(q, q), r);
+    const f2 c = fma2(both(-sc.cap), q, both(sc.cap));
+    return pair(copysignf(c.x, v.x), copysignf(c.y, v.y));
 }
 
 // A streaming read: not kept in L1.
@@ -274,46 +283,32 @@ struct Note {
         if (at) *at = stamp;
     }
 };
-// A chunk's logits after the soft-cap.
-template <typename T, bool CAP>
-__device__ __forceinline__ void cap_chunk(const uint4 &q, f2 (&v)[8 / sizeof(T)], const Scale &sc, const Note &note) {
+// A chunk's logits after the soft-cap, and (SLOPE) its slopes there.  LEFT: q
+// holds c(v) where |v| <= cap and v beyond (|c| is below 0.77 cap on the one side).
+template <typename T, bool CAP, bool SLOPE = false, bool LEFT = false>
+__device__ __forceinline__ void cap_chunk(const uint4 &q, f2 (&v)[8 / sizeof(T)], const Scale &sc, const Note &note, f2 *slopes = nullptr) {
     unpack<T>(q, v);
     if (!CAP) return;
     constexpr int N = 8 / sizeof(T);
     const bool far = max_abs<T>(q) > sc.cap;
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = cap_near(v[i], sc);
+    for (int i = 0; i < N; i++) {
+        if (!LEFT) v[i] = cap_near(v[i], sc);
+        if (SLOPE) slopes[i] = slope2(v[i], sc);
+    }
     if (far) {
         note.put();
         f2 raw[N];
         unpack<T>(q, raw);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (fabsf(raw[i].x) > sc.cap) v[i].x = cap_far(raw[i].x, sc);
-            if (fabsf(raw[i].y) > sc.cap) v[i].y = cap_far(raw[i].y, sc);
+            f2 slope;
+            const f2 c = cap_far2<SLOPE>(raw[i], sc, slope);
+            const bool x = fabsf(raw[i].x) > sc.cap, y = fabsf(raw[i].y) > sc.cap;
+            v[i] = pair(x ? c.x : v[i].x, y ? c.y : v[i].y);
+            if (SLOPE) slopes[i] = pair(x ? slope.x : slopes[i].x, y ? slope.y : slopes[i].y);
         }
     }
-}
-// A chunk's elements one after the other through f: little code and few
-// registers, for what is rare.
-template <typename T, typename F> __device__ __forceinline__ uint4 each_of(uint4 q, F f) {
-    uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll 1
-    for (int e = 0; e < (int)(16 / sizeof(T)); e++) {
-        // (the lowest element out, the result in at the top)
-        uint32_t in;
-        if constexpr (sizeof(T) == 4) {
-            in = __float_as_uint(f(__uint_as_float(w[0])));
-            w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = in;
-        } else {
-            float a, b;
-            halves(widen(w[0], T()), a, b);
-            in = narrow(pair(f(a), 0.0f), T());
-            w[0] = __funnelshift_r(w[0], w[1], 16), w[1] = __funnelshift_r(w[1], w[2], 16), w[2] = __funnelshift_r(w[2], w[3], 16);
-            w[3] = w[3] >> 16 | in << 16;
-        }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // What a thread writes of a chunk where 16-byte stores do not fit.
 template <typename T> __device__ __forceinline__ void store_each(T *g, const uint4 &q) {
@@ -458,30 +453,34 @@ template <bool ENT> struct GradRow {
         const float l = fmaf(c - m, k, -l2s), p = ex2(l);
         return ENT ? p * fmaf(cb, max_nan(l, D_MIN), ca) : p * ca;
     }
-    // A chunk of it.
-    template <typename T, bool CAP> __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
-        if (CAP && max_abs<T>(q) > sc.cap)
-            return each_of<T>(q, [&](float v) {
-                const float2 c = cap_both<CAP>(v, sc);
-                return one(c.x) * c.y;
-            });
-        return near<T, CAP>(q, sc);
+    // A chunk of it (LEFT: as cap_chunk).
+    template <typename T, bool CAP, bool LEFT = false> __device__ __forceinline__ uint4 chunk(const uint4 &q, const Scale &sc) const {
+        constexpr int N = 8 / sizeof(T);
+        f2 v[N], slopes[N];
+        cap_chunk<T, CAP, CAP, LEFT>(q, v, sc, Note{}, slopes);
+        return from<T, CAP>(v, slopes);
     }
     // The same where no logit lies above the soft-cap; DONE: q holds c(v) already.
     template <typename T, bool CAP, bool DONE = false>
     __device__ __forceinline__ uint4 near(const uint4 &q, const Scale &sc) const {
         constexpr int N = 8 / sizeof(T);
-        f2 v[N], o[N];
+        f2 v[N], slopes[N];
         unpack<T>(q, v);
 #pragma unroll
         for (int i = 0; i < N; i++) {
             if (CAP && !DONE) v[i] = cap_near(v[i], sc);
+            if (CAP) slopes[i] = slope2(v[i], sc);
+        }
+        return from<T, CAP>(v, slopes);
+    }
+    template <typename T, bool CAP>
+    __device__ __forceinline__ uint4 from(const f2 (&v)[8 / sizeof(T)], const f2 (&slopes)[8 / sizeof(T)]) const {
+        f2 o[8 / sizeof(T)];
+#pragma unroll
+        for (int i = 0; i < (int)(8 / sizeof(T)); i++) {
             const f2 l = fma2(add2(v[i], both(-m)), both(k), both(-l2s));
             o[i] = mul2(ex2_2(l), ENT ? fma2(both(cb), floor2(l), both(ca)) : both(ca));
-        }
-        if (CAP) {
-#pragma unroll
-            for (int i = 0; i < N; i++) o[i] = mul2(o[i], slope2(v[i], sc));
+            if (CAP) o[i] = mul2(o[i], slopes[i]);
         }
         return pack<T>(o);
     }
@@ -912,10 +911,20 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                     const uint32_t b = c * E;
                     return bits[b >> 5] >> (b & 31) & ((1u << E) - 1u);
                 };
-                auto capped_chunk = [&](const uint4 &q) {
+                // (LEAVE: c(v), and into the buffer what G starts from: v itself beyond the cap, for its slope)
+                auto capped_chunk = [&](const uint4 &q, uint4 *left) {
                     f2 v[E / 2];
                     cap_chunk<T, CAP>(q, v, A.sc, note);
-                    return pack<T>(v);
+                    const uint4 c = pack<T>(v);
+                    if (grad) {
+                        *left = c;
+                        if (max_abs<T>(q) > A.sc.cap) {
+                            const float cap = A.sc.cap;
+                            *left = make_uint4(fabsf(__uint_as_float(q.x)) > cap ? q.x : c.x, fabsf(__uint_as_float(q.y)) > cap ? q.y : c.y,
+                                               fabsf(__uint_as_float(q.z)) > cap ? q.z : c.z, fabsf(__uint_as_float(q.w)) > cap ? q.w : c.w);
+                        }
+                    }
+                    return c;
                 };
                 // (a chunk's named tokens left out)
                 auto leave_out = [&](uint4 &q, uint32_t mk) {
@@ -933,8 +942,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                         // (the soft-cap of all of them first: that of the largest alone would be waited for)
 #pragma unroll
                         for (int u = 0; u < STEP; u++) {
-                            q[u] = capped_chunk(q[u]);
-                            if (grad) buf[u * sum_threads] = q[u];
+                            q[u] = capped_chunk(q[u], buf + u * sum_threads);
                             if (mk[u]) mask_out<T>(q[u], mk[u]);
                         }
                         G.raise(max_of<T>(q), k);
@@ -958,7 +966,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 for (; c < copied; c += sum_threads, buf += sum_threads) {
                     uint4 q = buf[0];
                     const uint32_t mk = marks(c);
-                    if (LEAVE && grad) buf[0] = capped_chunk(q);
+                    if constexpr (LEAVE) capped_chunk(q, buf);
                     if (mk) leave_out(q, mk);
                     G.raise(capped<CAP>(max_of<T>(q), A.sc), k);
                     G.chunk(q, A.sc, mk, mk ? none : note);
@@ -1013,11 +1021,10 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
                 const T *x = R.at(sl.c0);
                 if (CAP && __builtin_expect(sh.far[i & 3] == i + 1, 0)) {
-                    // (under LEAVE the logits themselves are needed: no other thread writes over this one's chunks)
-#pragma unroll 1
-                    for (uint32_t c = g; c < copied; c += GT, buf += GT)
-                        store(c, gr.template chunk<T, CAP>(LEAVE ? ld_stream(x + (size_t)c * E) : *buf, A.sc));
-#pragma unroll 1
+                    // (777 x 151936 f32, cap 30: 196 us without such logits, 249 with 16 a row, 402 with half of them; 2048 x
+                    // 128256 bf16 394, 425, 677)
+#pragma unroll 2
+                    for (uint32_t c = g; c < copied; c += GT, buf += GT) store(c, gr.template chunk<T, CAP, LEAVE>(*buf, A.sc));
                     for (uint32_t c = copied + g; c < count; c += GT) store(c, gr.template chunk<T, CAP>(ld_stream(x + (size_t)c * E), A.sc));
                 } else {
                     if (wide) {
@@ -2040,7 +2047,7 @@ static bs_status check_logits(const bs_logits *x, Scale *sc, float *out_scale, b
     const double k2 = fmax(-2.0 * 1.4426950408889634 / (double)sc->cap, -3.4e38);
     sc->k2 = (float)k2;
     sc->k2_lo = (float)(k2 - (double)sc->k2);
-    sc->most = 64.0f * sc->cap;
+    sc->most = (float)fmin(fmax(64.0 * (double)sc->cap, 6e-37), 3.4e38);   // (2^(most k2) is 0)
     *out_scale = (float)(1.0 / scale);
     return BS_OK;
 }

@@ -242,8 +242,8 @@ def test_gradient_where_the_soft_cap_saturates(gpu_pkg, dtype, vocab, off):
     half, tiny = torch.finfo(dtype).eps / 2, (2.0**-25 if dtype == torch.float16 else 2.0**-126)
 
     def check(got, pre, size, what):
-        # the slope: t twice (4 half steps each) on at most 0.58 of it, over 0.42; beyond, the exponential's 5 and the
-        # quotient's 4, twice: 20 half steps with the products
+        # the slope: t twice (4 half steps each) on at most 0.58 of it, over 0.42; beyond, the exponent's rounding (18 at
+        # 9 cap, 16 here), the exponential's 4 and the quotient's 4, twice: 30 half steps with the products
         out = pre * slope
         tol = slope * (delta * size + 40 * EPS * size) + 1.01 * half * out.abs() + tiny
         bad = (got.double() - out).abs() > tol
