@@ -56,6 +56,7 @@ struct RowArgs {
     uint32_t bit_words;         // with a teacher: words of one bit per element of a slice
     Scale sc;
     const int32_t *tokens;
+    uint32_t zero;              // 0, which the compiler does not know
     long long wait_limit;       // clock cycles
     uint32_t gone_rank, gone_row;   // (for tests) the CTA of a row whose waits give up, from a cluster's i-th row on
     // outputs (null where not asked for)
@@ -358,8 +359,11 @@ template <typename T> struct Row {
 };
 
 // Running (M, S, U) of a set of logits.
-struct Stat {
-    float m, s, u;
+// S is kept in 64 bits from a warp's lanes on: the dozen additions that
+// fold a row would each round off half a step of 1 beside its largest logit.
+struct __align__(16) Stat {
+    double s;
+    float m, u;
 };
 // A maximum of -inf (all of the set masked) is replaced by 0 in differences,
 // so that the masked logits give 2^-inf = 0.
@@ -416,7 +420,7 @@ template <typename T, bool CAP, bool ENT> struct Gather {
         float a, b, c, d;
         halves(s, a, b);
         halves(u, c, d);
-        return Stat{m, a + b, c + d};
+        return Stat{(double)a + (double)b, m, c + d};
     }
 };
 
@@ -434,16 +438,11 @@ __device__ __forceinline__ uint32_t remote(const void *p, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void st_remote4(uint32_t addr, float a, float b, float c) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %1};" ::"r"(addr), "f"(a), "f"(b), "f"(c) : "memory");
-}
-
-// log2 S as exponent + log2 of the mantissa: exact to 2^-24 for any S.
-__device__ __forceinline__ double log2_d(float s) {
-    if (!(s > 0.0f) || isinf(s)) return (double)log2f(s);
-    int e;
-    float f = frexpf(s, &e);
-    return (double)e + (double)log2f(f);
+// A Stat into a shared variable of another CTA.
+__device__ __forceinline__ void st_remote(uint32_t addr, const Stat &a) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(__double2loint(a.s)),
+                 "r"(__double2hiint(a.s)), "r"(__float_as_uint(a.m)), "r"(__float_as_uint(a.u))
+                 : "memory");
 }
 
 // The gradient of one row: c'(v_j) p_j (ca + cb log2 p_j), log2 p_j = d_j - log2 S.
@@ -584,8 +583,8 @@ template <typename T, bool CAP> __host__ __device__ constexpr int sum_threads_of
     return CAP && sizeof(T) == 4 ? 384 : compute_threads<T>() / 2;
 }
 struct RowsShared {
-    float4 part[4][MAX_CWARPS];          // (m, s, u) of the warps S
-    float4 mail[4][MAX_CLUSTER];     // and of the row's CTAs; two for each warp A
+    Stat part[4][MAX_CWARPS];        // of the warps S; m is NaN where one gave up on its copy
+    uint4 mail[4][MAX_CLUSTER];      // and of the row's CTAs; two for each warp A
     Coef coef[4];
     uint32_t far[4];                 // i + 1: row i has a logit above the soft-cap in the slice
     uint32_t gone;                   // a wait of this CTA gave up
@@ -605,8 +604,8 @@ template <bool ENT, int W> __device__ __forceinline__ Stat fold_lanes(Stat a, fl
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     const float d = fmaxf((a.m - m) * k, D_MIN), f = ex2(d);
-    if (ENT) a.u = f * fmaf(d, a.s, a.u);
-    a.s *= f;
+    if (ENT) a.u = f * fmaf(d, (float)a.s, a.u);
+    a.s *= (double)f;
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) {
         a.s += __shfl_xor_sync(~0u, a.s, o);
@@ -628,10 +627,10 @@ __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive_local(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ void mail_send(const float4 *slot, const uint64_t *bar, uint32_t rank, const float4 &v) {
+__device__ __forceinline__ void mail_send(const uint4 *slot, const uint64_t *bar, uint32_t rank, const uint4 &v) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %5}, [%4];" ::"r"(
                      remote(slot, rank)),
-                 "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(remote(bar, rank)), "r"(__float_as_uint(v.w))
+                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(remote(bar, rank)), "r"(v.w)
                  : "memory");
 }
 // Takes bytes off what a phase waits for: those that nobody will send.
@@ -705,9 +704,9 @@ template <int N> __device__ __forceinline__ void by_lanes(double (&v)[N], double
 template <int OP>
 __device__ __forceinline__ Coef token_row(const RowArgs &A, uint32_t row, const Stat &st, const TokenIn &in, bool write) {
     // (u / s by one Newton step on the f32 reciprocal: 2^-46)
-    const double m = st.m, rs = (double)(1.0f / st.s), ratio = (double)st.u * (rs * (2.0 - (double)st.s * rs));
+    const double m = st.m, rs = (double)(1.0f / (float)st.s), ratio = (double)st.u * (rs * (2.0 - st.s * rs));
     // k is m log2 e in f32: to first order, what its rounding did to the sum
-    const double ln_s = log((double)st.s) + LN2_D * A.sc.dk * ratio;
+    const double ln_s = log(st.s) + LN2_D * A.sc.dk * ratio;
     const double lp = ((double)in.c_tok - m) * A.sc.md - ln_s;
     const double H = ln_s - LN2_D * (1.0 + A.sc.dk) * ratio;
     Coef c{st.m, (float)(ln_s * (1.0 / LN2_D)), 0.0f, 0.0f, 0.0f, 1u, 0.0, 0.0, 0.0};
@@ -766,7 +765,7 @@ template <bool TAIL>
 __device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, const Stat &st, double top, const Teacher &t, float w,
                                             bool write) {
     const double wm = (double)w * A.sc.md, u = (double)anchor(t.u);
-    double s = (double)st.s, big = (double)st.m, below = 1.0;
+    double s = st.s, big = (double)st.m, below = 1.0;
     if (TAIL) {
         const double d = ((double)st.m - (double)t.u) * A.sc.md, e = exp_d(-fabs(d));
         if (d >= 0.0) {
@@ -778,14 +777,14 @@ __device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, cons
         }
     }
     const double qr = 1.0 - t.mass;
-    double ln[3] = {s, (double)st.s, qr};
+    double ln[3] = {s, st.s, qr};
     if (TAIL) by_lanes(ln, [](double v) { return log(v); });
     else ln[0] = log(s);
     const double lse = (big - u) * A.sc.md + ln[0];   // relative to U
     double loss = t.cross + t.mass * lse, mass = t.mass;
     Coef c{st.m, (float)(ln[TAIL ? 1 : 0] * (1.0 / LN2_D)), 0.0f, 0.0f, 0.0f, 1u, lse, 0.0, wm};
     if (TAIL) {   // the rest as one outcome
-        if (st.s == 0.0f) {
+        if (st.s == 0.0) {
             c.m = c.l2s = 0.0f;
         } else {
             const bool has = !(qr <= 0.0);
@@ -793,7 +792,7 @@ __device__ __forceinline__ Coef teacher_row(const RowArgs &A, uint32_t row, cons
                 loss += qr * (ln[2] - (((double)st.m - big) * A.sc.md + ln[1] - ln[0]));
                 mass += qr;
             }
-            c.ca = (float)(wm * (mass * ((double)st.s * below / s) - (has ? qr : 0.0)));
+            c.ca = (float)(wm * (mass * (st.s * below / s) - (has ? qr : 0.0)));
         }
     } else {
         c.ca = (float)(wm * mass);
@@ -992,9 +991,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             }
             // (the buffer is written by copies again)
             if (LEAVE && grad) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            Stat st{-INFINITY, 0.0f, 0.0f};
+            Stat st{0.0, -INFINITY, 0.0f};
             if (there && sh.code[i & 15] >= 0) st = fold_lanes<!DIST, 32>(G.stat(), k);
-            if (lane == 0) sh.part[i & 3][tid >> 5] = make_float4(st.m, st.s, st.u, there ? 0.0f : 1.0f);
+            if (lane == 0) sh.part[i & 3][tid >> 5] = Stat{st.s, there ? st.m : NAN, st.u};
             bar_arrive(BAR_X + (i & 3), x_threads);
             if (!grad) bar_arrive(BAR_Z + (i & 3), z_threads);
         }
@@ -1111,14 +1110,9 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
             const int32_t edge = edge_of(i);
             const float c_edge = capped<CAP>(to_f(cur.edge), A.sc);
             const float c_tok = DIST ? 0.0f : capped<CAP>(to_f(cur.tok), A.sc);
-            Stat st{-INFINITY, 0.0f, 0.0f};
-            bool gave_up = false;
-            if (lane < sum_threads / 32) {
-                const float4 f = sh.part[i & 3][lane];
-                st = Stat{f.x, f.y, f.z};
-                gave_up = f.w != 0.0f;
-            }
-            stopped = __any_sync(~0u, gave_up || stopped);
+            Stat st{0.0, -INFINITY, 0.0f};
+            if (lane < sum_threads / 32) st = sh.part[i & 3][lane];
+            stopped = __any_sync(~0u, st.m != st.m || stopped);
             const bool wanted = sh.code[i & 15] >= 0;
             bool lost = wanted && stopped, live = wanted && !lost;
             if (DIST && live) live = sh.teacher[i & 3].live != 0u;
@@ -1128,7 +1122,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 const float one = c_edge == -INFINITY ? 0.0f : c_edge - c_edge == 0.0f ? 1.0f : NAN;
                 const float m = c_edge != c_edge ? st.m : fmaxf(st.m, c_edge);
                 const float da = fmaxf((st.m - m) * k, D_MIN), db = fmaxf((c_edge - m) * k, D_MIN), fa = ex2(da), fb = ex2(db);
-                st = Stat{m, st.s * fa + one * fb, fa * fmaf(da, st.s, st.u) + fb * (db * one)};
+                st = Stat{st.s * fa + (double)(one * fb), m, fa * fmaf(da, (float)st.s, st.u) + fb * (db * one)};
             }
             st = fold_lanes<!DIST, 32>(st, k);
             double top = TAIL && live ? sh.teacher[i & 3].top : 0.0;
@@ -1139,19 +1133,23 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 // write the gradient over it.
                 const uint32_t box = which * 2 + (sent & 1), turn = sent >> 1 & 1;
                 sent++;
-                float4 out = make_float4(st.m, st.s, st.u, c_tok);
-                if (TAIL) out.z = __int_as_float(__double2loint(top)), out.w = __int_as_float(__double2hiint(top));
+                const double big = TAIL ? top : st.s;   // (with a tail the named ids' sum has the 64 bits, the rest's 32)
+                const float small = TAIL ? (float)st.s : st.u;
+                uint4 out = make_uint4(__double2loint(big), __double2hiint(big), __float_as_uint(st.m), __float_as_uint(small));
+                if (!DIST) out.x |= __float_as_uint(c_tok) & A.zero;
                 if (lane < ranks) mail_send(&sh.mail[box][rank], &sh.mail_bar[box], lane, out);
                 if (lane == 0) bar_expect(&sh.mail_bar[box], ranks * 16);
                 lost = !__all_sync(~0u, wait(&sh.mail_bar[box], turn, i));
                 live = live && !lost;
                 failed = stopped = lost;
-                st = Stat{-INFINITY, 0.0f, 0.0f};
+                st = Stat{0.0, -INFINITY, 0.0f};
                 top = 0.0;
                 if (lane < ranks) {
-                    const float4 f = sh.mail[box][lane];
-                    st = Stat{f.x, f.y, f.z};
-                    if (TAIL) top = __hiloint2double(__float_as_int(f.w), __float_as_int(f.z));
+                    const uint4 f = sh.mail[box][lane];
+                    const double big = __hiloint2double(f.y, f.x);
+                    const float small = __uint_as_float(f.w);
+                    st = Stat{TAIL ? (double)small : big, __uint_as_float(f.z), TAIL ? 0.0f : small};
+                    if (TAIL) top = big;
                 }
                 if (TAIL) {
                     for (int o = MAX_CLUSTER / 2; o; o >>= 1) top += __shfl_xor_sync(~0u, top, o);
@@ -1883,8 +1881,7 @@ __device__ __forceinline__ void select_top(const Row<T> &R, uint32_t row, const 
 // an SM: 97 and 95 us.
 constexpr int BATCH = 8;             // 16-byte loads of a thread under way before the first is used
 struct StreamShared {
-    Stat warp[WARPS];
-    float4 cta[8];
+    Stat warp[WARPS], cta[8];
 };
 template <typename T, bool CAP, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
@@ -1978,25 +1975,24 @@ __global__ void __launch_bounds__(THREADS, 4) k_stream(RowArgs A, TopArgs P) {
     if (lane == 0) sh.warp[tid >> 5] = st;
     __syncthreads();
     if (tid < 32) {
-        st = lane < WARPS ? sh.warp[lane] : Stat{-INFINITY, 0.0f, 0.0f};
+        st = lane < WARPS ? sh.warp[lane] : Stat{0.0, -INFINITY, 0.0f};
         st = fold_lanes<!TOP, 32>(st, k);
     }
     if (ranks > 1) {
         cluster_wait();
-        if (tid == 0) st_remote4(remote(&sh.cta[rank], 0), st.m, st.s, st.u);
+        if (tid == 0) st_remote(remote(&sh.cta[rank], 0), st);
         __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (tid < 32) {
-            const float4 f = lane < ranks ? sh.cta[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-            st = fold_lanes<!TOP, 32>(Stat{f.x, f.y, f.z}, k);
+            st = fold_lanes<!TOP, 32>(lane < ranks ? sh.cta[lane] : Stat{0.0, -INFINITY, 0.0f}, k);
         }
     }
     if (rank != 0) return;
     if constexpr (TOP) {
         // (the barriers above also made the tile maxima of all CTAs visible to this one)
         __shared__ TopShared ts;
-        if (tid == 0) P.lse[row] = (float)((double)st.m * (double)A.sc.m + LN2_D * log2_d(st.s));
+        if (tid == 0) P.lse[row] = (float)((double)st.m * A.sc.md + log(st.s));
         if (P.fused) select_top<T, CAP>(R, row, A.sc, P, ts, keys);
     } else if (tid == 0) {
         token_row<OP_LOGPROB>(A, row, st, TokenIn{1.0f, 0.0f, 0.0f, 0.0f, capped<CAP>(to_f(v_tok), A.sc), 1.0f}, true);

@@ -298,3 +298,26 @@ def test_small_terms_beside_a_large_one(gpu_pkg, dtype, rows):
     one = torch.ones(rows, device="cuda")
     p = gpu_pkg.policy_loss(x, at.int(), 0 * one, one, None, one, temperature=T)
     assert float((p.logprobs.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,vocab", [(1, 131072), (3, 40000), (600, 131072), (700, 8192)])
+def test_a_very_likely_token(gpu_pkg, dtype, rows, vocab):
+    """ln S of S = 1 + some 1e-5: what the fold of a row's sums would round away beside the 1."""
+    # d is a whole number and every term a power of two, as above; the small ones keep off the elements that the large one's
+    # thread would sum by itself (the first chunk of each step), where they meet it in f32
+    T = float(np.float32(1.0 / math.log(2.0)))
+    at = [p for p in range(100, vocab, 53) if min(p % 1024, p % 2048, p % 2560, p % 4096) >= 16][:500]
+    x = torch.full((rows, vocab), -math.inf, dtype=dtype, device="cuda")
+    x[:, 0] = 0.0
+    x[:, at] = -25.0
+    want = math.log1p(len(at) * math.exp(-25.0 / T))
+    t = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    one = torch.ones(rows, device="cuda")
+    # the result's rounding, 64 bits before it; the correction of k's rounding goes to first order
+    relative(gpu_pkg.token_logprobs(x, t, temperature=T).logprobs, [-want] * rows, 2 * EPS, "log-probability")
+    # (without the entropy's sum there is no correction: k is off by half a step at most, which a term of d = -25 feels
+    # 25 ln 2 = 17.4 times)
+    relative(gpu_pkg.top_logits(x, 3, temperature=T).lse, [want] * rows, (2 + 17.4) * EPS, "lse")
+    p = gpu_pkg.policy_loss(x, t, 0 * one, one, None, one, temperature=T)
+    relative(p.logprobs, [-want] * rows, 2 * EPS, "log-probability of the policy loss")
