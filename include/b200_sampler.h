@@ -247,8 +247,8 @@ bs_status bs_sample_static(const bs_config *cfg, uint64_t *d_rng, const float *d
  *     p_j = exp(z_j - lse),            lse = log sum_j exp(z_j),
  * and are stream-ordered: the pointers' device must be the current one, and
  * a call returns once the work is enqueued.  They hold no state, so any
- * number of calls may run at once.  The sums are f32, in an order fixed by
- * the sizes and the alignment: the same call gives the same bits.
+ * number of calls may run at once.  The sums are f32, folded in f64, in an
+ * order fixed by the sizes and the alignment: the same call gives the same bits.
  *
  * Logits of -inf are masked tokens (p = 0, gradient 0), a +inf logit makes its
  * row NaN, a row all of -inf has no distribution and is NaN too, with an lse of

@@ -515,19 +515,19 @@ template <bool ENT> struct GradRow {
 // travel.  A warp that shares the SM with these issues an instruction in some
 // ten cycles, so B's 64-bit work is spread over four rows and meets no barrier
 // of its own: with the four warps together on one row 512 x 256000 f32 with 128
-// ids took 262 us, so 214; 4000 x 8000 bf16 with 64 ids, where a row is short,
-// 71 and 88.  Barriers, in as many copies as rows can be between the two sides:
+// ids took 262 us, so 219; 4000 x 8000 bf16 with 64 ids, where a row is short,
+// 71 and 89.  Barriers, in as many copies as rows can be between the two sides:
 // X (S -> A: row i summed), Y (A -> G: its coefficients), Z (-> C, B: done
 // with; from G, or without a gradient from S and A); and mbarriers: full_bar
 // (copy -> S), slots_bar (B -> S), mail_bar (A -> A of the other CTAs).
 //
 // Measured (policy loss and gradient, of the copy bandwidth for one read and
-// one write): 777 x 151936 f32 155 us, 93 %; 2048 x 128256 bf16 212 us, 76 %,
+// one write): 777 x 151936 f32 157 us, 92 %; 2048 x 128256 bf16 214 us, 75 %,
 // where the sums are what takes longest (4,700 cycles a slice of 32,000 logits
 // beside the gradient's 4,200; the copies take 4,900 a row on the 132 SMs that
-// clusters of four find, their own sum with nothing beside it 2,600).  The 64-bit
-// scalars of a row, its lost-wait checks and sums by steps are 4 % of that: 205
-// us without.  Steps on the way, 4096 x 128256 bf16: one CTA a row, read twice 523 us; clusters of
+// clusters of four find, their own sum with nothing beside it 2,600).  A row's
+// scalars and folds in 64 bits, its checked waits and sums by steps are 4 % of
+// that: 205 us without.  Steps on the way, 4096 x 128256 bf16: one CTA a row, read twice 523 us; clusters of
 // small CTAs that keep the row 543; this pipeline with one set of warps for
 // both passes and copies by the threads 488, with bulk copies 441 (the threads'
 // copies stalled on the memory system's queue), sums and gradient by different
