@@ -118,8 +118,8 @@ __device__ __forceinline__ f2 floor2(f2 v) {   // at least D_MIN; a NaN stays
 // logits are, c = v + v y W(y) with y = (v / cap)^2 and W a polynomial: the least
 // largest relative error of c over y in [0, 1] with f32 coefficients, 4.7e-9.
 // The last fused step rounds once, what comes before it is at most 0.31 of c: at
-// most 3.3 half steps in all, 0.75 root mean square, as cap * tanhf(v / cap) has.
-// Ten FMA-pipe slots for two logits.  Beyond, c = cap - cap 2 e / (1 + e) with
+// most 3.3 half steps in all, 0.45 root mean square on the workloads' logits, where
+// cap * tanhf(v / cap) has 1.3.  Ten FMA-pipe slots for two logits.  Beyond, c = cap - cap 2 e / (1 + e) with
 // e = exp(-2 |v| / cap), the exponent rounded once: at most 3.9 half steps.
 __constant__ const float TANH_W[7] = {-0.33333295583724976f, 0.13332347571849823f, -0.0538799911737442f, 0.021487198770046234f,
                                       -0.007946893572807312f, 0.0023019297514110804f, -0.00035861122887581587f};
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
     const uint32_t sum_threads = grad ? ST : COMPUTE, x_threads = sum_threads + 32;
     const uint32_t y_threads = GT + 32;
     const uint32_t z_threads = (grad ? GT : COMPUTE + 32) + 32 + (DIST ? 32 : 0);
-    // f32 logits under a soft-cap: S leaves c(v) in the buffer, so that G need not work it out again
+    // f32 logits under a soft-cap: S leaves c(v) in the buffer, so that G need not work it out again (v above the cap)
     constexpr bool LEAVE = CAP && sizeof(T) == 4;
     // Chunks of a thread summed at a time.  Under a soft-cap, with 4 and 2: distillation 512 x 256000 f32 326 and 291 us,
     // 2048 x 128256 bf16 409 and 387; policy loss 777 x 151936 f32 197 and 195, 2048 x 128256 bf16 388 and 398.
@@ -1020,8 +1020,8 @@ __global__ void __launch_bounds__(row_threads(OP, compute_threads<T>()), 1) k_ro
                 const GradRow<OP == OP_POLICY_ENT> gr{cf.m, k, cf.l2s, cf.ca, cf.cb};
                 const T *x = R.at(sl.c0);
                 if (CAP && __builtin_expect(sh.far[i & 3] == i + 1, 0)) {
-                    // (777 x 151936 f32, cap 30: 196 us without such logits, 249 with 16 a row, 402 with half of them; 2048 x
-                    // 128256 bf16 394, 425, 677)
+                    // logits above the soft-cap (777 x 151936 f32, cap 30: 198 us without, 249 with 16 a row, 405 with half of
+                    // all; 2048 x 128256 bf16 401, 430, 682)
 #pragma unroll 2
                     for (uint32_t c = g; c < copied; c += GT, buf += GT) store(c, gr.template chunk<T, CAP, LEAVE>(*buf, A.sc));
                     for (uint32_t c = copied + g; c < count; c += GT) store(c, gr.template chunk<T, CAP>(ld_stream(x + (size_t)c * E), A.sc));
